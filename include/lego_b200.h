@@ -29,6 +29,7 @@ extern "C" {
 #define LEGO_MAX_STAGES   8   /* OrderBy stages in one GroupBy                          */
 #define LEGO_MAX_TERMS   32   /* digits of a folded layout                              */
 #define LEGO_MAX_GROUPS 256   /* problems in one grouped GEMM call                      */
+#define LEGO_MAX_DRAFT   64   /* drafted tokens of one sequence in tree attention      */
 #define LEGO_MAX_LUT (1 << 24) /* entries of one table-driven (LUT) permutation block   */
 
 /* status codes */
@@ -388,6 +389,103 @@ int32_t lego_grouped_gemm_f16_static(const void* const* A, const void* const* B,
                                      const int64_t* mnk, int32_t G,
                                      const lego_layout_t* const* tile_orders, uint32_t* dev_status,
                                      void* stream);
+
+/* ---- attention ------------------------------------------------------------ */
+
+/* element types of the operators below */
+enum { LEGO_F16 = 0, LEGO_BF16 = 1, LEGO_F32 = 2 };
+
+/* where the two values of a rotary pair p of R / 2 stand in the first R values of a head:
+ * half: p and p + R / 2 (the layout Col(R / 2, 2)); interleaved: 2 p and 2 p + 1
+ * (Row(R / 2, 2)).                                                              */
+enum { LEGO_PAIRS_HALF = 0, LEGO_PAIRS_INTERLEAVED = 1 };
+
+/* Rotary positions of up to two tensors [batch, length, heads[i], head_dim] in one launch
+ * (queries and keys; heads[1] = 0: one tensor).  Pair p of a token at position s turns by
+ * the angle s * freqs[p] and is multiplied by `scale`:
+ *   y1 = scale (x1 cos - x2 sin),  y2 = scale (x2 cos + x1 sin);
+ * inverse != 0 turns back by the same angle, which is the gradient's way.  The values from
+ * rotary_dim on are copied.  Angles are taken in 64 bits, the rotation in 32, one rounding
+ * at the end.  Strides are in elements (batch, token, head; the last axis is contiguous);
+ * outputs are contiguous.  positions: dev int32 or int64 (position_bytes 4 or 8) read at
+ * [b * position_stride[0] + s * position_stride[1]]; freqs: dev double[rotary_dim / 2].
+ * No counterpart in the reference.                                              */
+typedef struct lego_rotary {
+  int32_t dtype, pairs, inverse, position_bytes;
+  int64_t batch, length, head_dim, rotary_dim;
+  int64_t heads[2];
+  int64_t stride[2][3];
+  int64_t position_stride[2];
+  float scale;
+  int32_t reserved;
+} lego_rotary_t;
+
+int32_t lego_rotary(const lego_rotary_t* desc, const void* x0, const void* x1, void* y0, void* y1,
+                    const void* positions, const double* freqs, void* stream);
+
+/* Attention of q [batch, q_len, q_heads, head_dim] over k, v [batch, k_len, k_heads, head_dim],
+ * fp16 or bf16.  Query head h reads key head h / (q_heads / k_heads).  Query i stands at
+ * position i + k_len - q_len of the keys (the last queries face the last keys).  Scores
+ *   s = softcap * tanh(scale q.k / softcap) - slopes[h] |position - j|
+ * (softcap 0: none; slopes NULL: none).  Key j is seen by the query at position p if
+ *   (not causal, or j <= p, or j < prefix[batch]) and documents[p] == documents[j] >= 0
+ * (prefix, documents NULL: no such condition; documents needs q_len <= k_len; document
+ * numbers may come in any order, runs of equal ones are what makes the call fast).  A query
+ * that sees nothing gets zeros and lse = -inf, and no gradient passes it.  Values of keys
+ * and queries with a negative document are not used at all, be they NaN.
+ * o: contiguous like q; lse: dev float[batch, q_heads, q_len], the natural logarithm of the
+ * sum of exp(s).  Strides in elements (batch, token, head), multiples of 8, pointers 16-byte
+ * aligned; head_dim a multiple of 8 up to 128.  No counterpart in the reference.
+ *
+ * The backward pass takes o, lse as the forward pass left them and d_o (contiguous like q)
+ * and writes contiguous dq, dk, dv: same bits on every run, no atomics.
+ * workspace: lego_attention_workspace_bytes() bytes of device memory, 16-byte aligned, of
+ * any contents, that no other call in flight uses.                              */
+typedef struct lego_attention {
+  int32_t dtype, causal;
+  int64_t batch, q_len, k_len, q_heads, k_heads, head_dim;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  float scale, softcap;
+  const float* slopes;
+  const int32_t* prefix;
+  const int32_t* documents;
+} lego_attention_t;
+
+int64_t lego_attention_workspace_bytes(const lego_attention_t* desc, int32_t backward);
+int32_t lego_attention_fwd(const lego_attention_t* desc, const void* q, const void* k, const void* v, void* o,
+                           float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+int32_t lego_attention_bwd(const lego_attention_t* desc, const void* q, const void* k, const void* v,
+                           const void* o, const float* lse, const void* d_o, void* dq, void* dk, void* dv,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Attention of `drafted` (1 .. 64) new tokens per sequence over a paged cache.  Token t of
+ * sequence b, whose keys and values stand in place lengths[b] + t of the sequence, sees the
+ * lengths[b] tokens cached before the draft, its ancestors in the draft and itself.
+ * parents: dev int32[batch, drafted], the draft token t follows (-1: the cached text; else
+ * less than t); a token with any other parent, or that descends from one, is unused: its
+ * output is zero.  parents NULL: a chain, each token follows the one before (drafted = 1:
+ * plain decoding).  A sequence with lengths[b] < 0 is unused.  The distance of the bias is
+ * that of the positions, a drafted token's being lengths[b] + its depth.
+ * Place p of sequence b is slot p % page_size of page page_table[b * table_stride + p /
+ * page_size] of k_cache, v_cache [pages, page_size, k_heads, head_dim]; a page number outside
+ * [0, pages), or a place at or past max_pages * page_size, holds nothing (its keys are
+ * hidden).  Scores as in lego_attention.  q [batch, drafted, q_heads, head_dim]; o
+ * contiguous.  Strides in elements (batch, token, head / page, slot, head), multiples of 8,
+ * pointers 16-byte aligned; head_dim a multiple of 8 up to 128.  workspace as above.
+ * No counterpart in the reference.                                              */
+typedef struct lego_tree_attention {
+  int32_t dtype, reserved;
+  int64_t batch, drafted, q_heads, k_heads, head_dim;
+  int64_t pages, page_size, max_pages, table_stride;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  float scale, softcap;
+} lego_tree_attention_t;
+
+int64_t lego_tree_attention_workspace_bytes(const lego_tree_attention_t* desc);
+int32_t lego_tree_attention(const lego_tree_attention_t* desc, const void* q, const void* k_cache,
+                            const void* v_cache, const int32_t* page_table, const int32_t* lengths,
+                            const int32_t* parents, const float* slopes, void* o, void* workspace,
+                            int64_t workspace_bytes, void* stream);
 
 /* ---- housekeeping --------------------------------------------------------- */
 

@@ -15,6 +15,7 @@ MAX_BLOCKS = 4
 MAX_STAGES = 8
 MAX_TERMS = 32
 MAX_GROUPS = 256
+MAX_DRAFT = 64
 
 BLOCK_REGP = 0
 BLOCK_ANTIDIAG = 1
@@ -83,6 +84,35 @@ class DmaPlan(C.Structure):
                 ("tile_bytes", C.c_int64), ("load", DmaSide), ("store", DmaSide), ("outer", DmaOuter * 8)]
 
 
+F16, BF16, F32 = 0, 1, 2
+PAIRS_HALF, PAIRS_INTERLEAVED = 0, 1
+
+
+class Rotary(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("pairs", C.c_int32), ("inverse", C.c_int32), ("position_bytes", C.c_int32),
+                ("batch", C.c_int64), ("length", C.c_int64), ("head_dim", C.c_int64), ("rotary_dim", C.c_int64),
+                ("heads", C.c_int64 * 2), ("stride", (C.c_int64 * 3) * 2), ("position_stride", C.c_int64 * 2),
+                ("scale", C.c_float), ("reserved", C.c_int32)]
+
+
+class Attention(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("causal", C.c_int32),
+                ("batch", C.c_int64), ("q_len", C.c_int64), ("k_len", C.c_int64), ("q_heads", C.c_int64),
+                ("k_heads", C.c_int64), ("head_dim", C.c_int64),
+                ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+                ("scale", C.c_float), ("softcap", C.c_float),
+                ("slopes", C.c_void_p), ("prefix", C.c_void_p), ("documents", C.c_void_p)]
+
+
+class TreeAttention(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("reserved", C.c_int32),
+                ("batch", C.c_int64), ("drafted", C.c_int64), ("q_heads", C.c_int64), ("k_heads", C.c_int64),
+                ("head_dim", C.c_int64), ("pages", C.c_int64), ("page_size", C.c_int64), ("max_pages", C.c_int64),
+                ("table_stride", C.c_int64),
+                ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+                ("scale", C.c_float), ("softcap", C.c_float)]
+
+
 LayoutP = C.POINTER(Layout)
 
 # name -> (restype, argtypes); must list every function include/lego_b200.h declares.
@@ -122,6 +152,12 @@ SIGNATURES = {
     "lego_grouped_gemm_f16_static": (C.c_int32, [C.POINTER(C.c_void_p), C.POINTER(C.c_void_p),
                                                  C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.c_int32,
                                                  C.POINTER(LayoutP), C.c_void_p, C.c_void_p]),
+    "lego_rotary": (C.c_int32, [C.POINTER(Rotary)] + [C.c_void_p] * 7),
+    "lego_attention_workspace_bytes": (C.c_int64, [C.POINTER(Attention), C.c_int32]),
+    "lego_attention_fwd": (C.c_int32, [C.POINTER(Attention)] + [C.c_void_p] * 6 + [C.c_int64, C.c_void_p]),
+    "lego_attention_bwd": (C.c_int32, [C.POINTER(Attention)] + [C.c_void_p] * 10 + [C.c_int64, C.c_void_p]),
+    "lego_tree_attention_workspace_bytes": (C.c_int64, [C.POINTER(TreeAttention)]),
+    "lego_tree_attention": (C.c_int32, [C.POINTER(TreeAttention)] + [C.c_void_p] * 9 + [C.c_int64, C.c_void_p]),
     "lego_copy_2d": (C.c_int32, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p]),
     "lego_device_status": (C.c_int32, [C.c_void_p, C.POINTER(C.c_uint32)]),
     "lego_status_string": (C.c_char_p, [C.c_int32]),

@@ -1,0 +1,201 @@
+// Rotary positions: pairs of a head's values turned by position * frequency.
+//
+// Every value is read once and written once and nothing else is large, so the kernel is
+// bound by memory; what must not cost is the angle.  A block takes a few tokens: its
+// threads first put the tokens' cosines and sines (one pair of a token per thread and
+// step, shared by all heads of both tensors) into shared memory, then turn the heads with
+// 16-byte loads and stores.  The angle is position * frequency in 64 bits, reduced to a
+// fraction of a turn there (positions of 10^5 and more leave no digits of a 32-bit angle),
+// sine and cosine of the fraction are taken in 32 bits.
+#include "attention.cuh"
+#include "ptx_sm100.cuh"
+
+namespace lego {
+namespace {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotMaxTokens = 8;      // tokens per block at most
+
+struct RotArgs {
+  const void* x[2];
+  void* y[2];
+  long long in_stride[2][3];
+  int heads[2];
+  const void* positions;
+  long long pos_stride[2];
+  const double* freqs;
+  long long tokens;       // batch * length
+  long long length;
+  int dim, half;          // head_dim, rotary_dim / 2
+  int pos64, inverse;
+  float scale;
+  int per_block;          // tokens per block
+};
+
+// VEC values of T at once; VEC = 16 / sizeof(T) for aligned tensors, 1 otherwise.
+template <typename T, int VEC> struct Pack { T v[VEC]; };
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_pack(const T* p) {
+  Pack<T, VEC> r;
+  if constexpr (VEC * sizeof(T) == 16) *reinterpret_cast<uint4*>(&r) = __ldcs(reinterpret_cast<const uint4*>(p));
+  else r.v[0] = *p;
+  return r;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, VEC>& r) {
+  if constexpr (VEC * sizeof(T) == 16) __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&r));
+  else *p = r.v[0];
+}
+
+// A unit of work is VEC values of the rotated part and their partners (half: two packs;
+// interleaved: one pack of whole pairs, or the two values of one pair when VEC is 1), or
+// one pack of the part that is copied.
+template <typename T, int VEC, bool HALF>
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotArgs a) {
+  extern __shared__ float2 turn[];   // [token][pair] (cos, sin), scaled
+  ptx::launch_dependents();
+  ptx::grid_dependency_wait();
+  const long long t0 = (long long)blockIdx.x * a.per_block;
+  const int nt = (int)(a.tokens - t0 < a.per_block ? a.tokens - t0 : a.per_block);
+
+  for (int i = threadIdx.x; i < nt * a.half; i += kRotThreads) {
+    const int t = i / a.half, p = i - t * a.half;
+    const long long b = (t0 + t) / a.length, s = (t0 + t) - b * a.length;
+    const long long at = b * a.pos_stride[0] + s * a.pos_stride[1];
+    const double pos = a.pos64 ? (double)reinterpret_cast<const long long*>(a.positions)[at]
+                               : (double)reinterpret_cast<const int*>(a.positions)[at];
+    double turns = pos * a.freqs[p] * 0.15915494309189533577;   // 1 / (2 pi)
+    turns -= rint(turns);
+    float sn, cs;
+    sincospif(2.0f * (float)turns, &sn, &cs);
+    turn[i] = make_float2(a.scale * cs, a.scale * (a.inverse ? -sn : sn));
+  }
+  __syncthreads();
+
+  const int rot_units = HALF ? a.half / VEC : (VEC > 1 ? 2 * a.half / VEC : a.half);
+  const int copy_units = (a.dim - 2 * a.half) / VEC;
+  const int per_head = rot_units + copy_units;
+  const int h0 = a.heads[0], heads = h0 + a.heads[1];
+  const int units = nt * heads * per_head;
+#pragma unroll 2
+  for (int i = threadIdx.x; i < units; i += kRotThreads) {
+    const int head_id = i / per_head, u = i - head_id * per_head;
+    const int t = head_id / heads, hh = head_id - t * heads;
+    const int which = hh >= h0, h = which ? hh - h0 : hh;
+    const long long tok = t0 + t;
+    const long long b = tok / a.length, s = tok - b * a.length;
+    const T* x = reinterpret_cast<const T*>(a.x[which]) + b * a.in_stride[which][0] + s * a.in_stride[which][1] +
+                 h * a.in_stride[which][2];
+    T* y = reinterpret_cast<T*>(a.y[which]) + (tok * a.heads[which] + h) * a.dim;
+    if (u >= rot_units) {
+      const int c = 2 * a.half + (u - rot_units) * VEC;
+      store_pack<T, VEC>(y + c, load_pack<T, VEC>(x + c));
+      continue;
+    }
+    const float2* cs = turn + t * a.half;
+    if constexpr (HALF || VEC == 1) {
+      const int p = u * VEC;
+      const int c1 = HALF ? p : 2 * p, c2 = HALF ? p + a.half : 2 * p + 1;
+      const Pack<T, VEC> x1 = load_pack<T, VEC>(x + c1), x2 = load_pack<T, VEC>(x + c2);
+      Pack<T, VEC> y1, y2;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float2 k = cs[p + e];
+        const float f1 = to_f32(x1.v[e]), f2 = to_f32(x2.v[e]);
+        from_f32(f1 * k.x - f2 * k.y, &y1.v[e]);
+        from_f32(f2 * k.x + f1 * k.y, &y2.v[e]);
+      }
+      store_pack<T, VEC>(y + c1, y1);
+      store_pack<T, VEC>(y + c2, y2);
+    } else {
+      const int p = u * (VEC / 2);
+      const Pack<T, VEC> xv = load_pack<T, VEC>(x + 2 * p);
+      Pack<T, VEC> yv;
+#pragma unroll
+      for (int e = 0; e < VEC / 2; ++e) {
+        const float2 k = cs[p + e];
+        const float f1 = to_f32(xv.v[2 * e]), f2 = to_f32(xv.v[2 * e + 1]);
+        from_f32(f1 * k.x - f2 * k.y, &yv.v[2 * e]);
+        from_f32(f2 * k.x + f1 * k.y, &yv.v[2 * e + 1]);
+      }
+      store_pack<T, VEC>(y + 2 * p, yv);
+    }
+  }
+}
+
+template <typename T, int VEC>
+cudaError_t launch_rotary(const RotArgs& a, bool half, long long blocks, size_t smem, cudaStream_t s) {
+  return half ? launch_overlapped(rotary_kernel<T, VEC, true>, dim3((unsigned)blocks), dim3(kRotThreads), smem, s, a)
+              : launch_overlapped(rotary_kernel<T, VEC, false>, dim3((unsigned)blocks), dim3(kRotThreads), smem, s, a);
+}
+
+template <typename T>
+cudaError_t launch_rotary_type(const RotArgs& a, bool half, bool vec, long long blocks, size_t smem, cudaStream_t s) {
+  constexpr int VEC = 16 / sizeof(T);
+  return vec ? launch_rotary<T, VEC>(a, half, blocks, smem, s) : launch_rotary<T, 1>(a, half, blocks, smem, s);
+}
+
+}  // namespace
+}  // namespace lego
+
+using namespace lego;
+
+extern "C" int32_t lego_rotary(const lego_rotary_t* d, const void* x0, const void* x1, void* y0, void* y1,
+                               const void* positions, const double* freqs, void* stream) {
+  if (!d) return LEGO_ERR_NULL;
+  if (d->dtype < LEGO_F16 || d->dtype > LEGO_F32) return LEGO_ERR_UNSUPPORTED;
+  if (d->pairs != LEGO_PAIRS_HALF && d->pairs != LEGO_PAIRS_INTERLEAVED) return LEGO_ERR_UNSUPPORTED;
+  if (d->position_bytes != 4 && d->position_bytes != 8) return LEGO_ERR_UNSUPPORTED;
+  if (d->batch < 0 || d->length < 0 || d->heads[0] < 0 || d->heads[1] < 0) return LEGO_ERR_DIM;
+  if (d->head_dim < 1 || d->head_dim > 1024 || d->rotary_dim < 2 || d->rotary_dim > d->head_dim || (d->rotary_dim & 1))
+    return LEGO_ERR_SIZE;
+  if (d->heads[0] > 65536 || d->heads[1] > 65536) return LEGO_ERR_SIZE;
+  if (d->batch == 0 || d->length == 0 || d->heads[0] + d->heads[1] == 0) return LEGO_OK;
+  if (!positions || !freqs) return LEGO_ERR_NULL;
+  if ((d->heads[0] && (!x0 || !y0)) || (d->heads[1] && (!x1 || !y1))) return LEGO_ERR_NULL;
+  if (d->batch > (1LL << 40) / d->length) return LEGO_ERR_OVERFLOW;
+
+  RotArgs a = {};
+  const void* xs[2] = {x0, x1};
+  void* ys[2] = {y0, y1};
+  const int eb = d->dtype == LEGO_F32 ? 4 : 2, vec_elems = 16 / eb;
+  const bool half = d->pairs == LEGO_PAIRS_HALF;
+  // whole 16-byte packs: every row of a head starts on such a boundary and no pack holds the
+  // border between the halves, or between the rotated and the copied part
+  bool vec = d->head_dim % vec_elems == 0 && (half ? d->rotary_dim / 2 : d->rotary_dim) % vec_elems == 0;
+  for (int i = 0; i < 2; ++i) {
+    a.x[i] = xs[i];
+    a.y[i] = ys[i];
+    a.heads[i] = (int)d->heads[i];
+    if (!d->heads[i]) continue;
+    if (((uintptr_t)xs[i] | (uintptr_t)ys[i]) & (uintptr_t)(eb - 1)) return LEGO_ERR_ALIGN;
+    vec = vec && (((uintptr_t)xs[i] | (uintptr_t)ys[i]) & 15) == 0;
+    for (int k = 0; k < 3; ++k) {
+      a.in_stride[i][k] = d->stride[i][k];
+      vec = vec && d->stride[i][k] % vec_elems == 0;
+    }
+  }
+  a.positions = positions;
+  a.pos_stride[0] = d->position_stride[0];
+  a.pos_stride[1] = d->position_stride[1];
+  a.freqs = freqs;
+  a.tokens = d->batch * d->length;
+  a.length = d->length;
+  a.dim = (int)d->head_dim;
+  a.half = (int)d->rotary_dim / 2;
+  a.pos64 = d->position_bytes == 8;
+  a.inverse = d->inverse != 0;
+  a.scale = d->scale;
+  a.per_block = 1;
+  while (a.per_block < kRotMaxTokens && a.tokens / (2 * a.per_block) >= 148 * 8) a.per_block *= 2;
+  const long long blocks = (a.tokens + a.per_block - 1) / a.per_block;
+  if (blocks > 0x7fffffffLL) return LEGO_ERR_SIZE;
+  const size_t smem = (size_t)a.per_block * a.half * sizeof(float2);   // at most 8 x 512 x 8 = 32 KiB
+  cudaStream_t s = (cudaStream_t)stream;
+  cudaError_t e;
+  if (d->dtype == LEGO_F16) e = launch_rotary_type<__half>(a, half, vec, blocks, smem, s);
+  else if (d->dtype == LEGO_BF16) e = launch_rotary_type<__nv_bfloat16>(a, half, vec, blocks, smem, s);
+  else e = launch_rotary_type<float>(a, half, vec, blocks, smem, s);
+  LEGO_CUDA_TRY(e);
+  return LEGO_OK;
+}

@@ -7,7 +7,9 @@ The names and argument meaning follow the callables the reference generates:
 (``triton_generated/layernorm/layernorm.py:279-340``),
 ``lego_group_gemm_fn(group_A, group_B)``
 (``triton_generated/grouped_gemm/grouped_gemm.py:120-162``), plus ``permute`` /
-``transpose`` for the MLIR transpose programs and the index-map evaluator.
+``transpose`` for the MLIR transpose programs and the index-map evaluator.  ``rotary``,
+``attention`` and ``tree_attention`` (no counterpart there) are the rest of a language model's
+attention layer, in training and over a paged cache.
 
 Tensors are torch tensors; torch only owns memory and streams here.  A CUDA
 tensor is processed in place on the current stream.  A CPU tensor is staged
@@ -18,6 +20,7 @@ op raises; there is no CPU implementation behind them.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import List, Optional, Sequence
 
 import torch
@@ -29,6 +32,7 @@ from .lowering import lower, lower_optional
 __all__ = [
     "eval_apply", "eval_inv", "eval_range", "permute", "permute_plan", "permute_dma_plan", "permute_slabs", "permute_slab_info", "transpose", "softmax",
     "LEGOLayerNorm", "lego_layer_norm", "layer_norm_fwd", "layer_norm_bwd", "matmul", "lego_group_gemm_fn",
+    "rotary", "rotary_frequencies", "LEGORotary", "attention", "attention_fwd", "attention_bwd", "LEGOAttention", "tree_attention",
     "grouped_swizzle_layout", "default_group_m", "default_tile_order", "row_tiling_layout", "device_status", "tune", "selftest_bounded_wait",
 ]
 
@@ -772,3 +776,356 @@ def _group_gemm_from_host(group_A, group_B, tile_orders) -> List[torch.Tensor]:
         outs.append(out)
     pipe.finish()
     return outs
+
+
+# ---- attention ----------------------------------------------------------------------
+
+_ATTN_TYPES = {torch.float16: _abi.F16, torch.bfloat16: _abi.BF16}
+_ROTARY_TYPES = {**_ATTN_TYPES, torch.float32: _abi.F32}
+
+
+def _same_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
+    """The device of a call: that of its CUDA tensors, which have to share one (host tensors are
+    staged to it); the current device when all are host tensors."""
+    dev = None
+    for t in (first, *others):
+        if t is not None and t.is_cuda:
+            if dev is not None and t.device != dev:
+                raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+            dev = t.device
+    return dev if dev is not None else _device()
+
+
+def _ready(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    return t if t.is_cuda else t.to(dev, non_blocking=True)
+
+
+def _dense(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """On the device, contiguous, on a 16-byte boundary."""
+    t = _ready(t, dev).contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _strided(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """On the device in a form the kernels read in place: last axis contiguous, the other strides
+    whole 16-byte steps, the first value on such a boundary; a copy where it is not."""
+    t = _ready(t, dev)
+    steps = 16 // t.element_size()
+    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0 and all(
+            n == 1 or (s > 0 and s % steps == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])):
+        return t
+    return _dense(t, dev)
+
+
+def _strides(t: torch.Tensor):
+    """Strides of the leading axes in elements; an axis of one has none of its own."""
+    return tuple(t.shape[-1] if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+
+
+def _check_int32(t: Optional[torch.Tensor], name: str, shape) -> None:
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+
+
+def _check_slopes(t: Optional[torch.Tensor], heads: int) -> None:
+    if t is None:
+        return
+    if t.dtype != torch.float32 or tuple(t.shape) != (heads,):
+        raise ValueError(f"slopes must be float32 [{heads}], got {t.dtype} {list(t.shape)}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("slopes are constants of the bias: no gradient is computed for them")
+
+
+def _optional(t: Optional[torch.Tensor], dev: torch.device) -> Optional[torch.Tensor]:
+    return None if t is None else _ready(t, dev).contiguous()
+
+
+def _scores(scale: Optional[float], softcap: float, dim: int):
+    scale = dim ** -0.5 if scale is None else float(scale)
+    softcap = float(softcap)
+    if not math.isfinite(scale) or not math.isfinite(softcap) or softcap < 0:
+        raise ValueError("scale must be finite, softcap finite and not negative")
+    return scale, softcap
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
+                       original_length: int = 8192, low: float = 1.0, high: float = 4.0, device=None) -> torch.Tensor:
+    """Angles per position of the ``dim / 2`` pairs ``rotary`` turns, float64:
+    ``base ** (-2 p / dim)``, stretched for contexts ``factor`` times the trained ``original_length``
+    by ``scaling``: ``"linear"`` all of them; ``"ntk"`` through the base, the first pair not at all and the
+    last one fully; ``"bands"`` by how often a pair turns within the trained length: at least ``high``
+    times, kept; at most ``low`` times, stretched fully; blended linearly in between."""
+    if dim < 2 or dim % 2:
+        raise ValueError("dim must be even and at least 2")
+    if not (math.isfinite(base) and base > 0 and math.isfinite(factor) and factor >= 1):
+        raise ValueError("base must be positive and factor at least 1")
+    if scaling == "ntk":
+        base = base * factor ** (dim / (dim - 2)) if dim > 2 else base
+    f = base ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "bands":
+        if original_length < 1 or not 0 <= low < high:
+            raise ValueError("bands need original_length >= 1 and 0 <= low < high")
+        keep = ((original_length * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        f = f * (keep + (1 - keep) / factor)
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    return f if device is None else f.to(device)
+
+
+def _rotary(xs, positions, freqs, pairs, scale, inverse):
+    """Turned copies of ``xs`` (one or two tensors ``[B, S, H_i, D]``), one launch."""
+    kind = {"half": _abi.PAIRS_HALF, "interleaved": _abi.PAIRS_INTERLEAVED}.get(pairs)
+    if kind is None:
+        raise ValueError(f"pairs must be 'half' or 'interleaved', got {pairs!r}")
+    x = xs[0]
+    for t in xs:
+        if t.dim() != 4 or t.dtype not in _ROTARY_TYPES or t.dtype != x.dtype:
+            raise ValueError("rotary takes [B, S, H, D] tensors of one type: float16, bfloat16 or float32")
+        if t.shape[:2] != x.shape[:2] or t.shape[3] != x.shape[3]:
+            raise ValueError("the tensors must agree in batch, length and head size")
+    B, S, _, D = x.shape
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((B, S), (S,)):
+        raise ValueError(f"positions must be int32 or int64 [{B}, {S}] or [{S}]")
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or freqs.numel() < 1 or 2 * freqs.numel() > D:
+        raise ValueError(f"freqs must be float64 of 1 .. {D // 2} pairs")
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    dev = _same_device(*xs, positions, freqs)
+    with torch.cuda.device(dev):
+        src = [_ready(t, dev) for t in xs]
+        src = [t if t.stride(-1) == 1 or D == 1 else t.contiguous() for t in src]
+        pos, fr = _ready(positions, dev), _ready(freqs, dev).contiguous()
+        out = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in src]
+        d = _abi.Rotary(dtype=_ROTARY_TYPES[x.dtype], pairs=kind, inverse=int(inverse), position_bytes=pos.element_size(),
+                        batch=B, length=S, head_dim=D, rotary_dim=2 * fr.numel(), scale=float(scale))
+        d.position_stride[:] = (0 if pos.dim() == 1 else pos.stride(0), pos.stride(-1))
+        for i, t in enumerate(src):
+            d.heads[i] = t.shape[2]
+            d.stride[i][:] = _strides(t)
+        two = len(src) > 1
+        _abi.check(_abi.lib().lego_rotary(C.byref(d), src[0].data_ptr(), src[1].data_ptr() if two else None,
+                                          out[0].data_ptr(), out[1].data_ptr() if two else None, pos.data_ptr(),
+                                          fr.data_ptr(), _stream()), "lego_rotary")
+        return [_like_input(o, t) for o, t in zip(out, xs)]
+
+
+class LEGORotary(torch.autograd.Function):
+    """``LEGORotary.apply(q, k, positions, freqs, pairs, scale)``; ``k`` may be None."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, freqs, pairs, scale):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions, freqs)
+        ctx.pairs, ctx.scale = pairs, scale
+        out = _rotary([q] if k is None else [q, k], positions, freqs, pairs, scale, False)
+        return (out[0], out[1] if k is not None else None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        positions, freqs = ctx.saved_tensors
+        given = [g for g in (dq, dk) if g is not None]
+        back = iter(_rotary(given, positions, freqs, ctx.pairs, ctx.scale, True) if given else ())
+        return tuple(None if g is None else next(back) for g in (dq, dk)) + (None,) * 4
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, *,
+           pairs: str = "half", scale: float = 1.0):
+    """Queries ``[B, S, Hq, D]`` and keys ``[B, S, Hk, D]`` turned by their positions, in one launch:
+    pair ``p`` of the first ``2 len(freqs)`` values of every head by the angle ``position * freqs[p]``
+    (``rotary_frequencies``), the rest copied.  ``pairs``: ``"half"`` pairs value p with value p + len(freqs),
+    ``"interleaved"`` 2p with 2p + 1.  ``positions``: int32 or int64 ``[B, S]`` or ``[S]``.  ``scale``
+    multiplies the turned values.  Differentiable in q and k.  Returns ``(q, k)``, or q alone when
+    ``k`` is None.  float16, bfloat16 or float32, any strides with a contiguous last axis."""
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        out = LEGORotary.apply(q, k, positions, freqs, pairs, scale)
+        return out[0] if k is None else out
+    out = _rotary([q] if k is None else [q, k], positions, freqs, pairs, scale, False)
+    return out[0] if k is None else tuple(out)
+
+
+def _attention_desc(q, k, v, causal, prefix, documents, softcap, slopes, scale):
+    """Checks of an attention call; ``(device, descriptor, tensors it refers to)`` with q, k, v first."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("attention takes q [B, Sq, Hq, D] and k, v [B, Sk, Hk, D]")
+    if q.dtype not in _ATTN_TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("attention takes float16 or bfloat16 tensors of one type")
+    B, Sq, Hq, D = q.shape
+    Sk, Hk = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError("q, k, v must agree in batch and head size, k and v in shape")
+    if Hk < 1 or Hq % Hk:
+        raise ValueError(f"{Hq} query heads cannot share {Hk} key heads evenly")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError("head size must be a multiple of 8 up to 128")
+    if prefix is not None and not causal:
+        raise ValueError("a prefix needs causal=True")
+    if documents is not None and Sq > Sk:
+        raise ValueError("documents need as many keys as queries at least")
+    _check_int32(prefix, "prefix", (B,))
+    _check_int32(documents, "documents", (B, Sk))
+    _check_slopes(slopes, Hq)
+    scale, softcap = _scores(scale, softcap, D)
+    dev = _same_device(q, k, v, prefix, documents, slopes)
+    keep = [_strided(q, dev), _strided(k, dev), _strided(v, dev), _optional(prefix, dev), _optional(documents, dev),
+            _optional(slopes, dev)]
+    d = _abi.Attention(dtype=_ATTN_TYPES[q.dtype], causal=int(bool(causal)), batch=B, q_len=Sq, k_len=Sk, q_heads=Hq,
+                       k_heads=Hk, head_dim=D, scale=scale, softcap=softcap, prefix=_ptr(keep[3]),
+                       documents=_ptr(keep[4]), slopes=_ptr(keep[5]))
+    d.q_stride[:], d.k_stride[:], d.v_stride[:] = (_strides(t) for t in keep[:3])
+    return dev, d, keep
+
+
+def _attention_workspace(d, backward, dev):
+    n = _abi.lib().lego_attention_workspace_bytes(C.byref(d), backward)
+    _abi.check(min(n, 0), "lego_attention_workspace_bytes")
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=dev), n
+
+
+def attention_fwd(q, k, v, causal=False, prefix=None, documents=None, softcap=0.0, slopes=None, scale=None):
+    """Attention forward: ``(o, lse)``, see ``attention``; lse is float32 ``[B, Hq, Sq]``."""
+    dev, d, keep = _attention_desc(q, k, v, causal, prefix, documents, softcap, slopes, scale)
+    B, Sq, Hq, _ = q.shape
+    with torch.cuda.device(dev):
+        o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=dev)
+        if k.shape[1] == 0:
+            o.zero_()
+            lse.fill_(-math.inf)
+        elif o.numel():
+            ws, n = _attention_workspace(d, 0, dev)
+            _abi.check(_abi.lib().lego_attention_fwd(C.byref(d), *(t.data_ptr() for t in keep[:3]), o.data_ptr(),
+                                                     lse.data_ptr(), ws.data_ptr(), n, _stream()), "lego_attention_fwd")
+        return _like_input(o, q), _like_input(lse, q)
+
+
+def attention_bwd(do, q, k, v, o, lse, causal=False, prefix=None, documents=None, softcap=0.0, slopes=None, scale=None):
+    """Attention backward from what ``attention_fwd`` took and gave: ``(dq, dk, dv)``, contiguous,
+    the same bits on every run."""
+    dev, d, keep = _attention_desc(q, k, v, causal, prefix, documents, softcap, slopes, scale)
+    _same_device(do, o, lse, keep[0])
+    B, Sq, Hq, _ = q.shape
+    if do.shape != q.shape or o.shape != q.shape or tuple(lse.shape) != (B, Hq, Sq):
+        raise ValueError("do and o must have q's shape, lse [B, Hq, Sq]")
+    if do.dtype != q.dtype or o.dtype != q.dtype or lse.dtype != torch.float32:
+        raise ValueError("do and o must have q's type, lse float32")
+    with torch.cuda.device(dev):
+        dod, od, lsed = _dense(do, dev), _dense(o, dev), _dense(lse, dev)
+        dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=dev) for t in (q, k, v))
+        if dq.numel() == 0 or dk.numel() == 0:
+            for g in (dq, dk, dv):
+                g.zero_()
+        else:
+            ws, n = _attention_workspace(d, 1, dev)
+            _abi.check(_abi.lib().lego_attention_bwd(C.byref(d), *(t.data_ptr() for t in keep[:3]), od.data_ptr(),
+                                                     lsed.data_ptr(), dod.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                                                     dv.data_ptr(), ws.data_ptr(), n, _stream()), "lego_attention_bwd")
+        return _like_input(dq, q), _like_input(dk, k), _like_input(dv, v)
+
+
+class LEGOAttention(torch.autograd.Function):
+    """``LEGOAttention.apply(q, k, v, causal, prefix, documents, softcap, slopes, scale)`` -> ``(o, lse)``."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, causal, prefix, documents, softcap, slopes, scale):
+        o, lse = attention_fwd(q, k, v, causal, prefix, documents, softcap, slopes, scale)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(lse)
+        ctx.save_for_backward(q, k, v, o, lse, prefix, documents, slopes)
+        ctx.rest = (causal, softcap, scale)
+        return o, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, _):
+        if do is None:
+            return (None,) * 9
+        q, k, v, o, lse, prefix, documents, slopes = ctx.saved_tensors
+        causal, softcap, scale = ctx.rest
+        return (*attention_bwd(do, q, k, v, o, lse, causal, prefix, documents, softcap, slopes, scale), *(None,) * 6)
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False,
+              prefix: Optional[torch.Tensor] = None, documents: Optional[torch.Tensor] = None, softcap: float = 0.0,
+              slopes: Optional[torch.Tensor] = None, scale: Optional[float] = None, return_lse: bool = False):
+    """``softmax(scores) v`` of q ``[B, Sq, Hq, D]`` over k, v ``[B, Sk, Hk, D]`` (Hq a multiple of Hk;
+    float16 or bfloat16, D a multiple of 8 up to 128), without the scores ever in memory.
+
+    Query i stands at position ``i + Sk - Sq`` of the keys.  Scores are ``scale q.k`` (default
+    ``D ** -0.5``), bent by ``softcap * tanh(. / softcap)`` when ``softcap`` is positive, minus
+    ``slopes[h] * |position - j|`` when ``slopes`` (float32 ``[Hq]``) is given.  ``causal``: a query sees the
+    keys up to its position, and those before ``prefix[b]`` (int32 ``[B]``) too.  ``documents`` (int32
+    ``[B, Sk]``): only keys of the query's own document; negative numbers mark padding, which sees and
+    shows nothing and whose values are not used.  A query that sees no key gets zeros.
+
+    Differentiable in q, k and v.  ``return_lse``: also the logarithm of each row's sum, float32
+    ``[B, Hq, Sq]`` (no gradient).  A key hidden from one query but seen by another has to be finite."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        o, lse = LEGOAttention.apply(q, k, v, causal, prefix, documents, softcap, slopes, scale)
+    else:
+        o, lse = attention_fwd(q, k, v, causal, prefix, documents, softcap, slopes, scale)
+    return (o, lse) if return_lse else o
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                   lengths: torch.Tensor, parents: Optional[torch.Tensor] = None, *, softcap: float = 0.0,
+                   slopes: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of drafted tokens q ``[B, T, Hq, D]`` (T up to 64) over a cache of pages
+    ``[pages, page_size, Hk, D]``: the serving form of ``attention``, with the same scores.
+
+    Place p of sequence b is slot ``p % page_size`` of page ``page_table[b, p // page_size]`` (int32).
+    ``lengths`` (int32 ``[B]``) counts the tokens cached before the draft; the keys and values of
+    drafted token t stand in place ``lengths[b] + t``.  A drafted token sees the cached tokens, the
+    drafted ones it descends from and itself.  ``parents`` (int32 ``[B, T]``) names the draft token
+    each one follows, -1 the cached text; None is a chain, so T = 1 is plain decoding.  A token whose
+    parent is neither -1 nor an earlier token, or descends from such a one, is unused and gets zeros,
+    as do all tokens of a sequence of negative length.  What the cache holds past a sequence's last
+    place is not used.  No gradient."""
+    if q.dim() != 4 or k_cache.dim() != 4 or v_cache.dim() != 4:
+        raise ValueError("tree_attention takes q [B, T, Hq, D] and caches [pages, page_size, Hk, D]")
+    if q.dtype not in _ATTN_TYPES or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError("tree_attention takes float16 or bfloat16 tensors of one type")
+    B, T, Hq, D = q.shape
+    pages, page_size, Hk, _ = k_cache.shape
+    if k_cache.shape != v_cache.shape or k_cache.shape[3] != D:
+        raise ValueError("q and the caches must agree in head size, the caches in shape")
+    if Hk < 1 or Hq % Hk:
+        raise ValueError(f"{Hq} query heads cannot share {Hk} key heads evenly")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError("head size must be a multiple of 8 up to 128")
+    if not 1 <= T <= _abi.MAX_DRAFT:
+        raise ValueError(f"1 .. {_abi.MAX_DRAFT} drafted tokens per sequence")
+    if page_table.dim() != 2 or pages < 1 or page_size < 1 or page_table.shape[1] < 1:
+        raise ValueError("page_table must be int32 [B, pages of a sequence], the cache must not be empty")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_cache, v_cache)):
+        raise ValueError("tree_attention has no gradient: call it under torch.no_grad()")
+    _check_int32(page_table, "page_table", (B, page_table.shape[1]))
+    _check_int32(lengths, "lengths", (B,))
+    _check_int32(parents, "parents", (B, T))
+    _check_slopes(slopes, Hq)
+    scale, softcap = _scores(scale, softcap, D)
+    dev = _same_device(q, k_cache, v_cache, page_table, lengths, parents, slopes)
+    with torch.cuda.device(dev):
+        table, lens, par, sl = (_optional(t, dev) for t in (page_table, lengths, parents, slopes))
+        qd, kd, vd = _strided(q, dev), _strided(k_cache, dev), _strided(v_cache, dev)
+        o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        if B == 0 or Hq == 0:
+            return _like_input(o, q)
+        d = _abi.TreeAttention(dtype=_ATTN_TYPES[q.dtype], batch=B, drafted=T, q_heads=Hq, k_heads=Hk, head_dim=D,
+                               pages=pages, page_size=page_size, max_pages=table.shape[1], table_stride=table.shape[1],
+                               scale=scale, softcap=softcap)
+        d.q_stride[:], d.k_stride[:], d.v_stride[:] = _strides(qd), _strides(kd), _strides(vd)
+        lib = _abi.lib()
+        n = lib.lego_tree_attention_workspace_bytes(C.byref(d))
+        _abi.check(min(n, 0), "lego_tree_attention_workspace_bytes")
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+        _abi.check(lib.lego_tree_attention(C.byref(d), qd.data_ptr(), kd.data_ptr(), vd.data_ptr(), table.data_ptr(),
+                                           lens.data_ptr(), _ptr(par), _ptr(sl), o.data_ptr(), ws.data_ptr(), n,
+                                           _stream()), "lego_tree_attention")
+        return _like_input(o, q)
