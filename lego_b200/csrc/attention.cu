@@ -36,6 +36,54 @@ int32_t attention_problem(const lego_attention_t* d, AttnProblem* p) {
   p->slopes = d->slopes;
   p->prefix = d->prefix;
   p->documents = d->documents;
+  p->key_docs = p->query_docs = nullptr;
+  return LEGO_OK;
+}
+
+int64_t attention_docs_bytes(const AttnProblem& p) {
+  return p.documents ? (int64_t)p.batch * (tiles_of(p.k_len) + tiles_of(p.q_len)) * (int64_t)sizeof(int4) : 0;
+}
+
+namespace {
+
+// One block of 128 threads per tile: the range of its documents.
+__global__ void __launch_bounds__(kTile) attn_docs_kernel(const int* docs, int4* out, int batch, int q_len, int k_len) {
+  __shared__ int lo[4], hi[4], neg[4];
+  const int nk = tiles_of(k_len), nq = tiles_of(q_len);
+  ptx::grid_dependency_wait();
+  const int id = blockIdx.x;
+  const bool keys = id < batch * nk;
+  const int b = keys ? id / nk : (id - batch * nk) / nq;
+  const int tile = keys ? id % nk : (id - batch * nk) % nq;
+  const int at = (keys ? 0 : k_len - q_len) + tile * kTile + threadIdx.x;   // queries are the last of the keys
+  const int d = at < k_len ? docs[(long long)b * k_len + at] : 0;
+  const bool real = at < k_len;
+  const int mn = __reduce_min_sync(~0u, real && d >= 0 ? d : 0x7fffffff);
+  const int mx = __reduce_max_sync(~0u, real && d >= 0 ? d : -1);
+  const int ng = __any_sync(~0u, real && d < 0);
+  const int w = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0) {
+    lo[w] = mn;
+    hi[w] = mx;
+    neg[w] = ng;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0)
+    out[id] = make_int4(min(min(lo[0], lo[1]), min(lo[2], lo[3])), max(max(hi[0], hi[1]), max(hi[2], hi[3])),
+                        neg[0] | neg[1] | neg[2] | neg[3], 0);
+}
+
+}  // namespace
+
+int32_t attention_docs(AttnProblem* p, void* where, cudaStream_t s) {
+  if (!p->documents) return LEGO_OK;
+  const long long nk = (long long)p->batch * tiles_of(p->k_len), nq = (long long)p->batch * tiles_of(p->q_len);
+  if (nk + nq > 0x7fffffffLL) return LEGO_ERR_SIZE;
+  int4* out = reinterpret_cast<int4*>(where);
+  LEGO_CUDA_TRY(launch_overlapped(attn_docs_kernel, dim3((unsigned)(nk + nq)), dim3(kTile), 0, s, p->documents, out,
+                                  p->batch, p->q_len, p->k_len));
+  p->key_docs = out;
+  p->query_docs = out + nk;
   return LEGO_OK;
 }
 
@@ -100,31 +148,6 @@ __device__ __forceinline__ Row row_of(long long id, int heads, int len) {
 template <typename T>
 __device__ __forceinline__ const T* at(const void* x, const long long* st, int b, int i, int h) {
   return reinterpret_cast<const T*>(x) + b * st[0] + i * st[1] + h * st[2];
-}
-
-template <typename T>
-__global__ void fwd_kernel(AttnProblem p, const void* q, const void* k, const void* v, T* o, float* lse) {
-  const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (id >= (long long)p.batch * p.q_heads * p.q_len) return;
-  const Row r = row_of(id, p.q_heads, p.q_len);
-  const int pos = r.i + p.offset;
-  float qv[MAXD], acc[MAXD] = {}, kv[MAXD], m = -INFINITY, l = 0.f, bend;
-  load_row(at<T>(q, p.q_stride, r.b, r.i, r.h), p.dim, lane, qv);
-  for (int j = 0; j < p.k_len; ++j) {
-    if (!sees(p, r.b, pos, j)) continue;
-    load_row(at<T>(k, p.k_stride, r.b, j, r.h / p.group), p.dim, lane, kv);
-    const float s = score(p, dot(qv, kv), r.h, pos, j, &bend);
-    const float mn = fmaxf(m, s);
-    const float a = mn == -INFINITY ? 1.f : expf(m - mn), w = mn == -INFINITY ? 0.f : expf(s - mn);
-    load_row(at<T>(v, p.v_stride, r.b, j, r.h / p.group), p.dim, lane, kv);
-    l = l * a + w;
-#pragma unroll
-    for (int e = 0; e < MAXD; ++e) acc[e] = acc[e] * a + w * kv[e];
-    m = mn;
-  }
-  store_row(o + (((long long)r.b * p.q_len + r.i) * p.q_heads + r.h) * p.dim, p.dim, lane, acc, l > 0.f ? 1.f / l : 0.f);
-  if (lane == 0) lse[id] = l > 0.f ? m + logf(l) : -INFINITY;
 }
 
 template <typename T>
@@ -206,26 +229,7 @@ int64_t lego_attention_workspace_bytes(const lego_attention_t* d, int32_t backwa
   AttnProblem p;
   const int32_t st = attention_problem(d, &p);
   if (st != LEGO_OK) return st;
-  return backward ? (int64_t)p.batch * p.q_heads * p.q_len * 4 : 0;
-}
-
-int32_t lego_attention_fwd(const lego_attention_t* d, const void* q, const void* k, const void* v, void* o,
-                           float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
-  AttnProblem p;
-  const int32_t st = attention_problem(d, &p);
-  if (st != LEGO_OK) return st;
-  if (!q || !k || !v || !o || !lse) return LEGO_ERR_NULL;
-  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) & 15) return LEGO_ERR_ALIGN;
-  if (workspace_bytes < lego_attention_workspace_bytes(d, 0)) return LEGO_ERR_SIZE;
-  (void)workspace;
-  cudaStream_t s = (cudaStream_t)stream;
-  const long long rows = (long long)p.batch * p.q_heads * p.q_len;
-  if (d->dtype == LEGO_F16)
-    fwd_kernel<__half><<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(p, q, k, v, (__half*)o, lse);
-  else
-    fwd_kernel<__nv_bfloat16><<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(p, q, k, v, (__nv_bfloat16*)o, lse);
-  LEGO_CUDA_TRY(cudaGetLastError());
-  return LEGO_OK;
+  return attention_docs_bytes(p) + (backward ? (int64_t)p.batch * p.q_heads * p.q_len * 4 : 0);
 }
 
 int32_t lego_attention_bwd(const lego_attention_t* d, const void* q, const void* k, const void* v, const void* o,

@@ -1,0 +1,459 @@
+// Attention forward on tcgen05 (sm_100a): O = softmax(cap / bias / mask of scale Q K^T) V
+// without the scores in memory.
+//
+// One CTA takes 256 queries of one head as two tiles of 128 rows and walks the tiles of 128
+// keys that some of its rows see.  Per tile of scores: S = Q K^T into TMEM (both operands
+// from shared memory), a warpgroup with one thread per row turns S into weights
+// P = exp2(s - m) and writes them over S in TMEM as packed 16-bit pairs, and O += P V takes
+// P from TMEM.  The two row tiles alternate: while one's scores are in its warpgroup, the
+// tensor core works for the other.  Warps: 0-3 and 4-7 softmax of row tile 0 and 1 (and
+// their epilogue), 8 TMA loads, 9 MMA issue (10 and 11 fill up their warpgroup).
+//
+// Running maximum: the reference value m of a row moves only when a tile's maximum exceeds it
+// by more than 2^8 -- weights stay below 2^8, the row sum is kept in 32 bits -- so O in
+// TMEM is rarely rescaled.  The sum adds the weights before they are rounded to 16 bits;
+// that rounding, half a step of the type per weight, and the one of the result are the only
+// ones below 32 bits.
+//
+// Tiles no row of the CTA sees are not loaded (causal and prefix limits, document ranges);
+// the mask is evaluated only on tiles that are not seen whole, as 128 bits per row.
+#include <cuda.h>
+
+#include "attention.cuh"
+#include "tma_host.cuh"
+
+namespace lego {
+namespace {
+
+constexpr int kFwdThreads = 384;
+// Registers: the launch gives every thread of the three warpgroups 168 (64512 in all); a
+// softmax thread holds a row of 128 scores, the loads and the MMA issue need few.
+constexpr int kFwdRegs = 168, kSoftmaxRegs = 216, kOtherRegs = 72;
+static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kFwdRegs, "more registers than the launch has would wait forever");
+constexpr float kRescale = 8.f;      // log2 of the growth a row's reference value may lag behind
+
+template <int DP> constexpr int fwd_stages() { return DP == 128 ? 5 : 8; }
+template <int DP> constexpr int fwd_smem() { return (2 + fwd_stages<DP>()) * tile_bytes<DP>() + 1024 + 512; }
+
+struct FwdArgs {
+  CUtensorMap q, k, v, o;
+  AttnProblem p;
+  const uint16_t* v_raw;
+  float* lse;
+  uint32_t* status;
+  int q_tiles;          // of 256 queries
+};
+
+struct FwdShared {
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t kv_full[8], kv_empty[8];
+  int lo[2], hi[2];     // tiles of keys that row tile t sees
+  uint32_t tmem_base, abort_flag;
+};
+
+template <int DP, bool BF16, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_constant__ FwdArgs a) {
+  constexpr int TILE = tile_bytes<DP>(), NS = fwd_stages<DP>();
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = ptx::smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  FwdShared* sh = reinterpret_cast<FwdShared*>(smem + (2 + NS) * TILE);
+  volatile uint32_t* abort_flag = &sh->abort_flag;
+  const uint32_t q_smem = ptx::smem_u32(smem), kv_smem = q_smem + 2 * TILE;
+  const AttnProblem& p = a.p;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the last queries, which see the most keys of a causal mask, come first
+  const int heads = p.batch * p.q_heads;
+  const int qt = a.q_tiles - 1 - (int)(blockIdx.x / heads);
+  const int bh = blockIdx.x % heads, b = bh / p.q_heads, h = bh % p.q_heads, hk = h / p.group;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      ptx::mbar_init(ptx::smem_u32(&sh->q_full[t]), 1);
+      ptx::mbar_init(ptx::smem_u32(&sh->s_full[t]), 1);
+      ptx::mbar_init(ptx::smem_u32(&sh->p_full[t]), 4);
+      ptx::mbar_init(ptx::smem_u32(&sh->o_full[t]), 1);
+    }
+    for (int s = 0; s < NS; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&sh->kv_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&sh->kv_empty[s]), 1);
+    }
+    sh->abort_flag = 0;
+    ptx::fence_barrier_init();
+    ptx::fence_proxy_async();
+    ptx::prefetch_tensormap(&a.q);
+    ptx::prefetch_tensormap(&a.k);
+    ptx::prefetch_tensormap(&a.v);
+    ptx::prefetch_tensormap(&a.o);
+  }
+  if (warp == 9) {
+    ptx::tmem_alloc(ptx::smem_u32(&sh->tmem_base), 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::grid_dependency_wait();
+  const int prefix = prefix_of(p, b);
+  if (warp < 2) {   // range of key tiles of row tile `warp`
+    const int q0 = qt * 2 * kTile + warp * kTile;
+    int lo = 0, hi = 0;
+    if (q0 < p.q_len) {
+      const int last_row = q0 + kTile - 1 < p.q_len - 1 ? q0 + kTile - 1 : p.q_len - 1;
+      hi = tiles_of(last_key(p, prefix, last_row + p.offset) + 1);   // last_key may be negative: no tile
+      if (hi < 0) hi = 0;
+      if (p.documents) {
+        const int4 mine = p.query_docs[(long long)b * tiles_of(p.q_len) + q0 / kTile];
+        const int4* kd = p.key_docs + (long long)b * tiles_of(p.k_len);
+        int first = hi, last = -1;
+        for (int j = lane; j < hi; j += 32)
+          if (docs_meet(kd[j], mine)) {
+            if (j < first) first = j;
+            last = j;
+          }
+        lo = __reduce_min_sync(~0u, first);
+        hi = __reduce_max_sync(~0u, last) + 1;
+      }
+    }
+    if (lane == 0) {
+      sh->lo[warp] = lo;
+      sh->hi[warp] = hi > lo ? hi : lo;
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = sh->tmem_base;
+  const int lo0 = sh->lo[0], hi0 = sh->hi[0], lo1 = sh->lo[1], hi1 = sh->hi[1];
+  const bool any0 = lo0 < hi0, any1 = lo1 < hi1;
+  const int lo = !any0 ? lo1 : !any1 ? lo0 : lo0 < lo1 ? lo0 : lo1;
+  const int hi = !any0 ? hi1 : !any1 ? hi0 : hi0 > hi1 ? hi0 : hi1;
+
+  if (warp >= 8) {
+  ptx::regs_less<kOtherRegs>();
+  if (warp == 8) {
+    // ---------------- loads ----------------
+    bool ok = true;
+    if (lane == 0) {
+      for (int t = 0; t < 2; ++t) {
+        if (!(t ? any1 : any0)) continue;
+        const uint32_t bar = ptx::smem_u32(&sh->q_full[t]);
+        ptx::mbar_arrive_expect_tx(bar, TILE);
+        for (int c = 0; c < DP / 64; ++c) {
+          const int32_t at[5] = {c * 64, qt * 2 * kTile + t * kTile, h, b, 0};
+          ptx::tma_load_nd(4, q_smem + t * TILE + c * kBoxBytes, &a.q, at, bar);
+        }
+      }
+    }
+    const int4* kd = p.documents ? p.key_docs + (long long)b * tiles_of(p.k_len) : nullptr;
+    uint32_t n = 0;      // ring slots filled so far
+    for (int j = lo; ok && j < hi; ++j) {
+      const bool dirty = kd && kd[j].z;
+      for (int kv = 0; kv < 2; ++kv, ++n) {
+        const uint32_t slot = n % NS, round = n / NS;
+        const uint32_t full = ptx::smem_u32(&sh->kv_full[slot]);
+        if (lane == 0)
+          ok = ptx::mbar_wait_bounded(ptx::smem_u32(&sh->kv_empty[slot]), (round & 1) ^ 1, abort_flag, kAttnWait);
+        ok = __shfl_sync(~0u, ok ? 1 : 0, 0);
+        if (!ok) {
+          if (lane == 0) attn_fail(a.status, abort_flag, 0x410000u | slot);
+          break;
+        }
+        if (kv == 1 && dirty) {   // padding among these keys: their values must not meet a zero weight
+          copy_tile_clean<DP>(smem + (2 + slot) * TILE, a.v_raw + b * p.v_stride[0] + hk * p.v_stride[2], p.v_stride[1],
+                              p.dim, j * kTile, p.k_len, p.documents + (long long)b * p.k_len, lane);
+          if (lane == 0) ptx::mbar_arrive(full);
+        } else if (lane == 0) {
+          ptx::mbar_arrive_expect_tx(full, TILE);
+          for (int c = 0; c < DP / 64; ++c) {
+            const int32_t at[5] = {c * 64, j * kTile, hk, b, 0};
+            ptx::tma_load_nd(4, kv_smem + slot * TILE + c * kBoxBytes, kv ? &a.v : &a.k, at, full);
+          }
+        }
+      }
+    }
+    if (lane == 0 && *abort_flag) {   // leave no copy in flight
+      uint32_t never = 0;
+      for (int t = 0; t < 2; ++t)
+        if (t ? any1 : any0) ptx::mbar_wait_bounded(ptx::smem_u32(&sh->q_full[t]), 0, &never, kAttnWait);
+      for (uint32_t s = 0; s < (uint32_t)NS; ++s)
+        if (n > s) ptx::mbar_wait_bounded(ptx::smem_u32(&sh->kv_full[s]), ((n - 1 - s) / NS) & 1, &never, kAttnWait);
+    }
+  } else if (warp == 9) {
+    // ---------------- MMA issue ----------------
+    if (lane == 0) {
+      const uint32_t id_s = idesc_of<BF16>(kTile, false), id_o = idesc_of<BF16>(DP, true);
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
+        if (ok && !ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait)) {
+          attn_fail(a.status, abort_flag, code);
+          ok = false;
+        }
+      };
+      uint32_t done[2] = {0, 0};     // weight tiles multiplied so far
+      bool have_q[2] = {false, false};
+      for (int j = lo; ok && j <= hi && lo < hi; ++j) {
+        const uint32_t nk = 2 * (j - lo), nv = nk - 1;   // ring positions of K(j), V(j - 1)
+        if (j < hi) wait(&sh->kv_full[nk % NS], (nk / NS) & 1, 0x420000u);
+        if (j > lo) wait(&sh->kv_full[nv % NS], (nv / NS) & 1, 0x420001u);
+        ptx::tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int l = t ? lo1 : lo0, e = t ? hi1 : hi0;
+          const uint32_t s_tmem = tmem + t * kTile, o_tmem = tmem + 2 * kTile + t * DP;
+          if (j - 1 >= l && j - 1 < e) {     // O += P V(j - 1)
+            wait(&sh->p_full[t], done[t] & 1, 0x430000u | t);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const uint32_t v_tile = kv_smem + (nv % NS) * TILE;
+#pragma unroll
+            for (int s = 0; s < kTile / 16; ++s)
+              ptx::mma_f16_ts(o_tmem, s_tmem + s * 8, desc_mn_major(v_tile, s), id_o, (done[t] | s) != 0);
+            ++done[t];
+            if (j == e) ptx::mma_commit(ptx::smem_u32(&sh->o_full[t]));
+          }
+          if (j >= l && j < e) {             // S = Q K(j)
+            if (!have_q[t]) {
+              wait(&sh->q_full[t], 0, 0x440000u | t);
+              if (!ok) break;
+              have_q[t] = true;
+              ptx::tc_fence_after();
+            }
+            const uint32_t k_tile = kv_smem + (nk % NS) * TILE;
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s)
+              ptx::mma_f16_ss(s_tmem, desc_k_major(q_smem + t * TILE, s), desc_k_major(k_tile, s), id_s, s != 0);
+            ptx::mma_commit(ptx::smem_u32(&sh->s_full[t]));
+          }
+        }
+        if (!ok) break;
+        if (j > lo) ptx::mma_commit(ptx::smem_u32(&sh->kv_empty[nv % NS]));
+        if (j < hi) ptx::mma_commit(ptx::smem_u32(&sh->kv_empty[nk % NS]));
+      }
+    }
+  }
+  } else {
+    ptx::regs_more<kSoftmaxRegs>();
+    // ---------------- softmax, epilogue ----------------
+    const int t = warp >> 2, quarter = warp & 3;
+    const int l = t ? lo1 : lo0, e = t ? hi1 : hi0;
+    const int q0 = qt * 2 * kTile + t * kTile;
+    const int row = q0 + quarter * 32 + lane, pos = row + p.offset;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_tmem = tmem + lanes + t * kTile, o_tmem = tmem + lanes + 2 * kTile + t * DP;
+    const int last = last_key(p, prefix, pos);
+    const int last_first = last_key(p, prefix, q0 + p.offset);      // of the tile's first row: the smallest
+    int own_doc = -1;
+    int4 tile_docs = make_int4(0, 0, 0, 0);
+    const int* docs = nullptr;
+    const int4* kd = nullptr;
+    if (p.documents && l < e) {
+      docs = p.documents + (long long)b * p.k_len;
+      kd = p.key_docs + (long long)b * tiles_of(p.k_len);
+      if (row < p.q_len) own_doc = docs[pos];
+      tile_docs = p.query_docs[(long long)b * tiles_of(p.q_len) + q0 / kTile];
+    }
+    // log2 units: z = raw * by, or cap_by * tanh(raw * u_by / (2 log2 e)); minus slope * distance
+    const float by = p.scale * kLog2e;
+    const float u_by = CAP ? 2.f * kLog2e * p.scale / p.softcap : 0.f, cap_by = p.softcap * kLog2e;
+    const float slope = BIAS && p.slopes ? p.slopes[h] * kLog2e : 0.f;
+    float m = -INFINITY, sum = 0.f;
+    bool ok = true;
+    for (int j = l; j < e; ++j) {
+      const int j0 = j * kTile;
+      bool masked = j0 + kTile - 1 > last_first;
+      if (kd) masked = masked || !docs_same(kd[j], tile_docs);
+      if (!ptx::mbar_wait_bounded(ptx::smem_u32(&sh->s_full[t]), (j - l) & 1, abort_flag, kAttnWait)) {
+        ok = false;
+      }
+      if (!__all_sync(~0u, ok)) {
+        if (lane == 0) attn_fail(a.status, abort_flag, 0x450000u | t);
+        ok = false;
+        break;
+      }
+      ptx::tc_fence_after();
+      float s[kTile];
+#pragma unroll
+      for (int c = 0; c < kTile; c += 32) ptx::tmem_ld_32x32(s_tmem + c, reinterpret_cast<uint32_t*>(s) + c);
+      ptx::tmem_ld_wait();
+      if (CAP || BIAS) {
+#pragma unroll
+        for (int c = 0; c < kTile; ++c) {
+          float z = CAP ? cap_by * tanh_of(s[c] * u_by) : s[c] * by;
+          if (BIAS) z = fmaf(-slope, fabsf((float)(pos - j0 - c)), z);
+          s[c] = z;
+        }
+      }
+      if (masked) {
+        uint32_t see[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) see[w] = bits_upto(last - j0, w);
+        if (docs) {
+          int other[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int c = j0 + 32 * w + lane;
+            other[w] = c < p.k_len ? docs[c] : -1;
+          }
+          mask_documents(see, other, own_doc);
+        }
+#pragma unroll
+        for (int c = 0; c < kTile; ++c) s[c] = (see[c >> 5] >> (c & 31)) & 1u ? s[c] : -INFINITY;
+      }
+      float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
+      float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      if (!CAP && !BIAS) mt *= by;     // by > 0 in this instance
+      if (j == l) {
+        m = mt;
+      } else if (__any_sync(~0u, mt > m + kRescale)) {
+        const float mn = fmaxf(m, mt);
+        const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
+        m = mn;
+        sum *= f;
+#pragma unroll
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          ptx::tmem_ld_32x32(o_tmem + c, o);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+          ptx::tmem_st_32x16(o_tmem + c, o);
+          ptx::tmem_st_32x16(o_tmem + c + 16, o + 16);
+        }
+      }
+      const float mu = m == -INFINITY ? 0.f : m;
+      float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      const float2 by2 = make_float2(by, by), mu2 = make_float2(-mu, -mu);
+#pragma unroll
+      for (int c = 0; c < kTile; c += 32) {
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float2 z = make_float2(s[c + i], s[c + i + 1]);
+          z = CAP || BIAS ? ptx::add2(z, mu2) : ptx::fma2(z, by2, mu2);
+          const float2 x = make_float2(ex2(z.x), ex2(z.y));
+          add[(i >> 1) & 1] = ptx::add2(add[(i >> 1) & 1], x);
+          w[i >> 1] = pack2<BF16>(x.x, x.y);
+        }
+        ptx::tmem_st_32x16(s_tmem + c / 2, w);
+      }
+      sum += (add[0].x + add[0].y) + (add[1].x + add[1].y);
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->p_full[t]));
+    }
+    // result
+    const bool has = sum > 0.f || sum != sum;
+    const float inv = has ? 1.f / sum : 0.f;
+    if (row < p.q_len && ok)
+      a.lse[((long long)b * p.q_heads + h) * p.q_len + row] = has ? (m + log2f(sum)) * kLn2 : -INFINITY;
+    if (ok && l < e) {
+      if (!ptx::mbar_wait_bounded(ptx::smem_u32(&sh->o_full[t]), 0, abort_flag, kAttnWait)) ok = false;
+      if (!__all_sync(~0u, ok)) {
+        if (lane == 0) attn_fail(a.status, abort_flag, 0x460000u | t);
+        ok = false;
+      }
+      ptx::tc_fence_after();
+    }
+    if (ok && q0 + quarter * 32 < p.q_len) {   // the tile's own queries are no longer needed: stage there
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        if (l < e) {
+          ptx::tmem_ld_32x32(o_tmem + c, o);
+          ptx::tmem_ld_wait();
+        }
+        uint8_t* dst = smem + t * TILE + (c >> 6) * kBoxBytes + (quarter * 32 + lane) * 128;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] = has ? pack2<BF16>(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv) : 0u;
+          *reinterpret_cast<uint4*>(dst + (((((c & 32) >> 3) + i) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      ptx::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c) {
+          const int32_t at[5] = {c * 64, q0 + quarter * 32, h, b, 0};
+          ptx::tma_store_nd(4, &a.o, at, q_smem + t * TILE + c * kBoxBytes + quarter * 4096);
+        }
+        ptx::bulk_commit_group();
+        ptx::bulk_wait_group_read<0>();
+      }
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int DP, bool BF16, bool CAP, bool BIAS>
+int32_t launch_fwd(const FwdArgs& a, int device, cudaStream_t s) {
+  static PerDeviceFlag ready;
+  auto kernel = attn_fwd_kernel<DP, BF16, CAP, BIAS>;
+  if (!ready.test(device)) {
+    LEGO_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, fwd_smem<DP>()));
+    ready.set(device);
+  }
+  const long long ctas = (long long)a.q_tiles * a.p.batch * a.p.q_heads;
+  if (ctas > 0x7fffffffLL) return LEGO_ERR_SIZE;
+  LEGO_CUDA_TRY(launch_overlapped(kernel, dim3((unsigned)ctas), dim3(kFwdThreads), fwd_smem<DP>(), s, a));
+  return LEGO_OK;
+}
+
+template <int DP, bool BF16>
+int32_t launch_fwd_scores(const FwdArgs& a, int device, cudaStream_t s) {
+  // The instance without cap and bias compares raw scores and scales them afterwards, which
+  // needs a positive scale; the bias instance takes the others with a slope of zero.
+  const bool cap = a.p.softcap > 0.f, bias = a.p.slopes || (!cap && !(a.p.scale > 0.f));
+  if (cap) return bias ? launch_fwd<DP, BF16, true, true>(a, device, s) : launch_fwd<DP, BF16, true, false>(a, device, s);
+  return bias ? launch_fwd<DP, BF16, false, true>(a, device, s) : launch_fwd<DP, BF16, false, false>(a, device, s);
+}
+
+}  // namespace
+}  // namespace lego
+
+using namespace lego;
+
+extern "C" int32_t lego_attention_fwd(const lego_attention_t* d, const void* q, const void* k, const void* v, void* o,
+                                      float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+  FwdArgs a = {};
+  int32_t st = attention_problem(d, &a.p);
+  if (st != LEGO_OK) return st;
+  if (!q || !k || !v || !o || !lse) return LEGO_ERR_NULL;
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)workspace) & 15) return LEGO_ERR_ALIGN;
+  const int64_t need = lego_attention_workspace_bytes(d, 0);
+  if (need && !workspace) return LEGO_ERR_NULL;
+  if (workspace_bytes < need) return LEGO_ERR_SIZE;
+  DeviceCtx* ctx = device_ctx(&st);
+  if (!ctx) return st;
+  EncodeFn enc = encode_fn(&st);
+  if (!enc) return st;
+  const AttnProblem& p = a.p;
+  const bool bf16 = d->dtype == LEGO_BF16;
+  const long long o_stride[3] = {(long long)p.q_len * p.q_heads * p.dim, (long long)p.q_heads * p.dim, p.dim};
+  if (make_tmap_heads(enc, &a.q, bf16, q, p.dim, p.q_len, p.q_heads, p.batch, p.q_stride, kTile) != LEGO_OK ||
+      make_tmap_heads(enc, &a.k, bf16, k, p.dim, p.k_len, p.k_heads, p.batch, p.k_stride, kTile) != LEGO_OK ||
+      make_tmap_heads(enc, &a.v, bf16, v, p.dim, p.k_len, p.k_heads, p.batch, p.v_stride, kTile) != LEGO_OK ||
+      make_tmap_heads(enc, &a.o, bf16, o, p.dim, p.q_len, p.q_heads, p.batch, o_stride, 32) != LEGO_OK)
+    return LEGO_ERR_UNSUPPORTED;
+  cudaStream_t s = (cudaStream_t)stream;
+  st = attention_docs(&a.p, workspace, s);
+  if (st != LEGO_OK) return st;
+  a.v_raw = (const uint16_t*)v;
+  a.lse = lse;
+  a.status = ctx->status_word;
+  a.q_tiles = (p.q_len + 2 * kTile - 1) / (2 * kTile);
+  if (p.dim <= 64)
+    return bf16 ? launch_fwd_scores<64, true>(a, ctx->device, s) : launch_fwd_scores<64, false>(a, ctx->device, s);
+  return bf16 ? launch_fwd_scores<128, true>(a, ctx->device, s) : launch_fwd_scores<128, false>(a, ctx->device, s);
+}

@@ -81,4 +81,21 @@ inline int32_t make_tmap_group_major(EncodeFn enc, CUtensorMap* out, CUtensorMap
   return r == CUDA_SUCCESS ? LEGO_OK : LEGO_ERR_UNSUPPORTED;
 }
 
+// 4-D map of a [batch, tokens, heads, dim] tensor of 16-bit values as (dim, token, head, batch),
+// 128-byte swizzle: a box is 64 values of `rows` tokens of one head.  Values past `dim` and
+// tokens past the end read as zeros and are not written.  Strides in elements.
+inline int32_t make_tmap_heads(EncodeFn enc, CUtensorMap* out, bool bf16, const void* base, uint64_t dim,
+                               uint64_t tokens, uint64_t heads, uint64_t batch, const long long* stride,
+                               uint32_t rows) {
+  const cuuint64_t dims[4] = {dim, tokens, heads, batch};
+  const cuuint64_t strides[3] = {(cuuint64_t)stride[1] * 2, (cuuint64_t)stride[2] * 2, (cuuint64_t)stride[0] * 2};
+  const cuuint32_t box[4] = {64, rows, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? LEGO_OK : LEGO_ERR_UNSUPPORTED;
+}
+
 }  // namespace lego
