@@ -98,21 +98,22 @@ __device__ __forceinline__ uint32_t bits_upto(int last, int w) {
 }
 // Clears the columns whose document differs from this lane's: other[w] is the document of
 // column 32 w + lane, own this lane's row's.  All lanes of the warp take part.
-__device__ __forceinline__ void mask_documents(uint32_t (&m)[4], const int (&other)[4], int own) {
-  uint32_t same[4] = {0, 0, 0, 0};
+template <int W>
+__device__ __forceinline__ void mask_documents(uint32_t (&m)[W], const int (&other)[W], int own) {
+  uint32_t same[W] = {};
   uint32_t todo = __ballot_sync(~0u, own >= 0);
   while (todo) {
     const int d = __shfl_sync(~0u, own, __ffs(todo) - 1);
     const bool mine = own == d;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < W; ++w) {
       const uint32_t eq = __ballot_sync(~0u, other[w] == d);
       if (mine) same[w] = eq;
     }
     todo &= ~__ballot_sync(~0u, mine);
   }
 #pragma unroll
-  for (int w = 0; w < 4; ++w) m[w] &= same[w];
+  for (int w = 0; w < W; ++w) m[w] &= same[w];
 }
 
 // ---- tiles in shared memory ----------------------------------------------------------------

@@ -1,0 +1,956 @@
+// Attention backward on tcgen05 (sm_100a).
+//
+//   P = exp(s - lse), dV = P^T dO, dP = dO V^T, dS = P (dP - delta) (1 - tanh^2 of a cap),
+//   dQ = scale dS K, dK = scale dS^T Q, delta = row sum of dO O.
+//
+// Three launches.  A preparation writes delta and the rows' log-sums in the form the others
+// use.  The key kernel takes a tile of 128 keys per CTA and walks the tiles of queries of
+// all heads that share the key head: dK and dV stay in TMEM from the first to the last, so
+// shared heads are summed in a fixed order.  The query kernel takes a tile of 128 queries
+// and walks the keys: dQ stays in TMEM.  Scores are computed in both, seven products instead
+// of the five that one kernel with a sum of dQ over CTAs in memory would take; in return no
+// addition depends on the order in which CTAs happen to run, and there is no dQ in 32 bits to
+// clear, add to and convert.
+//
+// Key kernel: S^T = K Q^T and dP^T = V dO^T into TMEM, one thread per key and half the
+// columns (two warpgroups); P^T and dS^T go back over them as 16-bit pairs and are the TMEM
+// operands of dV += P^T dO and dK += dS^T Q.  The order of issue is dV(n), S(n + 1), dK(n),
+// dP(n + 1): the products of one kind run while the warps work on the other.  All 512
+// columns of TMEM are in use (64-wide heads: 384).  Query kernel: S in two buffers, so the
+// weights of a tile are ready when its dP is.
+//
+// fp16: P is kept times 2^14 (weights of long rows fall below the type's normal range) and dS
+// times a power of two per key head that a bound on it, 2 D max|dO| max|V|, leaves in range;
+// both are taken out of the 32-bit sums at the end.
+#include <cuda.h>
+
+#include "attention.cuh"
+#include "tma_host.cuh"
+
+namespace lego {
+namespace {
+
+constexpr int kBwdThreads = 384;
+constexpr int kBwdRegs = 168, kMathRegs = 216, kBwdOtherRegs = 72;
+static_assert(2 * kMathRegs + kBwdOtherRegs <= 3 * kBwdRegs, "more registers than the launch has would wait forever");
+constexpr int kWeightShift = 14;     // fp16: log2 of the factor on P
+constexpr float kScoreLimit = 30000.f;   // fp16: what the bound on dS is scaled to stay under
+
+struct BwdArgs {
+  CUtensorMap q, k, v, d_o;          // boxes of 128 tokens
+  CUtensorMap dq, dk, dv;            // boxes of 32 tokens
+  AttnProblem p;
+  const uint16_t *q_raw, *k_raw, *o_raw, *do_raw, *v_raw;
+  const float* lse;
+  float *neg_lse, *neg_delta;        // [batch][q_heads][q_len up to whole tiles], log2 units
+  uint32_t* peak;                    // fp16: [batch][k_heads][2] bits of max|dO|, max|V|
+  uint32_t* status;
+};
+
+__device__ __forceinline__ long long row_slot(const AttnProblem& p, int b, int h) {
+  return ((long long)b * p.q_heads + h) * tiles_of(p.q_len) * kTile;
+}
+
+// fp16: the power of two dS is kept times, from the peaks of one key head.
+__device__ __forceinline__ float score_factor(const BwdArgs& a, int b, int hk) {
+  const uint32_t* pk = a.peak + ((long long)b * a.p.k_heads + hk) * 2;
+  const float bound = 2.f * a.p.dim * __uint_as_float(pk[0]) * __uint_as_float(pk[1]);
+  if (!(bound > 1e-30f) || !(bound < 1e30f)) return 1.f;
+  return ldexpf(1.f, ilogbf(kScoreLimit / bound));
+}
+
+// A maximum over many rows: most rows find a larger one there already and leave it.
+__device__ __forceinline__ void raise_peak(uint32_t* at, uint32_t bits) {
+  if (bits > __ldcg(at)) atomicMax(at, bits);
+}
+
+// ---- preparation -----------------------------------------------------------------------------
+
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if constexpr (BF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+
+// A warp per row, four values a lane: delta, the negated log-sum, and in fp16 the peaks of dO
+// and V.  Rows past q_len (whole tiles) and padding get weight zero: -inf.  Memory bound; the
+// peaks are maxima, so the order of the atomics does not matter.
+template <bool BF16>
+__global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __grid_constant__ BwdArgs a) {
+  const AttnProblem& p = a.p;
+  ptx::grid_dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int padded = tiles_of(p.q_len) * kTile;
+  const long long rows = (long long)p.batch * padded * p.q_heads;
+  if (id < rows) {
+    const int h = (int)(id % p.q_heads), i = (int)(id / p.q_heads % padded), b = (int)(id / p.q_heads / padded);
+    float delta = 0.f, peak = 0.f, nl = -INFINITY;
+    const bool real = i < p.q_len &&
+                      (!p.documents || p.documents[(long long)b * p.k_len + p.offset + i] >= 0);
+    if (real) {
+      const long long at = (((long long)b * p.q_len + i) * p.q_heads + h) * p.dim;
+      if (lane * 4 < p.dim) {
+        const uint2 x = *reinterpret_cast<const uint2*>(a.o_raw + at + lane * 4);
+        const uint2 g = *reinterpret_cast<const uint2*>(a.do_raw + at + lane * 4);
+        const float2 x0 = unpack2<BF16>(x.x), x1 = unpack2<BF16>(x.y), g0 = unpack2<BF16>(g.x), g1 = unpack2<BF16>(g.y);
+        delta = fmaf(x0.x, g0.x, fmaf(x0.y, g0.y, fmaf(x1.x, g1.x, x1.y * g1.y)));
+        peak = fmaxf(fmaxf(fabsf(g0.x), fabsf(g0.y)), fmaxf(fabsf(g1.x), fabsf(g1.y)));
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) delta += __shfl_xor_sync(~0u, delta, o);
+      const float ls = a.lse[((long long)b * p.q_heads + h) * p.q_len + i];
+      if (ls > -INFINITY) nl = -ls * kLog2e + (BF16 ? 0.f : (float)kWeightShift);
+      if (!BF16) {
+        const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(peak));
+        if (lane == 0) raise_peak(a.peak + ((long long)b * p.k_heads + h / p.group) * 2, top);
+      }
+    }
+    if (lane == 0) {
+      const long long at = row_slot(p, b, h) + i;
+      a.neg_lse[at] = nl;
+      a.neg_delta[at] = -delta;
+    }
+    return;
+  }
+  if (BF16) return;
+  const long long key = id - rows;
+  if (key >= (long long)p.batch * p.k_len * p.k_heads) return;
+  const int h = (int)(key % p.k_heads), j = (int)(key / p.k_heads % p.k_len), b = (int)(key / p.k_heads / p.k_len);
+  if (p.documents && p.documents[(long long)b * p.k_len + j] < 0) return;
+  float peak = 0.f;
+  if (lane * 4 < p.dim) {
+    const uint2 x = *reinterpret_cast<const uint2*>(a.v_raw + b * p.v_stride[0] + j * p.v_stride[1] + h * p.v_stride[2] + lane * 4);
+    const float2 x0 = unpack2<BF16>(x.x), x1 = unpack2<BF16>(x.y);
+    peak = fmaxf(fmaxf(fabsf(x0.x), fabsf(x0.y)), fmaxf(fabsf(x1.x), fabsf(x1.y)));
+  }
+  const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(peak));
+  if (lane == 0) raise_peak(a.peak + ((long long)b * p.k_heads + h) * 2 + 1, top);
+}
+
+// ---- shared by the two product kernels ---------------------------------------------------------
+
+struct Scores {      // log2 units, as in the forward pass
+  float by, u_by, cap_by, slope;
+};
+template <bool CAP>
+__device__ __forceinline__ Scores scores_of(const AttnProblem& p, int h) {
+  Scores s;
+  s.by = p.scale * kLog2e;
+  s.u_by = CAP ? 2.f * kLog2e * p.scale / p.softcap : 0.f;
+  s.cap_by = p.softcap * kLog2e;
+  s.slope = p.slopes ? p.slopes[h] * kLog2e : 0.f;
+  return s;
+}
+
+// A pair of raw scores -> weights x = 2^(z + nl) and what the score gradient is multiplied by,
+// w = x (1 - tanh^2).  far: distances.
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ void weights(float2 s, float2 nl, const Scores& sc, float2 far, float2* x, float2* w) {
+  float2 z;
+  float2 bend = make_float2(1.f, 1.f);
+  if (CAP) {
+    const float2 t = make_float2(tanh_of(s.x * sc.u_by), tanh_of(s.y * sc.u_by));
+    z = ptx::fma2(t, make_float2(sc.cap_by, sc.cap_by), nl);
+    bend = ptx::fma2(make_float2(-t.x, -t.y), t, bend);
+  } else {
+    z = ptx::fma2(s, make_float2(sc.by, sc.by), nl);
+  }
+  if (BIAS) z = ptx::fma2(make_float2(-sc.slope, -sc.slope), far, z);
+  *x = make_float2(ex2(z.x), ex2(z.y));
+  *w = CAP ? ptx::mul2(*x, bend) : *x;
+}
+
+// 16-bit rows of 32 lanes x DP columns of TMEM, times `by`, staged and stored by TMA.
+template <int DP, bool BF16>
+__device__ __forceinline__ void store_rows(const CUtensorMap* map, uint32_t tmem, bool any, float by, uint8_t* stage,
+                                           int row0, int head, int b, int lane) {
+#pragma unroll
+  for (int c = 0; c < DP; c += 32) {
+    uint32_t o[32];
+    if (any) {
+      ptx::tmem_ld_32x32(tmem + c, o);
+      ptx::tmem_ld_wait();
+    }
+    uint8_t* dst = stage + (c >> 6) * kBoxBytes + lane * 128;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[k] = any ? pack2<BF16>(__uint_as_float(o[8 * i + 2 * k]) * by, __uint_as_float(o[8 * i + 2 * k + 1]) * by) : 0u;
+      *reinterpret_cast<uint4*>(dst + (((((c & 32) >> 3) + i) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  ptx::fence_proxy_async();
+  __syncwarp();
+  if (lane == 0) {
+#pragma unroll
+    for (int c = 0; c < DP / 64; ++c) {
+      const int32_t at[5] = {c * 64, row0, head, b, 0};
+      ptx::tma_store_nd(4, map, at, ptx::smem_u32(stage) + c * kBoxBytes);
+    }
+    ptx::bulk_commit_group();
+    ptx::bulk_wait_group_read<0>();
+  }
+}
+
+// TMEM column of 16 tokens' packed pairs: a warpgroup's half of the columns lies over the
+// scores that this warpgroup has read, the first half at 0, the second at 64.
+__device__ __forceinline__ uint32_t packed_at(int step) { return (step < 4 ? 0 : 64) + (step & 3) * 8; }
+
+// ---- dK, dV --------------------------------------------------------------------------------------
+
+template <int DP> constexpr int key_stages() { return DP == 128 ? 2 : 4; }
+template <int DP> constexpr int key_smem() {
+  return (2 + 2 * key_stages<DP>()) * tile_bytes<DP>() + key_stages<DP>() * 1024 + 1024 + 512;
+}
+
+struct KeyShared {
+  uint64_t kv_full[2], s_full, p_full, dp_full, ds_full, acc_full;
+  uint64_t q_full[4], q_empty[4], do_full[4], do_empty[4];
+  int lo, hi;
+  uint32_t tmem_base, abort_flag;
+};
+
+template <int DP, bool BF16, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __grid_constant__ BwdArgs a) {
+  constexpr int TILE = tile_bytes<DP>(), NS = key_stages<DP>();
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = ptx::smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  // K, V, ring of Q, ring of dO, ring of the rows' (-lse, -delta)
+  float* stats = reinterpret_cast<float*>(smem + (2 + 2 * NS) * TILE);
+  KeyShared* sh = reinterpret_cast<KeyShared*>(smem + (2 + 2 * NS) * TILE + NS * 1024);
+  volatile uint32_t* abort_flag = &sh->abort_flag;
+  const uint32_t k_smem = ptx::smem_u32(smem), v_smem = k_smem + TILE, q_smem = v_smem + TILE, do_smem = q_smem + NS * TILE;
+  const AttnProblem& p = a.p;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int heads = p.batch * p.k_heads;
+  const int kt = (int)(blockIdx.x / heads);      // the first keys, which most queries see, come first
+  const int b = blockIdx.x % heads / p.k_heads, hk = blockIdx.x % heads % p.k_heads;
+  const int j0 = kt * kTile;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) ptx::mbar_init(ptx::smem_u32(&sh->kv_full[t]), 1);
+    ptx::mbar_init(ptx::smem_u32(&sh->s_full), 1);
+    ptx::mbar_init(ptx::smem_u32(&sh->p_full), 8);
+    ptx::mbar_init(ptx::smem_u32(&sh->dp_full), 1);
+    ptx::mbar_init(ptx::smem_u32(&sh->ds_full), 8);
+    ptx::mbar_init(ptx::smem_u32(&sh->acc_full), 1);
+    for (int s = 0; s < NS; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&sh->q_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&sh->q_empty[s]), 1 + 8);    // the MMAs, and the warps done with the row sums
+      ptx::mbar_init(ptx::smem_u32(&sh->do_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&sh->do_empty[s]), 1);
+    }
+    sh->abort_flag = 0;
+    ptx::fence_barrier_init();
+    ptx::fence_proxy_async();
+    ptx::prefetch_tensormap(&a.q);
+    ptx::prefetch_tensormap(&a.k);
+    ptx::prefetch_tensormap(&a.v);
+    ptx::prefetch_tensormap(&a.d_o);
+  }
+  if (warp == 9) {
+    ptx::tmem_alloc(ptx::smem_u32(&sh->tmem_base), 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::grid_dependency_wait();
+  const int prefix = prefix_of(p, b);
+  if (warp == 0) {   // tiles of queries that see some key of the tile
+    const int nq = tiles_of(p.q_len);
+    int lo = 0, hi = nq;
+    if (p.causal && j0 >= prefix) {      // from the query at position j0 on
+      const int first = j0 - p.offset;
+      lo = first <= 0 ? 0 : first >= p.q_len ? nq : first / kTile;
+    }
+    if (p.documents && lo < hi) {
+      const int4 mine = p.key_docs[(long long)b * tiles_of(p.k_len) + kt];
+      const int4* qd = p.query_docs + (long long)b * nq;
+      int first = hi, last = -1;
+      for (int i = lo + lane; i < hi; i += 32)
+        if (docs_meet(qd[i], mine)) {
+          if (i < first) first = i;
+          last = i;
+        }
+      lo = __reduce_min_sync(~0u, first);
+      hi = __reduce_max_sync(~0u, last) + 1;
+    }
+    if (lane == 0) {
+      sh->lo = lo;
+      sh->hi = hi > lo ? hi : lo;
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = sh->tmem_base;
+  const uint32_t s_at = tmem, dp_at = tmem + kTile, dv_at = tmem + 2 * kTile, dk_at = dv_at + DP;
+  const int lo = sh->lo, per_head = sh->hi - lo, steps = per_head * p.group;
+
+  if (warp >= 8) {
+    ptx::regs_less<kBwdOtherRegs>();
+    if (warp == 8 && steps > 0) {
+      // ---------------- loads ----------------
+      bool ok = true;
+      if (lane == 0)
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t bar = ptx::smem_u32(&sh->kv_full[t]);
+          ptx::mbar_arrive_expect_tx(bar, TILE);
+          for (int c = 0; c < DP / 64; ++c) {
+            const int32_t at[5] = {c * 64, j0, hk, b, 0};
+            ptx::tma_load_nd(4, (t ? v_smem : k_smem) + c * kBoxBytes, t ? &a.v : &a.k, at, bar);
+          }
+        }
+      const int4* qd = p.documents ? p.query_docs + (long long)b * tiles_of(p.q_len) : nullptr;
+      int n = 0;
+      for (; ok && n < steps; ++n) {
+        const int h = hk * p.group + n / per_head, i = lo + n % per_head;
+        const uint32_t slot = n % NS, parity = ((n / NS) & 1) ^ 1;
+        const bool dirty = qd && qd[i].z;
+        for (int g = 0; g < 2; ++g) {       // Q with the rows' sums, then dO
+          const uint32_t full = ptx::smem_u32(g ? &sh->do_full[slot] : &sh->q_full[slot]);
+          if (lane == 0)
+            ok = ptx::mbar_wait_bounded(ptx::smem_u32(g ? &sh->do_empty[slot] : &sh->q_empty[slot]), parity, abort_flag, kAttnWait);
+          ok = __shfl_sync(~0u, ok ? 1 : 0, 0);
+          if (!ok) {
+            if (lane == 0) attn_fail(a.status, abort_flag, 0x510000u | slot);
+            break;
+          }
+          const uint32_t tile = (g ? do_smem : q_smem) + slot * TILE;
+          if (dirty) {     // padding among the queries must not meet a zero weight
+            const uint16_t* base = g ? a.do_raw + ((long long)b * p.q_len * p.q_heads + h) * p.dim
+                                     : a.q_raw + b * p.q_stride[0] + h * p.q_stride[2];
+            copy_tile_clean<DP>(smem + (tile - k_smem), base, g ? (long long)p.q_heads * p.dim : p.q_stride[1], p.dim,
+                                i * kTile, p.q_len, p.documents + (long long)b * p.k_len + p.offset, lane);
+          }
+          if (lane == 0) {
+            const uint32_t bytes = (dirty ? 0 : TILE) + (g ? 0 : 1024);
+            if (bytes) ptx::mbar_arrive_expect_tx(full, bytes);
+            else ptx::mbar_arrive(full);
+            if (!dirty)
+              for (int c = 0; c < DP / 64; ++c) {
+                const int32_t at[5] = {c * 64, i * kTile, h, b, 0};
+                ptx::tma_load_nd(4, tile + c * kBoxBytes, g ? &a.d_o : &a.q, at, full);
+              }
+            if (!g) {
+              const long long at = row_slot(p, b, h) + i * kTile;
+              ptx::bulk_load(ptx::smem_u32(stats + slot * 256), a.neg_lse + at, 512, full);
+              ptx::bulk_load(ptx::smem_u32(stats + slot * 256 + 128), a.neg_delta + at, 512, full);
+            }
+          }
+        }
+      }
+      if (lane == 0 && *abort_flag) {   // leave no copy in flight
+        uint32_t never = 0;
+        for (int t = 0; t < 2; ++t) ptx::mbar_wait_bounded(ptx::smem_u32(&sh->kv_full[t]), 0, &never, kAttnWait);
+        for (int s = 0; s < NS; ++s)
+          if (n > s) {
+            ptx::mbar_wait_bounded(ptx::smem_u32(&sh->q_full[s]), ((n - 1 - s) / NS) & 1, &never, kAttnWait);
+            ptx::mbar_wait_bounded(ptx::smem_u32(&sh->do_full[s]), ((n - 1 - s) / NS) & 1, &never, kAttnWait);
+          }
+      }
+    } else if (warp == 9 && lane == 0 && steps > 0) {
+      // ---------------- MMA issue ----------------
+      const uint32_t id_s = idesc_of<BF16>(kTile, false), id_d = idesc_of<BF16>(DP, true);
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
+        if (ok && !ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait)) {
+          attn_fail(a.status, abort_flag, code);
+          ok = false;
+        }
+        ptx::tc_fence_after();
+      };
+      auto score_product = [&](uint32_t d, uint32_t own, uint32_t other, uint64_t* bar) {
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) ptx::mma_f16_ss(d, desc_k_major(own, s), desc_k_major(other, s), id_s, s != 0);
+        ptx::mma_commit(ptx::smem_u32(bar));
+      };
+      auto sum_product = [&](uint32_t d, uint32_t w, uint32_t other, bool add, uint64_t* bar) {
+#pragma unroll
+        for (int s = 0; s < kTile / 16; ++s) ptx::mma_f16_ts(d, w + packed_at(s), desc_mn_major(other, s), id_d, add || s != 0);
+        ptx::mma_commit(ptx::smem_u32(bar));
+      };
+      wait(&sh->kv_full[0], 0, 0x520000u);
+      wait(&sh->q_full[0], 0, 0x520001u);
+      if (ok) score_product(s_at, k_smem, q_smem, &sh->s_full);
+      wait(&sh->kv_full[1], 0, 0x520002u);
+      wait(&sh->do_full[0], 0, 0x520003u);
+      if (ok) score_product(dp_at, v_smem, do_smem, &sh->dp_full);
+      for (int n = 0; ok && n < steps; ++n) {
+        const uint32_t slot = n % NS, next = (n + 1) % NS, next_parity = ((n + 1) / NS) & 1;
+        const bool more = n + 1 < steps;
+        wait(&sh->p_full, n & 1, 0x530000u);
+        if (!ok) break;
+        sum_product(dv_at, s_at, do_smem + slot * TILE, n != 0, &sh->do_empty[slot]);
+        if (more) {
+          wait(&sh->q_full[next], next_parity, 0x530001u);
+          if (!ok) break;
+          score_product(s_at, k_smem, q_smem + next * TILE, &sh->s_full);
+        }
+        wait(&sh->ds_full, n & 1, 0x530002u);
+        if (!ok) break;
+        sum_product(dk_at, dp_at, q_smem + slot * TILE, n != 0, &sh->q_empty[slot]);
+        if (more) {
+          wait(&sh->do_full[next], next_parity, 0x530003u);
+          if (!ok) break;
+          score_product(dp_at, v_smem, do_smem + next * TILE, &sh->dp_full);
+        }
+      }
+      if (ok) ptx::mma_commit(ptx::smem_u32(&sh->acc_full));
+    }
+  } else {
+    ptx::regs_more<kMathRegs>();
+    // ---------------- weights and score gradients, epilogue ----------------
+    const int half = warp >> 2, quarter = warp & 3;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_tmem = s_at + lanes + half * 64, dp_tmem = dp_at + lanes + half * 64;
+    const int key = j0 + quarter * 32 + lane;
+    const float ds_factor = BF16 ? 1.f : score_factor(a, b, hk);
+    const float w_by = BF16 ? 1.f : ldexpf(ds_factor, -kWeightShift);
+    int own_doc = -1;
+    int4 tile_docs = make_int4(0, 0, 0, 0);
+    const int* docs = nullptr;      // of query 0 on
+    const int4* qd = nullptr;
+    if (p.documents && steps > 0) {
+      docs = p.documents + (long long)b * p.k_len + p.offset;
+      qd = p.query_docs + (long long)b * tiles_of(p.q_len);
+      if (key < p.k_len) own_doc = p.documents[(long long)b * p.k_len + key];
+      tile_docs = p.key_docs[(long long)b * tiles_of(p.k_len) + kt];
+    }
+    const bool behind = !p.causal || key < prefix;       // seen from every position
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
+      if (!ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait)) ok = false;
+      if (!__all_sync(~0u, ok)) {
+        if (lane == 0) attn_fail(a.status, abort_flag, code);
+        ok = false;
+      }
+      ptx::tc_fence_after();
+      return ok;
+    };
+    for (int n = 0; n < steps; ++n) {
+      const int h = hk * p.group + n / per_head, i0 = (lo + n % per_head) * kTile;
+      const uint32_t slot = n % NS;
+      const Scores sc = scores_of<CAP>(p, h);
+      // seen whole: the first query sees the last key (queries past the end have weight zero)
+      bool masked = p.causal && last_key(p, prefix, i0 + p.offset) < j0 + kTile - 1;
+      if (qd) masked = masked || !docs_same(qd[lo + n % per_head], tile_docs);
+      const float4* nl4 = reinterpret_cast<const float4*>(stats + slot * 256 + half * 64);
+      const float4* nd4 = nl4 + 32;
+      // the row sums arrive with Q, before the scores made from it
+      if (!wait(&sh->q_full[slot], (n / NS) & 1, 0x540000u) || !wait(&sh->s_full, n & 1, 0x540001u)) break;
+      float w[64];
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) ptx::tmem_ld_32x32(s_tmem + c, reinterpret_cast<uint32_t*>(w) + c);
+      ptx::tmem_ld_wait();
+      uint32_t see[2] = {~0u, ~0u};
+      if (masked) {
+        if (!behind) {
+          const int first = key - p.offset - i0 - half * 64;      // column of the first query at the key's position or past it
+          see[0] = ~bits_upto(first - 1, 0);
+          see[1] = ~bits_upto(first - 1, 1);
+        }
+        if (docs) {
+          int other[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int i = i0 + half * 64 + x * 32 + lane;
+            other[x] = i < p.q_len ? docs[i] : -1;
+          }
+          mask_documents(see, other, own_doc);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 nl = nl4[(c + e) >> 2];
+          float2 far[2];
+          if (BIAS) {
+            const float d = (float)(i0 + half * 64 + c + e + p.offset - key);
+            far[0] = make_float2(fabsf(d), fabsf(d + 1.f));
+            far[1] = make_float2(fabsf(d + 2.f), fabsf(d + 3.f));
+          }
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int at = c + e + 2 * x;
+            float2 px, pw;
+            weights<CAP, BIAS>(make_float2(w[at], w[at + 1]), x ? make_float2(nl.z, nl.w) : make_float2(nl.x, nl.y), sc,
+                               far[x], &px, &pw);
+            if (masked) {
+              if (!((see[at >> 5] >> (at & 31)) & 1u)) px.x = pw.x = 0.f;
+              if (!((see[at >> 5] >> ((at + 1) & 31)) & 1u)) px.y = pw.y = 0.f;
+            }
+            packed[(e + 2 * x) >> 1] = pack2<BF16>(px.x, px.y);
+            w[at] = pw.x;
+            w[at + 1] = pw.y;
+          }
+        }
+        ptx::tmem_st_32x16(s_tmem + c / 2, packed);
+      }
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->p_full));
+
+      if (!wait(&sh->dp_full, n & 1, 0x540002u)) break;
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        float d[32];
+        ptx::tmem_ld_32x32(dp_tmem + c, reinterpret_cast<uint32_t*>(d));
+        ptx::tmem_ld_wait();
+        uint32_t packed[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 nd = nd4[(c + e) >> 2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int at = c + e + 2 * x;
+            float2 f = make_float2(w[at], w[at + 1]);
+            if (!BF16) f = ptx::mul2(f, make_float2(w_by, w_by));
+            float2 g = ptx::add2(make_float2(d[e + 2 * x], d[e + 2 * x + 1]), x ? make_float2(nd.z, nd.w) : make_float2(nd.x, nd.y));
+            g = ptx::mul2(f, g);
+            if (masked) {     // not 0 * infinity
+              if (!((see[at >> 5] >> (at & 31)) & 1u)) g.x = 0.f;
+              if (!((see[at >> 5] >> ((at + 1) & 31)) & 1u)) g.y = 0.f;
+            }
+            packed[(e + 2 * x) >> 1] = pack2<BF16>(g.x, g.y);
+          }
+        }
+        // over the columns this warp has read: 0 .. 15 first, then 16 .. 31 of its half
+        ptx::tmem_st_32x16(dp_tmem + c / 2, packed);
+      }
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        ptx::mbar_arrive(ptx::smem_u32(&sh->ds_full));
+        ptx::mbar_arrive(ptx::smem_u32(&sh->q_empty[slot]));    // done with the row sums
+      }
+    }
+    if (ok && steps > 0) wait(&sh->acc_full, 0, 0x550000u);
+    const int row0 = j0 + quarter * 32;
+    if (ok && row0 < p.k_len) {      // staged where K and V were
+      if (half == 0)
+        store_rows<DP, BF16>(&a.dv, dv_at + lanes, steps > 0, BF16 ? 1.f : ldexpf(1.f, -kWeightShift),
+                             smem + TILE + quarter * 4096, row0, hk, b, lane);
+      else
+        store_rows<DP, BF16>(&a.dk, dk_at + lanes, steps > 0, p.scale / ds_factor, smem + quarter * 4096, row0, hk, b, lane);
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- dQ --------------------------------------------------------------------------------------------
+
+template <int DP> constexpr int query_k_stages() { return DP == 128 ? 3 : 4; }
+template <int DP> constexpr int query_v_stages() { return DP == 128 ? 2 : 3; }
+template <int DP> constexpr int query_smem() {
+  return (2 + query_k_stages<DP>() + query_v_stages<DP>()) * tile_bytes<DP>() + 1024 + 512;
+}
+
+struct QueryShared {
+  uint64_t q_full[2], s_full[2], dp_full, ds_full, acc_full;
+  uint64_t k_full[4], k_empty[4], v_full[3], v_empty[3];
+  int lo, hi;
+  uint32_t tmem_base, abort_flag;
+};
+
+template <int DP, bool BF16, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const __grid_constant__ BwdArgs a) {
+  constexpr int TILE = tile_bytes<DP>(), NK = query_k_stages<DP>(), NV = query_v_stages<DP>();
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = ptx::smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  QueryShared* sh = reinterpret_cast<QueryShared*>(smem + (2 + NK + NV) * TILE);
+  volatile uint32_t* abort_flag = &sh->abort_flag;
+  const uint32_t q_smem = ptx::smem_u32(smem), do_smem = q_smem + TILE, k_smem = do_smem + TILE, v_smem = k_smem + NK * TILE;
+  const AttnProblem& p = a.p;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int heads = p.batch * p.q_heads;
+  const int qt = tiles_of(p.q_len) - 1 - (int)(blockIdx.x / heads);
+  const int b = blockIdx.x % heads / p.q_heads, h = blockIdx.x % heads % p.q_heads, hk = h / p.group;
+  const int q0 = qt * kTile;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      ptx::mbar_init(ptx::smem_u32(&sh->q_full[t]), 1);
+      ptx::mbar_init(ptx::smem_u32(&sh->s_full[t]), 1);
+    }
+    ptx::mbar_init(ptx::smem_u32(&sh->dp_full), 1);
+    ptx::mbar_init(ptx::smem_u32(&sh->ds_full), 8);
+    ptx::mbar_init(ptx::smem_u32(&sh->acc_full), 1);
+    for (int s = 0; s < NK; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&sh->k_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&sh->k_empty[s]), 1);
+    }
+    for (int s = 0; s < NV; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&sh->v_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&sh->v_empty[s]), 1);
+    }
+    sh->abort_flag = 0;
+    ptx::fence_barrier_init();
+    ptx::fence_proxy_async();
+    ptx::prefetch_tensormap(&a.q);
+    ptx::prefetch_tensormap(&a.k);
+    ptx::prefetch_tensormap(&a.v);
+    ptx::prefetch_tensormap(&a.d_o);
+  }
+  if (warp == 9) {
+    ptx::tmem_alloc(ptx::smem_u32(&sh->tmem_base), 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::grid_dependency_wait();
+  const int prefix = prefix_of(p, b);
+  const int4* kd = p.documents ? p.key_docs + (long long)b * tiles_of(p.k_len) : nullptr;
+  if (warp == 0) {
+    const int last_row = q0 + kTile - 1 < p.q_len - 1 ? q0 + kTile - 1 : p.q_len - 1;
+    int lo = 0, hi = tiles_of(last_key(p, prefix, last_row + p.offset) + 1);
+    if (hi < 0) hi = 0;
+    if (kd) {
+      const int4 mine = p.query_docs[(long long)b * tiles_of(p.q_len) + qt];
+      int first = hi, last = -1;
+      for (int j = lane; j < hi; j += 32)
+        if (docs_meet(kd[j], mine)) {
+          if (j < first) first = j;
+          last = j;
+        }
+      lo = __reduce_min_sync(~0u, first);
+      hi = __reduce_max_sync(~0u, last) + 1;
+    }
+    if (lane == 0) {
+      sh->lo = lo;
+      sh->hi = hi > lo ? hi : lo;
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = sh->tmem_base;
+  const uint32_t s_at = tmem, dp_at = tmem + 2 * kTile, dq_at = tmem + 3 * kTile;
+  const int lo = sh->lo, steps = sh->hi - lo;
+
+  if (warp >= 8) {
+    ptx::regs_less<kBwdOtherRegs>();
+    if (warp == 8 && steps > 0) {
+      // ---------------- loads ----------------
+      bool ok = true;
+      if (lane == 0)
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t bar = ptx::smem_u32(&sh->q_full[t]);
+          ptx::mbar_arrive_expect_tx(bar, TILE);
+          for (int c = 0; c < DP / 64; ++c) {
+            const int32_t at[5] = {c * 64, q0, h, b, 0};
+            ptx::tma_load_nd(4, (t ? do_smem : q_smem) + c * kBoxBytes, t ? &a.d_o : &a.q, at, bar);
+          }
+        }
+      int n = 0;
+      for (; ok && n < steps; ++n) {
+        const int j = lo + n;
+        for (int g = 0; g < 2; ++g) {
+          const uint32_t slot = n % (g ? NV : NK), parity = ((n / (g ? NV : NK)) & 1) ^ 1;
+          const uint32_t full = ptx::smem_u32(g ? &sh->v_full[slot] : &sh->k_full[slot]);
+          if (lane == 0)
+            ok = ptx::mbar_wait_bounded(ptx::smem_u32(g ? &sh->v_empty[slot] : &sh->k_empty[slot]), parity, abort_flag, kAttnWait);
+          ok = __shfl_sync(~0u, ok ? 1 : 0, 0);
+          if (!ok) {
+            if (lane == 0) attn_fail(a.status, abort_flag, 0x610000u | slot);
+            break;
+          }
+          if (!g && kd && kd[j].z) {   // padding among the keys must not meet a zero score gradient
+            copy_tile_clean<DP>(smem + (2 + slot) * TILE, a.k_raw + b * p.k_stride[0] + hk * p.k_stride[2], p.k_stride[1],
+                                p.dim, j * kTile, p.k_len, p.documents + (long long)b * p.k_len, lane);
+            if (lane == 0) ptx::mbar_arrive(full);
+          } else if (lane == 0) {
+            ptx::mbar_arrive_expect_tx(full, TILE);
+            for (int c = 0; c < DP / 64; ++c) {
+              const int32_t at[5] = {c * 64, j * kTile, hk, b, 0};
+              ptx::tma_load_nd(4, (g ? v_smem : k_smem) + slot * TILE + c * kBoxBytes, g ? &a.v : &a.k, at, full);
+            }
+          }
+        }
+      }
+      if (lane == 0 && *abort_flag) {   // leave no copy in flight
+        uint32_t never = 0;
+        for (int t = 0; t < 2; ++t) ptx::mbar_wait_bounded(ptx::smem_u32(&sh->q_full[t]), 0, &never, kAttnWait);
+        for (int s = 0; s < NK; ++s)
+          if (n > s) ptx::mbar_wait_bounded(ptx::smem_u32(&sh->k_full[s]), ((n - 1 - s) / NK) & 1, &never, kAttnWait);
+        for (int s = 0; s < NV; ++s)
+          if (n > s) ptx::mbar_wait_bounded(ptx::smem_u32(&sh->v_full[s]), ((n - 1 - s) / NV) & 1, &never, kAttnWait);
+      }
+    } else if (warp == 9 && lane == 0 && steps > 0) {
+      // ---------------- MMA issue ----------------
+      const uint32_t id_s = idesc_of<BF16>(kTile, false), id_d = idesc_of<BF16>(DP, true);
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
+        if (ok && !ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait)) {
+          attn_fail(a.status, abort_flag, code);
+          ok = false;
+        }
+        ptx::tc_fence_after();
+      };
+      auto score = [&](int n) {        // S(n) = Q K(n)
+        if (n >= steps) return;
+        wait(&sh->k_full[n % NK], (n / NK) & 1, 0x620000u);
+        if (!ok) return;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+          ptx::mma_f16_ss(s_at + (n & 1) * kTile, desc_k_major(q_smem, s), desc_k_major(k_smem + (n % NK) * TILE, s), id_s, s != 0);
+        ptx::mma_commit(ptx::smem_u32(&sh->s_full[n & 1]));
+      };
+      auto grad = [&](int n) {         // dP(n) = dO V(n)
+        if (n >= steps) return;
+        wait(&sh->v_full[n % NV], (n / NV) & 1, 0x620001u);
+        if (!ok) return;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+          ptx::mma_f16_ss(dp_at, desc_k_major(do_smem, s), desc_k_major(v_smem + (n % NV) * TILE, s), id_s, s != 0);
+        ptx::mma_commit(ptx::smem_u32(&sh->dp_full));
+        ptx::mma_commit(ptx::smem_u32(&sh->v_empty[n % NV]));
+      };
+      wait(&sh->q_full[0], 0, 0x620002u);
+      if (ok) score(0);
+      wait(&sh->q_full[1], 0, 0x620003u);
+      if (ok) grad(0);
+      if (ok) score(1);
+      for (int n = 0; ok && n < steps; ++n) {
+        wait(&sh->ds_full, n & 1, 0x630000u);
+        if (!ok) break;
+#pragma unroll
+        for (int s = 0; s < kTile / 16; ++s)
+          ptx::mma_f16_ts(dq_at, dp_at + packed_at(s), desc_mn_major(k_smem + (n % NK) * TILE, s), id_d, (n | s) != 0);
+        ptx::mma_commit(ptx::smem_u32(&sh->k_empty[n % NK]));
+        grad(n + 1);
+        if (ok) score(n + 2);
+      }
+      if (ok) ptx::mma_commit(ptx::smem_u32(&sh->acc_full));
+    }
+  } else {
+    ptx::regs_more<kMathRegs>();
+    // ---------------- score gradients, epilogue ----------------
+    const int half = warp >> 2, quarter = warp & 3;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t dp_tmem = dp_at + lanes + half * 64;
+    const int row = q0 + quarter * 32 + lane, pos = row + p.offset;
+    const int last = last_key(p, prefix, pos), last_first = last_key(p, prefix, q0 + p.offset);
+    const Scores sc = scores_of<CAP>(p, h);
+    const float ds_factor = BF16 ? 1.f : score_factor(a, b, hk);
+    const float w_by = BF16 ? 1.f : ldexpf(ds_factor, -kWeightShift);
+    const long long slot = row_slot(p, b, h) + row;
+    const float nl = a.neg_lse[slot], nd = a.neg_delta[slot];
+    const float2 nl2 = make_float2(nl, nl), nd2 = make_float2(nd, nd);
+    int own_doc = -1;
+    int4 tile_docs = make_int4(0, 0, 0, 0);
+    const int* docs = nullptr;
+    if (kd && steps > 0) {
+      docs = p.documents + (long long)b * p.k_len;
+      if (row < p.q_len) own_doc = docs[pos];
+      tile_docs = p.query_docs[(long long)b * tiles_of(p.q_len) + qt];
+    }
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
+      if (!ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait)) ok = false;
+      if (!__all_sync(~0u, ok)) {
+        if (lane == 0) attn_fail(a.status, abort_flag, code);
+        ok = false;
+      }
+      ptx::tc_fence_after();
+      return ok;
+    };
+    for (int n = 0; n < steps; ++n) {
+      const int j0 = (lo + n) * kTile;
+      bool masked = j0 + kTile - 1 > last_first;
+      if (kd) masked = masked || !docs_same(kd[lo + n], tile_docs);
+      if (!wait(&sh->s_full[n & 1], (n >> 1) & 1, 0x640000u)) break;
+      const uint32_t s_tmem = s_at + lanes + (n & 1) * kTile + half * 64;
+      float w[64];
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) ptx::tmem_ld_32x32(s_tmem + c, reinterpret_cast<uint32_t*>(w) + c);
+      ptx::tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        float2 far, px, pw;
+        if (BIAS) {
+          const float d = (float)(pos - j0 - half * 64 - c);
+          far = make_float2(fabsf(d), fabsf(d - 1.f));
+        }
+        weights<CAP, BIAS>(make_float2(w[c], w[c + 1]), nl2, sc, far, &px, &pw);
+        if (!BF16) pw = ptx::mul2(pw, make_float2(w_by, w_by));
+        w[c] = pw.x;
+        w[c + 1] = pw.y;
+      }
+      uint32_t see[2] = {~0u, ~0u};
+      if (masked) {
+        see[0] = bits_upto(last - j0 - half * 64, 0);
+        see[1] = bits_upto(last - j0 - half * 64, 1);
+        if (docs) {
+          int other[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int j = j0 + half * 64 + x * 32 + lane;
+            other[x] = j < p.k_len ? docs[j] : -1;
+          }
+          mask_documents(see, other, own_doc);
+        }
+      }
+      if (!wait(&sh->dp_full, n & 1, 0x640001u)) break;
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        float d[32];
+        ptx::tmem_ld_32x32(dp_tmem + c, reinterpret_cast<uint32_t*>(d));
+        ptx::tmem_ld_wait();
+        uint32_t packed[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const int at = c + e;
+          float2 g = ptx::add2(make_float2(d[e], d[e + 1]), nd2);
+          g = ptx::mul2(make_float2(w[at], w[at + 1]), g);
+          if (masked) {
+            if (!((see[at >> 5] >> (at & 31)) & 1u)) g.x = 0.f;
+            if (!((see[at >> 5] >> ((at + 1) & 31)) & 1u)) g.y = 0.f;
+          }
+          packed[e >> 1] = pack2<BF16>(g.x, g.y);
+        }
+        ptx::tmem_st_32x16(dp_tmem + c / 2, packed);
+      }
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->ds_full));
+    }
+    if (ok && steps > 0) wait(&sh->acc_full, 0, 0x650000u);
+    const int row0 = q0 + quarter * 32;
+    if (ok && half == 0 && row0 < p.q_len)      // staged where Q was
+      store_rows<DP, BF16>(&a.dq, dq_at + lanes, steps > 0, p.scale / ds_factor, smem + quarter * 4096, row0, h, b, lane);
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- launches ----------------------------------------------------------------------------------------
+
+template <int DP, bool BF16, bool CAP, bool BIAS>
+int32_t launch_bwd(const BwdArgs& a, int device, cudaStream_t s) {
+  static PerDeviceFlag ready;
+  auto keys = attn_bwd_keys_kernel<DP, BF16, CAP, BIAS>;
+  auto queries = attn_bwd_queries_kernel<DP, BF16, CAP, BIAS>;
+  if (!ready.test(device)) {
+    LEGO_CUDA_TRY(cudaFuncSetAttribute(keys, cudaFuncAttributeMaxDynamicSharedMemorySize, key_smem<DP>()));
+    LEGO_CUDA_TRY(cudaFuncSetAttribute(queries, cudaFuncAttributeMaxDynamicSharedMemorySize, query_smem<DP>()));
+    ready.set(device);
+  }
+  const long long key_ctas = (long long)tiles_of(a.p.k_len) * a.p.batch * a.p.k_heads;
+  const long long query_ctas = (long long)tiles_of(a.p.q_len) * a.p.batch * a.p.q_heads;
+  if (key_ctas > 0x7fffffffLL || query_ctas > 0x7fffffffLL) return LEGO_ERR_SIZE;
+  LEGO_CUDA_TRY(launch_overlapped(keys, dim3((unsigned)key_ctas), dim3(kBwdThreads), key_smem<DP>(), s, a));
+  LEGO_CUDA_TRY(launch_overlapped(queries, dim3((unsigned)query_ctas), dim3(kBwdThreads), query_smem<DP>(), s, a));
+  return LEGO_OK;
+}
+
+template <int DP, bool BF16>
+int32_t launch_bwd_scores(const BwdArgs& a, int device, cudaStream_t s) {
+  const bool cap = a.p.softcap > 0.f, bias = a.p.slopes != nullptr;
+  if (cap) return bias ? launch_bwd<DP, BF16, true, true>(a, device, s) : launch_bwd<DP, BF16, true, false>(a, device, s);
+  return bias ? launch_bwd<DP, BF16, false, true>(a, device, s) : launch_bwd<DP, BF16, false, false>(a, device, s);
+}
+
+// Workspace of the backward pass: document summaries, row sums, peaks.
+struct BwdLayout {
+  int64_t rows, neg_lse, neg_delta, peak, bytes;
+};
+BwdLayout bwd_layout(const AttnProblem& p) {
+  BwdLayout l;
+  l.rows = (int64_t)p.batch * p.q_heads * tiles_of(p.q_len) * kTile;
+  l.neg_lse = attention_docs_bytes(p);
+  l.neg_delta = l.neg_lse + l.rows * 4;
+  l.peak = l.neg_delta + l.rows * 4;
+  l.bytes = l.peak + ((int64_t)p.batch * p.k_heads * 8 + 15) / 16 * 16;
+  return l;
+}
+
+}  // namespace
+}  // namespace lego
+
+using namespace lego;
+
+extern "C" {
+
+int64_t lego_attention_workspace_bytes(const lego_attention_t* d, int32_t backward) {
+  AttnProblem p;
+  const int32_t st = attention_problem(d, &p);
+  if (st != LEGO_OK) return st;
+  return backward ? bwd_layout(p).bytes : attention_docs_bytes(p);
+}
+
+int32_t lego_attention_bwd(const lego_attention_t* d, const void* q, const void* k, const void* v, const void* o,
+                           const float* lse, const void* d_o, void* dq, void* dk, void* dv, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+  BwdArgs a = {};
+  int32_t st = attention_problem(d, &a.p);
+  if (st != LEGO_OK) return st;
+  if (!q || !k || !v || !o || !lse || !d_o || !dq || !dk || !dv || !workspace) return LEGO_ERR_NULL;
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)d_o | (uintptr_t)dq | (uintptr_t)dk |
+       (uintptr_t)dv | (uintptr_t)workspace) & 15)
+    return LEGO_ERR_ALIGN;
+  const AttnProblem& p = a.p;
+  const BwdLayout l = bwd_layout(p);
+  if (workspace_bytes < l.bytes) return LEGO_ERR_SIZE;
+  DeviceCtx* ctx = device_ctx(&st);
+  if (!ctx) return st;
+  EncodeFn enc = encode_fn(&st);
+  if (!enc) return st;
+  const bool bf16 = d->dtype == LEGO_BF16;
+  const long long q_dense[3] = {(long long)p.q_len * p.q_heads * p.dim, (long long)p.q_heads * p.dim, p.dim};
+  const long long k_dense[3] = {(long long)p.k_len * p.k_heads * p.dim, (long long)p.k_heads * p.dim, p.dim};
+  if (make_tmap_heads(enc, &a.q, bf16, q, p.dim, p.q_len, p.q_heads, p.batch, p.q_stride, kTile) != LEGO_OK ||
+      make_tmap_heads(enc, &a.k, bf16, k, p.dim, p.k_len, p.k_heads, p.batch, p.k_stride, kTile) != LEGO_OK ||
+      make_tmap_heads(enc, &a.v, bf16, v, p.dim, p.k_len, p.k_heads, p.batch, p.v_stride, kTile) != LEGO_OK ||
+      make_tmap_heads(enc, &a.d_o, bf16, d_o, p.dim, p.q_len, p.q_heads, p.batch, q_dense, kTile) != LEGO_OK ||
+      make_tmap_heads(enc, &a.dq, bf16, dq, p.dim, p.q_len, p.q_heads, p.batch, q_dense, 32) != LEGO_OK ||
+      make_tmap_heads(enc, &a.dk, bf16, dk, p.dim, p.k_len, p.k_heads, p.batch, k_dense, 32) != LEGO_OK ||
+      make_tmap_heads(enc, &a.dv, bf16, dv, p.dim, p.k_len, p.k_heads, p.batch, k_dense, 32) != LEGO_OK)
+    return LEGO_ERR_UNSUPPORTED;
+  cudaStream_t s = (cudaStream_t)stream;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  a.q_raw = (const uint16_t*)q;
+  a.k_raw = (const uint16_t*)k;
+  a.v_raw = (const uint16_t*)v;
+  a.o_raw = (const uint16_t*)o;
+  a.do_raw = (const uint16_t*)d_o;
+  a.lse = lse;
+  a.neg_lse = reinterpret_cast<float*>(ws + l.neg_lse);
+  a.neg_delta = reinterpret_cast<float*>(ws + l.neg_delta);
+  a.peak = reinterpret_cast<uint32_t*>(ws + l.peak);
+  a.status = ctx->status_word;
+  const long long rows = l.rows + (bf16 ? 0 : (long long)p.batch * p.k_len * p.k_heads), blocks = (rows + 7) / 8;
+  if (blocks > 0x7fffffffLL) return LEGO_ERR_SIZE;
+  st = attention_docs(&a.p, workspace, s);
+  if (st != LEGO_OK) return st;
+  if (bf16) {
+    LEGO_CUDA_TRY(launch_overlapped(attn_bwd_prep_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, s, a));
+  } else {
+    LEGO_CUDA_TRY(cudaMemsetAsync(a.peak, 0, (size_t)(l.bytes - l.peak), s));
+    LEGO_CUDA_TRY(launch_overlapped(attn_bwd_prep_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, s, a));
+  }
+  if (p.dim <= 64)
+    return bf16 ? launch_bwd_scores<64, true>(a, ctx->device, s) : launch_bwd_scores<64, false>(a, ctx->device, s);
+  return bf16 ? launch_bwd_scores<128, true>(a, ctx->device, s) : launch_bwd_scores<128, false>(a, ctx->device, s);
+}
+
+}  // extern "C"
