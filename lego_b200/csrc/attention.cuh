@@ -151,6 +151,61 @@ __device__ __forceinline__ void copy_tile_clean(uint8_t* tile, const uint16_t* b
   __syncwarp();
 }
 
+// ---- a tile of scores to weights ---------------------------------------------------------------
+
+// log2 of the growth a row's reference value may lag behind its maximum: weights stay below
+// 2^8, their sum is kept in 32 bits, and O in TMEM is rarely rescaled.
+constexpr float kRescale = 8.f;
+
+// One thread per row: the row's 128 scores s (hidden ones -inf) become weights
+// 2^(s by - m) (SCALED: s is in log2 units already), packed to 16 bits over columns 0 .. 63 of
+// s_tmem; their sum, before that rounding, is added to `sum`.  by > 0.  Not the first tile:
+// where some row of the warp outgrew its reference value, the rows' sums in o_tmem follow it.
+template <int DP, bool BF16, bool SCALED>
+__device__ __forceinline__ void weigh_tile(const float (&s)[kTile], float by, bool first, float* m, float* sum,
+                                           uint32_t s_tmem, uint32_t o_tmem) {
+  float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+  for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
+  float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  if (!SCALED) mt *= by;
+  if (first) {
+    *m = mt;
+  } else if (__any_sync(~0u, mt > *m + kRescale)) {
+    const float mn = fmaxf(*m, mt);
+    const float f = mn == -INFINITY ? 1.f : ex2(*m - mn);
+    *m = mn;
+    *sum *= f;
+#pragma unroll
+    for (int c = 0; c < DP; c += 16) {     // rare, and the scores fill the registers
+      uint32_t o[16];
+      ptx::tmem_ld_32x16(o_tmem + c, o);
+      ptx::tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+      ptx::tmem_st_32x16(o_tmem + c, o);
+    }
+  }
+  const float mu = *m == -INFINITY ? 0.f : *m;
+  float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  const float2 by2 = make_float2(by, by), mu2 = make_float2(-mu, -mu);
+#pragma unroll
+  for (int c = 0; c < kTile; c += 32) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float2 z = make_float2(s[c + i], s[c + i + 1]);
+      z = SCALED ? ptx::add2(z, mu2) : ptx::fma2(z, by2, mu2);
+      const float2 x = make_float2(ex2(z.x), ex2(z.y));
+      add[(i >> 1) & 1] = ptx::add2(add[(i >> 1) & 1], x);
+      w[i >> 1] = pack2<BF16>(x.x, x.y);
+    }
+    ptx::tmem_st_32x16(s_tmem + c / 2, w);
+  }
+  *sum += (add[0].x + add[0].y) + (add[1].x + add[1].y);
+  ptx::tmem_st_wait();
+}
+
 __device__ __forceinline__ void attn_fail(uint32_t* status, volatile uint32_t* abort_flag, uint32_t code) {
   *abort_flag = 1;
   atomicCAS(status, 0u, code);

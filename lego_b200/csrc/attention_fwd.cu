@@ -30,7 +30,6 @@ constexpr int kFwdThreads = 384;
 // softmax thread holds a row of 128 scores, the loads and the MMA issue need few.
 constexpr int kFwdRegs = 168, kSoftmaxRegs = 216, kOtherRegs = 72;
 static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kFwdRegs, "more registers than the launch has would wait forever");
-constexpr float kRescale = 8.f;      // log2 of the growth a row's reference value may lag behind
 
 template <int DP> constexpr int fwd_stages() { return DP == 128 ? 5 : 8; }
 template <int DP> constexpr int fwd_smem() { return (2 + fwd_stages<DP>()) * tile_bytes<DP>() + 1024 + 512; }
@@ -298,47 +297,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
 #pragma unroll
         for (int c = 0; c < kTile; ++c) s[c] = (see[c >> 5] >> (c & 31)) & 1u ? s[c] : -INFINITY;
       }
-      float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-      for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
-      float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      if (!CAP && !BIAS) mt *= by;     // by > 0 in this instance
-      if (j == l) {
-        m = mt;
-      } else if (__any_sync(~0u, mt > m + kRescale)) {
-        const float mn = fmaxf(m, mt);
-        const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
-        m = mn;
-        sum *= f;
-#pragma unroll
-        for (int c = 0; c < DP; c += 32) {
-          uint32_t o[32];
-          ptx::tmem_ld_32x32(o_tmem + c, o);
-          ptx::tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-          ptx::tmem_st_32x16(o_tmem + c, o);
-          ptx::tmem_st_32x16(o_tmem + c + 16, o + 16);
-        }
-      }
-      const float mu = m == -INFINITY ? 0.f : m;
-      float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      const float2 by2 = make_float2(by, by), mu2 = make_float2(-mu, -mu);
-#pragma unroll
-      for (int c = 0; c < kTile; c += 32) {
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float2 z = make_float2(s[c + i], s[c + i + 1]);
-          z = CAP || BIAS ? ptx::add2(z, mu2) : ptx::fma2(z, by2, mu2);
-          const float2 x = make_float2(ex2(z.x), ex2(z.y));
-          add[(i >> 1) & 1] = ptx::add2(add[(i >> 1) & 1], x);
-          w[i >> 1] = pack2<BF16>(x.x, x.y);
-        }
-        ptx::tmem_st_32x16(s_tmem + c / 2, w);
-      }
-      sum += (add[0].x + add[0].y) + (add[1].x + add[1].y);
-      ptx::tmem_st_wait();
+      weigh_tile<DP, BF16, CAP || BIAS>(s, by, j == l, &m, &sum, s_tmem, o_tmem);
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->p_full[t]));

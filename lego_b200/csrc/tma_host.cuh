@@ -81,8 +81,9 @@ inline int32_t make_tmap_group_major(EncodeFn enc, CUtensorMap* out, CUtensorMap
   return r == CUDA_SUCCESS ? LEGO_OK : LEGO_ERR_UNSUPPORTED;
 }
 
-// 4-D map of a [batch, tokens, heads, dim] tensor of 16-bit values as (dim, token, head, batch),
-// 128-byte swizzle: a box is 64 values of `rows` tokens of one head.  Values past `dim` and
+// 4-D map of a [batch, tokens, heads, dim] tensor of 16-bit values as (dim, token, head, batch) --
+// or of a paged cache [pages, slots, heads, dim] --, 128-byte swizzle: a box is 64 values of `rows`
+// tokens of one head.  Values past `dim` and
 // tokens past the end read as zeros and are not written.  Strides in elements.
 inline int32_t make_tmap_heads(EncodeFn enc, CUtensorMap* out, bool bf16, const void* base, uint64_t dim,
                                uint64_t tokens, uint64_t heads, uint64_t batch, const long long* stride,
