@@ -157,18 +157,11 @@ __device__ __forceinline__ void copy_tile_clean(uint8_t* tile, const uint16_t* b
 // 2^8, their sum is kept in 32 bits, and O in TMEM is rarely rescaled.
 constexpr float kRescale = 8.f;
 
-// One thread per row: the row's 128 scores s (hidden ones -inf) become weights
-// 2^(s by - m) (SCALED: s is in log2 units already), packed to 16 bits over columns 0 .. 63 of
-// s_tmem; their sum, before that rounding, is added to `sum`.  by > 0.  Not the first tile:
-// where some row of the warp outgrew its reference value, the rows' sums in o_tmem follow it.
-template <int DP, bool BF16, bool SCALED>
-__device__ __forceinline__ void weigh_tile(const float (&s)[kTile], float by, bool first, float* m, float* sum,
-                                           uint32_t s_tmem, uint32_t o_tmem) {
-  float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-  for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
-  float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-  if (!SCALED) mt *= by;
+// A row's reference value m for a tile whose maximum is mt (log2 units).  Not the first tile:
+// where some row of the warp outgrew its reference value, its sums, in `sum` and over DP columns
+// of o_tmem, follow it.
+template <int DP>
+__device__ __forceinline__ void follow_maximum(float mt, bool first, float* m, float* sum, uint32_t o_tmem) {
   if (first) {
     *m = mt;
   } else if (__any_sync(~0u, mt > *m + kRescale)) {
@@ -186,6 +179,20 @@ __device__ __forceinline__ void weigh_tile(const float (&s)[kTile], float by, bo
       ptx::tmem_st_32x16(o_tmem + c, o);
     }
   }
+}
+
+// One thread per row: the row's 128 scores s (hidden ones -inf) become weights
+// 2^(s by - m) (SCALED: s is in log2 units already), packed to 16 bits over columns 0 .. 63 of
+// s_tmem; their sum, before that rounding, is added to `sum`.  by > 0.
+template <int DP, bool BF16, bool SCALED>
+__device__ __forceinline__ void weigh_tile(const float (&s)[kTile], float by, bool first, float* m, float* sum,
+                                           uint32_t s_tmem, uint32_t o_tmem) {
+  float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+  for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
+  float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  if (!SCALED) mt *= by;
+  follow_maximum<DP>(mt, first, m, sum, o_tmem);
   const float mu = *m == -INFINITY ? 0.f : *m;
   float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   const float2 by2 = make_float2(by, by), mu2 = make_float2(-mu, -mu);

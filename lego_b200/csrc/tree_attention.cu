@@ -16,6 +16,12 @@
 // order of the keys.  Which runs a sequence is in follows from the lengths, which only the
 // device knows: every CTA adds them up.
 //
+// Few rows would leave most lanes of TMEM, and the warps that can read them, idle while one
+// warp works through 128 scores per row.  Up to 16 rows the queries therefore stand in the tile
+// four times, up to 64 twice: every copy weighs its own quarter or half of a tile's keys (its
+// weights of the others are zero) with its own m, sum and O, and the copies are put together
+// at a piece's end.
+//
 // Warps: 0-3 and 4-7 weights of the even and the odd tiles of a piece (each with its own m, sum
 // and O, put together at the piece's end), 8-11 loads, 12 MMA issue (13-15 fill up their
 // warpgroup).  Each loading lane looks up the place of one row of a tile.  Tiles of cached
@@ -34,13 +40,14 @@ namespace {
 
 constexpr int kMaxDraft = LEGO_MAX_DRAFT;
 constexpr int kTreeThreads = 512;
-constexpr int kTreeRegs = 128, kTreeMathRegs = 200, kTreeOtherRegs = 56;
+constexpr int kTreeRegs = 128, kTreeMathRegs = 176, kTreeOtherRegs = 80;
 static_assert(2 * kTreeMathRegs + 2 * kTreeOtherRegs <= 4 * kTreeRegs, "more registers than the launch has would wait forever");
 
 struct TreeProblem {
   int batch, drafted, q_heads, k_heads, dim, group;
   int pages, page_size, max_pages;
   int rows, row_tiles;          // rows of a key head: drafted * group; tiles of 128 of them
+  int copies;                   // of the rows in a tile: 4, 2 or 1
   long long table_stride;
   long long q_stride[3], k_stride[3], v_stride[3];
   float scale, softcap;
@@ -54,6 +61,7 @@ struct TreeProblem {
   uint32_t* status;
   int runs;                     // CTAs of the main kernel
   int box_rows;                 // rows of a TMA box of the cache; 0: 16-byte copies only
+  FastDiv by_page, by_group;
 };
 
 struct TreeMaps {
@@ -79,6 +87,7 @@ int32_t tree_problem(const lego_tree_attention_t* d, TreeProblem* p) {
   p->group = p->q_heads / p->k_heads;
   p->rows = p->drafted * p->group;
   p->row_tiles = tiles_of(p->rows);
+  p->copies = p->rows <= 16 ? 4 : p->rows <= 64 ? 2 : 1;
   if ((int64_t)p->batch * p->k_heads * p->row_tiles > 0x7fffffffLL) return LEGO_ERR_SIZE;
   p->pages = (int)d->pages;
   p->page_size = (int)d->page_size;
@@ -90,6 +99,10 @@ int32_t tree_problem(const lego_tree_attention_t* d, TreeProblem* p) {
     p->v_stride[i] = d->v_stride[i];
     if (d->q_stride[i] % 8 || d->k_stride[i] % 8 || d->v_stride[i] % 8) return LEGO_ERR_ALIGN;
   }
+  // every tile of the longest sequences the table has room for, in 31 bits
+  if ((int64_t)p->batch * p->k_heads * p->row_tiles * tiles_of(p->max_pages * p->page_size) > 0x7fffffffLL) return LEGO_ERR_SIZE;
+  p->by_page = make_fastdiv((uint64_t)p->page_size);
+  p->by_group = make_fastdiv((uint64_t)p->group);
   p->scale = d->scale;
   p->softcap = d->softcap;
   return LEGO_OK;
@@ -97,17 +110,14 @@ int32_t tree_problem(const lego_tree_attention_t* d, TreeProblem* p) {
 
 // ---- the line of tiles and its runs --------------------------------------------------------------
 
-// Places of sequence b that may be seen: cached and drafted tokens within the table.
-__device__ __forceinline__ int tree_places(const TreeProblem& p, int b) {
-  const int len = p.lengths[b];
+// Places of a sequence of `len` cached tokens that may be seen: those and the drafted ones, within
+// the table.
+__device__ __forceinline__ int tree_places(const TreeProblem& p, int len) {
   if (len < 0) return 0;
   const int room = p.max_pages * p.page_size;      // at most 2^30
   return len < room - p.drafted ? len + p.drafted : room;
 }
-__device__ __forceinline__ int tree_tiles(const TreeProblem& p, int b) { return tiles_of(tree_places(p, b)); }
-__device__ __forceinline__ long long run_begin(long long total, int runs, int c) {
-  return total / runs * c + total % runs * c / runs;
-}
+__device__ __forceinline__ int run_begin(int total, int runs, int c) { return total / runs * c + total % runs * c / runs; }
 
 // Every key of a tile is a cached token within the table.
 __device__ __forceinline__ bool all_cached(int tile, int len, int places) {
@@ -116,54 +126,31 @@ __device__ __forceinline__ bool all_cached(int tile, int len, int places) {
 }
 
 struct Piece {
-  int b, hk, rt;         // sequence, key head, row tile
+  int b, hk, rt;         // sequence (-1: no more pieces), key head, row tile
   int first, last;       // tiles [first, last)
-  int tiles;             // of the sequence
+  int len, places;       // of the sequence
 };
 
-struct Walk {
-  int b, hr, tile;       // next piece: sequence, key head * row tiles + row tile, tile
-  long long left;        // tiles of the run still to come
-};
-
-__device__ __forceinline__ bool next_piece(const TreeProblem& p, Walk& w, Piece* out) {
-  if (w.left <= 0) return false;
-  const int tiles = tree_tiles(p, w.b);
-  out->b = w.b;
-  out->hk = w.hr / p.row_tiles;
-  out->rt = w.hr % p.row_tiles;
-  out->tiles = tiles;
-  out->first = w.tile;
-  out->last = w.left < tiles - w.tile ? w.tile + (int)w.left : tiles;
-  w.left -= out->last - out->first;
-  w.tile = 0;
-  if (++w.hr == p.k_heads * p.row_tiles) {
-    w.hr = 0;
-    do ++w.b;
-    while (w.b < p.batch && w.left > 0 && tree_tiles(p, w.b) == 0);
-  }
-  return true;
-}
-
-// Sum over the block's threads of v and what the threads before this one add to; `warps` words of
-// shared memory.  Every thread takes part.
+// Sum over the block's threads of v and what the threads before this one add to; a word of shared
+// memory per warp.  Every thread takes part.
 template <int THREADS>
-__device__ __forceinline__ long long block_scan(long long v, long long* before, long long* words) {
+__device__ __forceinline__ int block_scan(int v, int* before, int* words) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long x = v;
+  int x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(~0u, x, o);
+    const int y = __shfl_up_sync(~0u, x, o);
     if (lane >= o) x += y;
   }
   __syncthreads();
   if (lane == 31) words[warp] = x;
   __syncthreads();
-  long long base = 0, total = 0;
+  int base = 0, total = 0;
 #pragma unroll
   for (int i = 0; i < THREADS / 32; ++i) {
-    if (i < warp) base += words[i];
-    total += words[i];
+    const int w = words[i];
+    if (i < warp) base += w;
+    total += w;
   }
   *before = base + x - v;
   return total;
@@ -227,12 +214,12 @@ template <int DP> constexpr int tree_stages() { return DP == 128 ? 5 : 10; }
 constexpr int kMaskRing = 8;    // see the note at its use
 struct TreeShared {
   Tree tree[2];
+  Piece piece[2];
   uint32_t exist[kMaskRing][4];
   uint64_t exist_full[kMaskRing], full[10], empty[10];
-  uint64_t tree_full[2], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], odd_done, o_free;
-  long long words[16];
-  long long start_left;
-  int start_b, start_hr, start_tile;
+  uint64_t piece_full[2], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], odd_done, o_free, merged;
+  int words[16];
+  int start_b, start_hr, start_tile, start_left;
   uint32_t tmem_base, abort_flag;
 };
 template <int DP> constexpr int tree_smem() { return (2 + tree_stages<DP>()) * tile_bytes<DP>() + 1024 + (int)sizeof(TreeShared); }
@@ -251,15 +238,16 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
-      ptx::mbar_init(ptx::smem_u32(&sh->tree_full[t]), 1);
-      ptx::mbar_init(ptx::smem_u32(&sh->q_full[t]), 4);
-      ptx::mbar_init(ptx::smem_u32(&sh->q_empty[t]), 1 + 8);   // the MMAs; the warps done with the tree
+      ptx::mbar_init(ptx::smem_u32(&sh->piece_full[t]), 1);
+      ptx::mbar_init(ptx::smem_u32(&sh->q_full[t]), 128);          // every loading thread's copies
+      ptx::mbar_init(ptx::smem_u32(&sh->q_empty[t]), 1 + 8 + 3);   // the MMAs; the warps done with the piece and its tree
       ptx::mbar_init(ptx::smem_u32(&sh->s_full[t]), 1);
       ptx::mbar_init(ptx::smem_u32(&sh->p_full[t]), 4);
       ptx::mbar_init(ptx::smem_u32(&sh->o_full[t]), 1);
     }
     ptx::mbar_init(ptx::smem_u32(&sh->odd_done), 4);
     ptx::mbar_init(ptx::smem_u32(&sh->o_free), 4);
+    ptx::mbar_init(ptx::smem_u32(&sh->merged), 4);
     for (int s = 0; s < NS; ++s) {
       ptx::mbar_init(ptx::smem_u32(&sh->full[s]), 128);     // every loading thread's copies
       ptx::mbar_init(ptx::smem_u32(&sh->empty[s]), 1);
@@ -276,26 +264,29 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
   }
   ptx::grid_dependency_wait();
   {   // this CTA's run: where it starts and how long it is
-    const long long per_tile = (long long)p.k_heads * p.row_tiles;
-    long long total = 0, before;
+    const int per_tile = p.k_heads * p.row_tiles;
+    auto units_of = [&](int b) { return b < p.batch ? tiles_of(tree_places(p, p.lengths[b])) * per_tile : 0; };
+    int total = 0, mine = 0, before = 0;
     for (int base = 0; base < p.batch; base += kTreeThreads) {
-      const int b = base + threadIdx.x;
-      total += block_scan<kTreeThreads>(b < p.batch ? tree_tiles(p, b) * per_tile : 0, &before, sh->words);
+      mine = units_of(base + threadIdx.x);
+      total += block_scan<kTreeThreads>(mine, &before, sh->words);
     }
-    const int runs = total < gridDim.x ? (int)total : (int)gridDim.x;
+    const int runs = total < (int)gridDim.x ? total : (int)gridDim.x;
     if ((int)blockIdx.x < runs) {
-      const long long u0 = run_begin(total, runs, blockIdx.x), u1 = run_begin(total, runs, blockIdx.x + 1);
-      long long passed = 0;
+      const int u0 = run_begin(total, runs, blockIdx.x), u1 = run_begin(total, runs, blockIdx.x + 1);
+      int passed = 0;
       for (int base = 0; base < p.batch; base += kTreeThreads) {
-        const int b = base + threadIdx.x;
-        const int tiles = b < p.batch ? tree_tiles(p, b) : 0;
-        const long long mine = tiles * per_tile;
-        const long long sum = block_scan<kTreeThreads>(mine, &before, sh->words);
-        const long long at = u0 - passed - before;
+        int sum = total;
+        if (p.batch > kTreeThreads) {     // not the sums of the last turn above
+          mine = units_of(base + threadIdx.x);
+          sum = block_scan<kTreeThreads>(mine, &before, sh->words);
+        }
+        const int at = u0 - passed - before;
         if (at >= 0 && at < mine) {
-          sh->start_b = b;
-          sh->start_hr = (int)(at / tiles);
-          sh->start_tile = (int)(at % tiles);
+          const int tiles = mine / per_tile;
+          sh->start_b = base + threadIdx.x;
+          sh->start_hr = at / tiles;
+          sh->start_tile = at % tiles;
           sh->start_left = u1 - u0;
         }
         passed += sum;
@@ -306,7 +297,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
-  Walk walk = {sh->start_b, sh->start_hr, sh->start_tile, sh->start_left};
   Piece pc;
 
   if (warp >= 12) {
@@ -324,11 +314,14 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
       };
       uint32_t pos = 0;                    // ring position of K(i)
       uint32_t weighed[2] = {0, 0};
-      for (int n = 0; ok && next_piece(p, walk, &pc); ++n) {
+      for (int n = 0; ok; ++n) {
+        wait(&sh->piece_full[n & 1], (n >> 1) & 1, 0x720005u);
+        pc = sh->piece[n & 1];
+        if (!ok || pc.b < 0) break;
         const int count = pc.last - pc.first;
         const uint32_t q_tile = q_smem + (n & 1) * TILE;
-        const int len = p.lengths[pc.b], places = tree_places(p, pc.b);
         wait(&sh->q_full[n & 1], (n >> 1) & 1, 0x720000u);
+        ptx::fence_proxy_async();      // the queries came as 16-byte copies, through the generic proxy
         for (int i = 0; ok && i <= count; ++i, pos += 2) {
           // the accumulators, and the place of the odd warps' statistics, have been read
           if (i == 1 && n > 0) wait(&sh->o_free, (n - 1) & 1, 0x720001u);
@@ -337,8 +330,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             const uint32_t slot = pos % NS;
             wait(&sh->full[slot], (pos / NS) & 1, 0x720002u);
             if (!ok) break;
-            if (!(p.box_rows && all_cached(pc.first + i, len, places)))
-              ptx::fence_proxy_async();      // 16-byte copies go through the generic proxy
+            if (!(p.box_rows && all_cached(pc.first + i, pc.len, pc.places)))
+              ptx::fence_proxy_async();      // so did these keys
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s)
               ptx::mma_f16_ss(tmem + (i & 1) * kTile, desc_k_major(q_tile, s), desc_k_major(kv_smem + slot * TILE, s), id_s, s != 0);
@@ -351,7 +344,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             wait(&sh->full[slot], (vpos / NS) & 1, 0x720003u);
             wait(&sh->p_full[t], weighed[t] & 1, 0x720004u);
             if (!ok) break;
-            if (!(p.box_rows && all_cached(pc.first + i - 1, len, places))) ptx::fence_proxy_async();
+            if (!(p.box_rows && all_cached(pc.first + i - 1, pc.len, pc.places))) ptx::fence_proxy_async();
             ++weighed[t];
 #pragma unroll
             for (int s = 0; s < kTile / 16; ++s)
@@ -378,48 +371,70 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
       if (!ok && lane == 0) attn_fail(p.status, abort_flag, code);
       return ok;
     };
-    for (int n = 0; ok && next_piece(p, walk, &pc); ++n) {
-      // the piece's queries and tree
-      if (!bounded(&sh->q_empty[n & 1], ((n >> 1) & 1) ^ 1, 0x710000u)) break;
-      Tree* tree = &sh->tree[n & 1];
+    // warp 8 walks the run and publishes its pieces
+    int next_b = sh->start_b, next_hr = sh->start_hr, next_tile = sh->start_tile, left = sh->start_left;
+    int len = left > 0 ? p.lengths[next_b] : 0;
+    for (int n = 0; ok; ++n) {
       if (w == 0) {
-        grow_tree(p, pc.b, tree, lane);
+        if (!bounded(&sh->q_empty[n & 1], ((n >> 1) & 1) ^ 1, 0x710000u)) break;
+        pc.b = -1;
+        if (left > 0) {
+          pc.b = next_b;
+          pc.hk = next_hr / p.row_tiles;
+          pc.rt = next_hr - pc.hk * p.row_tiles;
+          pc.len = len;
+          pc.places = tree_places(p, len);
+          pc.first = next_tile;
+          const int tiles = tiles_of(pc.places);
+          pc.last = left < tiles - next_tile ? next_tile + left : tiles;
+          left -= pc.last - pc.first;
+          next_tile = 0;
+          if (++next_hr == p.k_heads * p.row_tiles && left > 0) {
+            next_hr = 0;
+            do len = p.lengths[++next_b];      // units are left, so a sequence with tiles follows
+            while (len < 0);
+          }
+          grow_tree(p, pc.b, &sh->tree[n & 1], lane);
+        }
+        if (lane == 0) sh->piece[n & 1] = pc;
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->tree_full[n & 1]));
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->piece_full[n & 1]));
+      } else {
+        if (!bounded(&sh->piece_full[n & 1], (n >> 1) & 1, 0x710002u)) break;
+        pc = sh->piece[n & 1];
       }
-      uint8_t* q_tile = smem + (n & 1) * TILE;
+      if (pc.b < 0) break;
+      const Tree* tree = &sh->tree[n & 1];
+      const int per_copy = kTile / p.copies;
 #pragma unroll 4
       for (int i = 0; i < 32; i += PER) {
-        const int r = w * 32 + i + sub, row = pc.rt * kTile + r;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (row < p.rows && chunk_real) {
-          const int t = row / p.group, h = pc.hk * p.group + row % p.group;
-          x = *reinterpret_cast<const uint4*>(p.q + pc.b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2] + chunk * 8);
-        }
-        *reinterpret_cast<uint4*>(q_tile + (chunk >> 3) * kBoxBytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = x;
+        const int r = w * 32 + i + sub, row = pc.rt * kTile + (r & (per_copy - 1));
+        const bool copy = row < p.rows && chunk_real;
+        const int t = (int)fd_div((uint32_t)row, p.by_group), h = pc.hk * p.group + row - t * p.group;
+        const uint16_t* src = p.q + pc.b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2] + chunk * 8;
+        ptx::cp_async_16(q_smem + (n & 1) * TILE + (chunk >> 3) * kBoxBytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4),
+                         copy ? src : p.q, copy);
       }
-      ptx::fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->q_full[n & 1]));
-      if (!bounded(&sh->tree_full[n & 1], (n >> 1) & 1, 0x710002u)) break;
+      ptx::cp_async_arrive(ptx::smem_u32(&sh->q_full[n & 1]));
 
-      const int len = p.lengths[pc.b], places = tree_places(p, pc.b);
+      const int places = pc.places;
       const int* table = p.table + pc.b * p.table_stride;
       // page number of this lane's row of a tile, as the table has it; -1: the row does not exist
       auto page_of = [&](int tile) {
         const int j = tile * kTile + w * 32 + lane;
         if (tile >= pc.last || j >= places) return -1;
-        if (j >= len && tree->seen[j - len] == 0) return -1;
-        return table[j / p.page_size];
+        if (j >= pc.len && tree->seen[j - pc.len] == 0) return -1;
+        return table[fd_div((uint32_t)j, p.by_page)];
       };
       int page = page_of(pc.first);
       for (int tile = pc.first; ok && tile < pc.last; ++tile, ++tile_no) {
         const bool real = page >= 0 && page < p.pages;
         const int here = real ? page : p.pages;     // past the cache: a TMA box of zeros
         page = page_of(tile + 1);                   // on its way while this tile's copies are issued
-        const int in_page = (tile * kTile + w * 32 + lane) % p.page_size;
+        const int place = tile * kTile + w * 32 + lane;
+        const int in_page = place - (int)fd_div((uint32_t)place, p.by_page) * p.page_size;
         const uint32_t word = __ballot_sync(~0u, real);
-        const bool boxes = p.box_rows && all_cached(tile, len, places);
+        const bool boxes = p.box_rows && all_cached(tile, pc.len, places);
         for (int g = 0; g < 2; ++g, ++issued) {
           const uint32_t slot = issued % NS, full = ptx::smem_u32(&sh->full[slot]);
           if (!bounded(&sh->empty[slot], ((issued / NS) & 1) ^ 1, 0x710001u)) break;
@@ -446,8 +461,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             }
             continue;
           }
-          const long long* st = g ? p.v_stride : p.k_stride;
-          const long long row_at = real ? here * st[0] + in_page * st[1] + pc.hk * st[2] : 0;
+          const long long s0 = g ? p.v_stride[0] : p.k_stride[0], s1 = g ? p.v_stride[1] : p.k_stride[1],
+                          s2 = g ? p.v_stride[2] : p.k_stride[2];
+          const long long row_at = real ? here * s0 + in_page * s1 + pc.hk * s2 : 0;
           const uint16_t* src = g ? p.v : p.k;
 #pragma unroll 4
           for (int i = 0; i < 32; i += PER) {
@@ -460,6 +476,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
           ptx::cp_async_arrive(full);
         }
       }
+      if (w > 0 && lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->q_empty[n & 1]));
     }
     ptx::cp_async_wait_all();      // leave no copy in flight
   } else {
@@ -470,6 +487,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
     const uint32_t s_tmem = tmem + lanes + t * kTile, o_tmem = tmem + lanes + 2 * kTile + t * DP;
     const float by = p.scale * kLog2e;
     const float u_by = CAP ? 2.f * kLog2e * p.scale / p.softcap : 0.f, cap_by = p.softcap * kLog2e;
+    const int per_copy = kTile / p.copies, chunks = 4 / p.copies;     // rows; chunks of 32 columns a copy weighs
+    const int in_copy = (quarter * 32 + lane) & (per_copy - 1), copy = quarter * 32 / per_copy, chunk0 = copy * chunks;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
       if (!ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait)) ok = false;
@@ -479,15 +498,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
       }
       return ok;
     };
-    uint32_t scored = 0, tile_no = 0, mine = 0, paired = 0;
-    for (int n = 0; ok && next_piece(p, walk, &pc); ++n) {
+    uint32_t scored = 0, tile_no = 0, mine = 0, paired = 0, merges = 0;
+    for (int n = 0; ok; ++n) {
+      if (!wait(&sh->piece_full[n & 1], (n >> 1) & 1, 0x740000u)) break;
+      pc = sh->piece[n & 1];
+      if (pc.b < 0) break;
       const int count = pc.last - pc.first;
-      const int row = pc.rt * kTile + quarter * 32 + lane;
-      const bool real = row < p.rows, any_row = pc.rt * kTile + quarter * 32 < p.rows;
-      const int tok = real ? row / p.group : 0, h = pc.hk * p.group + (real ? row % p.group : 0);
-      if (!wait(&sh->q_full[n & 1], (n >> 1) & 1, 0x740000u)) break;
+      const int row = pc.rt * kTile + in_copy;
+      const bool real = row < p.rows, any_row = pc.rt * kTile + (quarter * 32 & (per_copy - 1)) < p.rows;
+      const int tok = real ? (int)fd_div((uint32_t)row, p.by_group) : 0, h = pc.hk * p.group + (real ? row - tok * p.group : 0);
       const Tree* tree = &sh->tree[n & 1];
-      const int len = p.lengths[pc.b];
+      const int len = pc.len;
       const unsigned long long seen = real ? tree->seen[tok] : 0;
       const int depth = tree->depth[tok];
       const float slope = BIAS && p.slopes ? p.slopes[h] * kLog2e : 0.f;
@@ -500,62 +521,93 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
           break;
         ++scored;
         ptx::tc_fence_after();
-        if (!any_row) {       // idle rows: whatever the product makes of what stands there, nobody reads it
-          ptx::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->p_full[t]));
-          continue;
-        }
-        float s[kTile];
+        if (any_row) {       // else whatever the product makes of what stands there: nobody reads it
+          // First the maximum; scores that are not used as the product leaves them go back to
+          // their place.  Then the weights.
+          float s[32], mt = -INFINITY;
+          bool back = CAP || BIAS;
+          for (int x = 0; x < chunks; ++x) {
+            const int c0 = 32 * (chunk0 + x);
+            ptx::tmem_ld_32x32(s_tmem + c0, reinterpret_cast<uint32_t*>(s));
+            uint32_t see = sh->exist[no % kMaskRing][chunk0 + x];
+            const int at = len - j0 - c0;      // column of the first drafted token
+            if (at < 32) {
+              const int shift = -at;           // draft token of column 0
+              const uint32_t drafted = shift <= -32 || shift >= 64 ? 0u : shift >= 0 ? (uint32_t)(seen >> shift) : (uint32_t)(seen << -shift);
+              see &= bits_upto(at - 1, 0) | drafted;
+            }
+            ptx::tmem_ld_wait();
+            if (CAP || BIAS) {
 #pragma unroll
-        for (int c = 0; c < kTile; c += 32) ptx::tmem_ld_32x32(s_tmem + c, reinterpret_cast<uint32_t*>(s) + c);
-        uint32_t see[4];
+              for (int c = 0; c < 32; ++c) {
+                float z = CAP ? cap_by * tanh_of(s[c] * u_by) : s[c] * by;
+                if (BIAS) z = fmaf(-slope, (float)(at - c) + (float)depth, z);     // cached tokens: none is ahead
+                s[c] = z;
+              }
+              if (BIAS && at < 32) {     // drafted tokens stand where their depth says, not their place
 #pragma unroll
-        for (int x = 0; x < 4; ++x) see[x] = sh->exist[no % kMaskRing][x];
-        ptx::tmem_ld_wait();
-        if (CAP || BIAS) {
+                for (int c = 0; c < 32; ++c) {
+                  const int d = c - at;
+                  if (d >= 0 && d < p.drafted)
+                    s[c] = fmaf(-slope, fabsf((float)(depth - tree->depth[d])) - (float)(depth - d), s[c]);
+                }
+              }
+            }
+            const bool hide = __any_sync(~0u, see != ~0u);
+            if (hide) {
 #pragma unroll
-          for (int c = 0; c < kTile; ++c) {
-            float z = CAP ? cap_by * tanh_of(s[c] * u_by) : s[c] * by;
-            if (BIAS) z = fmaf(-slope, (float)(len - j0 - c) + (float)depth, z);     // cached tokens: none is ahead
-            s[c] = z;
-          }
-        }
-        if (j0 + kTile > len) {      // drafted tokens among the keys
-          const int at = len - j0;   // column of the first; may be negative
-          if (BIAS) {                // they stand where their depth says, not their place
+              for (int c = 0; c < 32; ++c) s[c] = (see >> c) & 1u ? s[c] : -INFINITY;
+            }
+            float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int c = 0; c < kTile; ++c) {
-              const int d = c - at;
-              if (d >= 0 && d < p.drafted)
-                s[c] = fmaf(-slope, fabsf((float)(depth - tree->depth[d])) - (float)(depth - d), s[c]);
+            for (int c = 4; c < 32; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
+            mt = fmaxf(mt, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+            if (chunks > 1 && (CAP || BIAS || hide)) {
+              ptx::tmem_st_32x16(s_tmem + c0, reinterpret_cast<uint32_t*>(s));
+              ptx::tmem_st_32x16(s_tmem + c0 + 16, reinterpret_cast<uint32_t*>(s) + 16);
+              back = true;
             }
           }
-#pragma unroll
+          if (chunks > 1 && back) ptx::tmem_st_wait();
+          if (!CAP && !BIAS) mt *= by;     // by > 0 in this instance
+          follow_maximum<DP>(mt, i == t, &m, &sum, o_tmem);
+          const float mu = m == -INFINITY ? 0.f : m;
+          const float2 by2 = make_float2(by, by), mu2 = make_float2(-mu, -mu);
           for (int x = 0; x < 4; ++x) {
-            const int shift = 32 * x - at;     // draft token of column 32 x
-            uint32_t drafted = shift <= -32 || shift >= 64 ? 0u : shift >= 0 ? (uint32_t)(seen >> shift) : (uint32_t)(seen << -shift);
-            see[x] &= bits_upto(at - 1, x) | drafted;
-          }
-        }
-        if ((see[0] & see[1] & see[2] & see[3]) != ~0u) {
+            uint32_t w[16] = {};
+            if (x >= chunk0 && x < chunk0 + chunks) {
+              if (chunks > 1) {
+                ptx::tmem_ld_32x32(s_tmem + 32 * x, reinterpret_cast<uint32_t*>(s));
+                ptx::tmem_ld_wait();
+              }
+              float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-          for (int c = 0; c < kTile; ++c) s[c] = (see[c >> 5] >> (c & 31)) & 1u ? s[c] : -INFINITY;
+              for (int c = 0; c < 32; c += 2) {
+                float2 z = make_float2(s[c], s[c + 1]);
+                z = CAP || BIAS ? ptx::add2(z, mu2) : ptx::fma2(z, by2, mu2);
+                const float2 e = make_float2(ex2(z.x), ex2(z.y));
+                add[(c >> 1) & 1] = ptx::add2(add[(c >> 1) & 1], e);
+                w[c >> 1] = pack2<BF16>(e.x, e.y);
+              }
+              sum += (add[0].x + add[0].y) + (add[1].x + add[1].y);
+            }
+            ptx::tmem_st_32x16(s_tmem + 16 * x, w);      // over scores that have been read: chunk x / 2
+          }
+          ptx::tmem_st_wait();
         }
-        weigh_tile<DP, BF16, CAP || BIAS>(s, by, i == t, &m, &sum, s_tmem, o_tmem);
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->p_full[t]));
       }
+      if (!ok) break;
       tile_no += count;
       if (seen == 0) {        // an unused token: no weight, whatever it would have seen
         m = -INFINITY;
         sum = 0.f;
       }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->q_empty[n & 1]));    // done with the tree
-      if (!ok) break;
       if (t == 1) {       // leave (m, sum) where the scores were, for the other warpgroup
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->q_empty[n & 1]));    // done with the tree
         if (count < 2) continue;
         if (!wait(&sh->o_full[1], mine & 1, 0x750000u)) break;
         ++mine;
@@ -581,49 +633,121 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         sum1 = __uint_as_float(r[1]);
       }
       ptx::tc_fence_after();
-      const float top = fmaxf(m, m1);
-      const float mu = top == -INFINITY ? 0.f : top;
-      const float f0 = ex2(m - mu), f1 = ex2(m1 - mu);
-      const float all = sum * f0 + sum1 * f1;
-      const bool whole = pc.first == 0 && pc.last == pc.tiles;
+      float top = fmaxf(m, m1);
+      float mu = top == -INFINITY ? 0.f : top;
+      float f0 = ex2(m - mu), f1 = ex2(m1 - mu);
+      float all = sum * f0 + sum1 * f1;
+      // The copies of a row meet in the piece's place of queries, which no product reads any more
+      // (o_full) and the loads get back only afterwards.
+      uint8_t* scratch = smem + (n & 1) * TILE;
+      auto meet = [&]() {
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->merged));
+        return wait(&sh->merged, merges++ & 1, 0x750003u);
+      };
+      if (p.copies > 1) {
+        float2* stats = reinterpret_cast<float2*>(scratch);
+        stats[copy * per_copy + in_copy] = make_float2(top, all);
+        if (!meet()) break;
+        const float own = top;
+        for (int x = 0; x < p.copies; ++x) top = fmaxf(top, stats[x * per_copy + in_copy].x);
+        mu = top == -INFINITY ? 0.f : top;
+        all = 0.f;
+        for (int x = 0; x < p.copies; ++x) {
+          const float2 y = stats[x * per_copy + in_copy];
+          all = fmaf(y.y, ex2(y.x - mu), all);
+        }
+        const float f = ex2(own - mu);
+        f0 *= f;
+        f1 *= f;
+        if (!meet()) break;      // everyone has read them
+      }
+      const bool whole = pc.first == 0 && pc.last == tiles_of(pc.places);
       const bool has = all > 0.f || all != all;
       const float norm = whole ? (has ? 1.f / all : 0.f) : 1.f;
       const float g0 = sum != 0.f ? f0 * norm : 0.f, g1 = sum1 != 0.f ? f1 * norm : 0.f;
       // of an unfinished piece: the run's last when it starts its sequence, else the run's first
       const long long slot = 2 * (long long)blockIdx.x + (pc.first == 0 ? 1 : 0);
-      float* part = p.partial + (slot * kTile + quarter * 32 + lane) * DP;
-      uint16_t* out = p.o + (((long long)pc.b * p.drafted + tok) * p.q_heads + h) * p.dim;
-#pragma unroll
-      for (int c = 0; c < DP; c += 32) {
+      // 32 columns of this thread's row, both warpgroups' parts
+      auto combined = [&](int c, float (&v)[32]) {
         uint32_t o[32], o1[32];
         ptx::tmem_ld_32x32(o_tmem + c, o);
         if (count >= 2) ptx::tmem_ld_32x32(o_tmem + DP + c, o1);
         ptx::tmem_ld_wait();
-        float v[32];
 #pragma unroll
         for (int x = 0; x < 32; ++x) {
           v[x] = g0 != 0.f ? __uint_as_float(o[x]) * g0 : 0.f;
           if (count >= 2 && g1 != 0.f) v[x] = fmaf(__uint_as_float(o1[x]), g1, v[x]);
         }
-        if (!real) continue;
-        if (whole) {
+      };
+      if (p.copies > 1) {
+        // All copies put their part down, 128 threads add them up and write whole rows.  Two copies'
+        // 64 rows fit in two turns.
+        const int wide = p.copies == 4 ? DP : DP / 2, vecs = wide / 4;
+        float4* meeting = reinterpret_cast<float4*>(scratch);      // [copy][row][wide / 4], rows under a swizzle
+        for (int c0 = 0; ok && c0 < DP; c0 += wide) {
+          if (any_row) {
+#pragma unroll 1
+            for (int c = 0; c < wide; c += 32) {
+              float v[32];
+              combined(c0 + c, v);
+              if (real) {
+                float4* to = meeting + (copy * p.rows + in_copy) * vecs + c / 4;
 #pragma unroll
-          for (int x = 0; x < 32; x += 8)
-            if (c + x < p.dim)
-              *reinterpret_cast<uint4*>(out + c + x) = make_uint4(pack2<BF16>(v[x], v[x + 1]), pack2<BF16>(v[x + 2], v[x + 3]),
-                                                                  pack2<BF16>(v[x + 4], v[x + 5]), pack2<BF16>(v[x + 6], v[x + 7]));
-        } else {
+                for (int x = 0; x < 8; ++x) to[x ^ (in_copy & 7)] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+              }
+            }
+          }
+          if (!meet()) break;
+          for (int e = threadIdx.x; e < p.rows * vecs; e += 128) {
+            const int r = e / vecs, at = e % vecs, from = at ^ (r & 7);
+            float4 z = meeting[r * vecs + from];
+            for (int y = 1; y < p.copies; ++y) {
+              const float4 u = meeting[(y * p.rows + r) * vecs + from];
+              z = make_float4(z.x + u.x, z.y + u.y, z.z + u.z, z.w + u.w);
+            }
+            const int c = c0 + 4 * at;
+            if (whole) {
+              const int tk = (int)fd_div((uint32_t)r, p.by_group);
+              const long long head = (pc.b * (long long)p.drafted + tk) * p.q_heads + pc.hk * p.group + r - tk * p.group;
+              if (c < p.dim) *reinterpret_cast<uint2*>(p.o + head * p.dim + c) = make_uint2(pack2<BF16>(z.x, z.y), pack2<BF16>(z.z, z.w));
+            } else {
+              *reinterpret_cast<float4*>(p.partial + (slot * kTile + r) * DP + c) = z;
+            }
+          }
+          if (c0 + wide < DP && !meet()) break;     // before the next turn writes there
+        }
+      } else if (any_row) {
+        float* part = p.partial + (slot * kTile + in_copy) * DP;
+        uint16_t* out = p.o + (((long long)pc.b * p.drafted + tok) * p.q_heads + h) * p.dim;
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          float v[32];
+          combined(c, v);
+          if (!real) continue;
+          if (whole) {
 #pragma unroll
-          for (int x = 0; x < 32; x += 4) *reinterpret_cast<float4*>(part + c + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+            for (int x = 0; x < 32; x += 8)
+              if (c + x < p.dim)
+                *reinterpret_cast<uint4*>(out + c + x) = make_uint4(pack2<BF16>(v[x], v[x + 1]), pack2<BF16>(v[x + 2], v[x + 3]),
+                                                                    pack2<BF16>(v[x + 4], v[x + 5]), pack2<BF16>(v[x + 6], v[x + 7]));
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; x += 4) *reinterpret_cast<float4*>(part + c + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+          }
         }
       }
-      if (real && !whole) {
+      if (!ok) break;
+      if (real && !whole && copy == 0) {
         float2* ms = reinterpret_cast<float2*>(p.partial + 2 * (long long)p.runs * kTile * DP);
-        ms[slot * kTile + quarter * 32 + lane] = make_float2(top, all);
+        ms[slot * kTile + in_copy] = make_float2(top, all);
       }
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->o_free));
+      if (lane == 0) {
+        ptx::mbar_arrive(ptx::smem_u32(&sh->o_free));
+        ptx::mbar_arrive(ptx::smem_u32(&sh->q_empty[n & 1]));    // done with the tree and the place of the queries
+      }
     }
   }
 
@@ -643,26 +767,26 @@ constexpr int kJoinThreads = 128;
 // did not: results whose tiles lie in several runs, and zeros where there is no tile.
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ TreeProblem p) {
-  __shared__ long long words[kJoinThreads / 32];
-  __shared__ long long first_unit;
+  __shared__ int words[kJoinThreads / 32];
+  __shared__ int first_unit;
   ptx::grid_dependency_wait();
   const int per_tile = p.k_heads * p.row_tiles;
-  const int b = blockIdx.x / per_tile, hr = blockIdx.x % per_tile, hk = hr / p.row_tiles, rt = hr % p.row_tiles;
+  const int b = blockIdx.x / per_tile, hr = blockIdx.x - b * per_tile, hk = hr / p.row_tiles, rt = hr - hk * p.row_tiles;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int tiles = tree_tiles(p, b);
-  long long total = 0, before;
+  const int tiles = tiles_of(tree_places(p, p.lengths[b]));
+  int total = 0, before;
   for (int base = 0; base < p.batch; base += kJoinThreads) {
     const int i = base + threadIdx.x;
-    const long long sum = block_scan<kJoinThreads>(i < p.batch ? (long long)tree_tiles(p, i) * per_tile : 0, &before, words);
-    if (i == b) first_unit = total + before + (long long)hr * tiles;
+    const int sum = block_scan<kJoinThreads>(i < p.batch ? tiles_of(tree_places(p, p.lengths[i])) * per_tile : 0, &before, words);
+    if (i == b) first_unit = total + before + hr * tiles;
     total += sum;
   }
   __syncthreads();
   int c0 = 0, c1 = -1;
   if (tiles > 0) {
-    const int runs = total < p.runs ? (int)total : p.runs;
-    auto run_of = [&](long long u) {     // the run that holds unit u
-      int c = (int)((double)u * runs / total);
+    const int runs = total < p.runs ? total : p.runs;
+    auto run_of = [&](int u) {     // the run that holds unit u
+      int c = (int)((float)u * runs / total);
       c = c < 0 ? 0 : c >= runs ? runs - 1 : c;
       while (c > 0 && run_begin(total, runs, c) > u) --c;
       while (c + 1 < runs && run_begin(total, runs, c + 1) <= u) ++c;
@@ -699,7 +823,7 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
       for (int e = 0; e < V; ++e) acc[e] = fmaf(v[e], f, acc[e]);
     }
     const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    const int tok = row / p.group, h = hk * p.group + row % p.group;
+    const int tok = (int)fd_div((uint32_t)row, p.by_group), h = hk * p.group + row - tok * p.group;
     uint16_t* out = p.o + (((long long)b * p.drafted + tok) * p.q_heads + h) * p.dim + lane * V;
     if (lane * V < p.dim) {
 #pragma unroll
