@@ -434,10 +434,12 @@ int32_t lego_rotary(const lego_rotary_t* desc, const void* x0, const void* x1, v
  * that sees nothing gets zeros and lse = -inf, and no gradient passes it.  Values of keys
  * and queries with a negative document are not used at all, be they NaN.
  * o: contiguous like q; lse: dev float[batch, q_heads, q_len], the natural logarithm of the
- * sum of exp(s).  Strides in elements (batch, token, head), multiples of 8, pointers 16-byte
+ * sum of exp(s).  o_low (nullable, like o): what the rounding of o to its type left over, in
+ * that type; given to the backward pass it keeps the gradients of rows with one large weight
+ * as exact as the others.  Strides in elements (batch, token, head), multiples of 8, pointers 16-byte
  * aligned; head_dim a multiple of 8 up to 128.  No counterpart in the reference.
  *
- * The backward pass takes o, lse as the forward pass left them and d_o (contiguous like q)
+ * The backward pass takes o, o_low (or NULL), lse as the forward pass left them and d_o (contiguous like q)
  * and writes contiguous dq, dk, dv: same bits on every run, no atomics.
  * workspace: lego_attention_workspace_bytes() bytes of device memory, 16-byte aligned, of
  * any contents, that no other call in flight uses.                              */
@@ -453,10 +455,10 @@ typedef struct lego_attention {
 
 int64_t lego_attention_workspace_bytes(const lego_attention_t* desc, int32_t backward);
 int32_t lego_attention_fwd(const lego_attention_t* desc, const void* q, const void* k, const void* v, void* o,
-                           float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+                           void* o_low, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 int32_t lego_attention_bwd(const lego_attention_t* desc, const void* q, const void* k, const void* v,
-                           const void* o, const float* lse, const void* d_o, void* dq, void* dk, void* dv,
-                           void* workspace, int64_t workspace_bytes, void* stream);
+                           const void* o, const void* o_low, const float* lse, const void* d_o, void* dq, void* dk,
+                           void* dv, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Attention of `drafted` (1 .. 64) new tokens per sequence over a paged cache.  Token t of
  * sequence b, whose keys and values stand in place lengths[b] + t of the sequence, sees the

@@ -154,8 +154,8 @@ SIGNATURES = {
                                                  C.POINTER(LayoutP), C.c_void_p, C.c_void_p]),
     "lego_rotary": (C.c_int32, [C.POINTER(Rotary)] + [C.c_void_p] * 7),
     "lego_attention_workspace_bytes": (C.c_int64, [C.POINTER(Attention), C.c_int32]),
-    "lego_attention_fwd": (C.c_int32, [C.POINTER(Attention)] + [C.c_void_p] * 6 + [C.c_int64, C.c_void_p]),
-    "lego_attention_bwd": (C.c_int32, [C.POINTER(Attention)] + [C.c_void_p] * 10 + [C.c_int64, C.c_void_p]),
+    "lego_attention_fwd": (C.c_int32, [C.POINTER(Attention)] + [C.c_void_p] * 7 + [C.c_int64, C.c_void_p]),
+    "lego_attention_bwd": (C.c_int32, [C.POINTER(Attention)] + [C.c_void_p] * 11 + [C.c_int64, C.c_void_p]),
     "lego_tree_attention_workspace_bytes": (C.c_int64, [C.POINTER(TreeAttention)]),
     "lego_tree_attention": (C.c_int32, [C.POINTER(TreeAttention)] + [C.c_void_p] * 9 + [C.c_int64, C.c_void_p]),
     "lego_copy_2d": (C.c_int32, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p]),

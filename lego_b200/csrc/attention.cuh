@@ -59,6 +59,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if constexpr (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -158,10 +164,10 @@ __device__ __forceinline__ void copy_tile_clean(uint8_t* tile, const uint16_t* b
 constexpr float kRescale = 8.f;
 
 // A row's reference value m for a tile whose maximum is mt (log2 units).  Not the first tile:
-// where some row of the warp outgrew its reference value, its sums, in `sum` and over DP columns
-// of o_tmem, follow it.
+// where some row of the warp outgrew its reference value, its sums, in two registers and over DP
+// columns of o_tmem, follow it.
 template <int DP>
-__device__ __forceinline__ void follow_maximum(float mt, bool first, float* m, float* sum, uint32_t o_tmem) {
+__device__ __forceinline__ void follow_maximum(float mt, bool first, float* m, float* sum, float* sum2, uint32_t o_tmem) {
   if (first) {
     *m = mt;
   } else if (__any_sync(~0u, mt > *m + kRescale)) {
@@ -169,6 +175,7 @@ __device__ __forceinline__ void follow_maximum(float mt, bool first, float* m, f
     const float f = mn == -INFINITY ? 1.f : ex2(*m - mn);
     *m = mn;
     *sum *= f;
+    *sum2 *= f;
 #pragma unroll
     for (int c = 0; c < DP; c += 16) {     // rare, and the scores fill the registers
       uint32_t o[16];
@@ -183,18 +190,20 @@ __device__ __forceinline__ void follow_maximum(float mt, bool first, float* m, f
 
 // One thread per row: the row's 128 scores s (hidden ones -inf) become weights
 // 2^(s by - m) (SCALED: s is in log2 units already), packed to 16 bits over columns 0 .. 63 of
-// s_tmem; their sum, before that rounding, is added to `sum`.  by > 0.
+// s_tmem.  `sum` takes the weights as they are, for the row's logarithm; `packed_sum` as they
+// were rounded: divided by it, the result's weights add up to one, so an error all of them
+// share, above all that of a row's one large weight, falls out.  by > 0.
 template <int DP, bool BF16, bool SCALED>
 __device__ __forceinline__ void weigh_tile(const float (&s)[kTile], float by, bool first, float* m, float* sum,
-                                           uint32_t s_tmem, uint32_t o_tmem) {
+                                           float* packed_sum, uint32_t s_tmem, uint32_t o_tmem) {
   float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
   for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
   float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   if (!SCALED) mt *= by;
-  follow_maximum<DP>(mt, first, m, sum, o_tmem);
+  follow_maximum<DP>(mt, first, m, sum, packed_sum, o_tmem);
   const float mu = *m == -INFINITY ? 0.f : *m;
-  float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, packed_add[2] = {add[0], add[0]};
   const float2 by2 = make_float2(by, by), mu2 = make_float2(-mu, -mu);
 #pragma unroll
   for (int c = 0; c < kTile; c += 32) {
@@ -204,12 +213,15 @@ __device__ __forceinline__ void weigh_tile(const float (&s)[kTile], float by, bo
       float2 z = make_float2(s[c + i], s[c + i + 1]);
       z = SCALED ? ptx::add2(z, mu2) : ptx::fma2(z, by2, mu2);
       const float2 x = make_float2(ex2(z.x), ex2(z.y));
-      add[(i >> 1) & 1] = ptx::add2(add[(i >> 1) & 1], x);
+      const int k = (i >> 1) & 1;
+      add[k] = ptx::add2(add[k], x);
       w[i >> 1] = pack2<BF16>(x.x, x.y);
+      packed_add[k] = ptx::add2(packed_add[k], unpack2<BF16>(w[i >> 1]));
     }
     ptx::tmem_st_32x16(s_tmem + c / 2, w);
   }
   *sum += (add[0].x + add[0].y) + (add[1].x + add[1].y);
+  *packed_sum += (packed_add[0].x + packed_add[0].y) + (packed_add[1].x + packed_add[1].y);
   ptx::tmem_st_wait();
 }
 

@@ -40,7 +40,7 @@ struct BwdArgs {
   CUtensorMap q, k, v, d_o;          // boxes of 128 tokens
   CUtensorMap dq, dk, dv;            // boxes of 32 tokens
   AttnProblem p;
-  const uint16_t *q_raw, *k_raw, *o_raw, *do_raw, *v_raw;
+  const uint16_t *q_raw, *k_raw, *o_raw, *low_raw, *do_raw, *v_raw;    // low_raw: what o's rounding left, or null
   const float* lse;
   float *neg_lse, *neg_delta;        // [batch][q_heads][q_len up to whole tiles], log2 units
   uint32_t* peak;                    // fp16: [batch][k_heads][2] bits of max|dO|, max|V|
@@ -66,12 +66,6 @@ __device__ __forceinline__ void raise_peak(uint32_t* at, uint32_t bits) {
 
 // ---- preparation -----------------------------------------------------------------------------
 
-template <bool BF16>
-__device__ __forceinline__ float2 unpack2(uint32_t v) {
-  if constexpr (BF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
-  else return __half22float2(*reinterpret_cast<const __half2*>(&v));
-}
-
 // A warp per row, four values a lane: delta, the negated log-sum, and in fp16 the peaks of dO
 // and V.  Rows past q_len (whole tiles) and padding get weight zero: -inf.  Memory bound; the
 // peaks are maxima, so the order of the atomics does not matter.
@@ -93,7 +87,13 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __grid_constan
       if (lane * 4 < p.dim) {
         const uint2 x = *reinterpret_cast<const uint2*>(a.o_raw + at + lane * 4);
         const uint2 g = *reinterpret_cast<const uint2*>(a.do_raw + at + lane * 4);
-        const float2 x0 = unpack2<BF16>(x.x), x1 = unpack2<BF16>(x.y), g0 = unpack2<BF16>(g.x), g1 = unpack2<BF16>(g.y);
+        float2 x0 = unpack2<BF16>(x.x), x1 = unpack2<BF16>(x.y);
+        const float2 g0 = unpack2<BF16>(g.x), g1 = unpack2<BF16>(g.y);
+        if (a.low_raw) {
+          const uint2 y = *reinterpret_cast<const uint2*>(a.low_raw + at + lane * 4);
+          x0 = ptx::add2(x0, unpack2<BF16>(y.x));
+          x1 = ptx::add2(x1, unpack2<BF16>(y.y));
+        }
         delta = fmaf(x0.x, g0.x, fmaf(x0.y, g0.y, fmaf(x1.x, g1.x, x1.y * g1.y)));
         peak = fmaxf(fmaxf(fabsf(g0.x), fabsf(g0.y)), fmaxf(fabsf(g1.x), fabsf(g1.y)));
       }
@@ -899,13 +899,13 @@ int64_t lego_attention_workspace_bytes(const lego_attention_t* d, int32_t backwa
 }
 
 int32_t lego_attention_bwd(const lego_attention_t* d, const void* q, const void* k, const void* v, const void* o,
-                           const float* lse, const void* d_o, void* dq, void* dk, void* dv, void* workspace,
-                           int64_t workspace_bytes, void* stream) {
+                           const void* o_low, const float* lse, const void* d_o, void* dq, void* dk, void* dv,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
   BwdArgs a = {};
   int32_t st = attention_problem(d, &a.p);
   if (st != LEGO_OK) return st;
   if (!q || !k || !v || !o || !lse || !d_o || !dq || !dk || !dv || !workspace) return LEGO_ERR_NULL;
-  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)d_o | (uintptr_t)dq | (uintptr_t)dk |
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)o_low | (uintptr_t)d_o | (uintptr_t)dq | (uintptr_t)dk |
        (uintptr_t)dv | (uintptr_t)workspace) & 15)
     return LEGO_ERR_ALIGN;
   const AttnProblem& p = a.p;
@@ -932,6 +932,7 @@ int32_t lego_attention_bwd(const lego_attention_t* d, const void* q, const void*
   a.k_raw = (const uint16_t*)k;
   a.v_raw = (const uint16_t*)v;
   a.o_raw = (const uint16_t*)o;
+  a.low_raw = (const uint16_t*)o_low;
   a.do_raw = (const uint16_t*)d_o;
   a.lse = lse;
   a.neg_lse = reinterpret_cast<float*>(ws + l.neg_lse);

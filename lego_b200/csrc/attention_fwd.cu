@@ -11,9 +11,10 @@
 //
 // Running maximum: the reference value m of a row moves only when a tile's maximum exceeds it
 // by more than 2^8 -- weights stay below 2^8, the row sum is kept in 32 bits -- so O in
-// TMEM is rarely rescaled.  The sum adds the weights before they are rounded to 16 bits;
-// that rounding, half a step of the type per weight, and the one of the result are the only
-// ones below 32 bits.
+// TMEM is rarely rescaled.  The rounding of the weights to 16 bits, half a step of the type
+// each, and the one of the result are the only ones below 32 bits.  What the last one takes
+// away goes to a second output where the caller wants it: the backward pass subtracts dO O
+// from terms of nearly the same size wherever a row has one large weight.
 //
 // Tiles no row of the CTA sees are not loaded (causal and prefix limits, document ranges);
 // the mask is evaluated only on tiles that are not seen whole, as 128 bits per row.
@@ -35,7 +36,8 @@ template <int DP> constexpr int fwd_stages() { return DP == 128 ? 5 : 8; }
 template <int DP> constexpr int fwd_smem() { return (2 + fwd_stages<DP>()) * tile_bytes<DP>() + 1024 + 512; }
 
 struct FwdArgs {
-  CUtensorMap q, k, v, o;
+  CUtensorMap q, k, v, o, o_low;
+  int low;              // o_low is wanted
   AttnProblem p;
   const uint16_t* v_raw;
   float* lse;
@@ -254,7 +256,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
     const float by = p.scale * kLog2e;
     const float u_by = CAP ? 2.f * kLog2e * p.scale / p.softcap : 0.f, cap_by = p.softcap * kLog2e;
     const float slope = BIAS && p.slopes ? p.slopes[h] * kLog2e : 0.f;
-    float m = -INFINITY, sum = 0.f;
+    float m = -INFINITY, sum = 0.f, packed_sum = 0.f;
     bool ok = true;
     for (int j = l; j < e; ++j) {
       const int j0 = j * kTile;
@@ -297,14 +299,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
 #pragma unroll
         for (int c = 0; c < kTile; ++c) s[c] = (see[c >> 5] >> (c & 31)) & 1u ? s[c] : -INFINITY;
       }
-      weigh_tile<DP, BF16, CAP || BIAS>(s, by, j == l, &m, &sum, s_tmem, o_tmem);
+      weigh_tile<DP, BF16, CAP || BIAS>(s, by, j == l, &m, &sum, &packed_sum, s_tmem, o_tmem);
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->p_full[t]));
     }
     // result
     const bool has = sum > 0.f || sum != sum;
-    const float inv = has ? 1.f / sum : 0.f;
+    const float inv = packed_sum > 0.f || sum != sum ? 1.f / packed_sum : 0.f;
     if (row < p.q_len && ok)
       a.lse[((long long)b * p.q_heads + h) * p.q_len + row] = has ? (m + log2f(sum)) * kLn2 : -INFINITY;
     if (ok && l < e) {
@@ -315,7 +317,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
       }
       ptx::tc_fence_after();
     }
-    if (ok && q0 + quarter * 32 < p.q_len) {   // the tile's own queries are no longer needed: stage there
+    for (int low = 0; ok && low <= a.low && q0 + quarter * 32 < p.q_len; ++low) {   // the tile's own queries are no longer needed: stage there
 #pragma unroll
       for (int c = 0; c < DP; c += 32) {
         uint32_t o[32];
@@ -328,8 +330,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
         for (int i = 0; i < 4; ++i) {
           uint32_t w[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            w[k] = has ? pack2<BF16>(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv) : 0u;
+          for (int k = 0; k < 4; ++k) {
+            const float x = __uint_as_float(o[8 * i + 2 * k]) * inv, y = __uint_as_float(o[8 * i + 2 * k + 1]) * inv;
+            w[k] = inv != 0.f ? pack2<BF16>(x, y) : 0u;
+            if (low) {
+              const float2 z = unpack2<BF16>(w[k]);
+              w[k] = inv != 0.f ? pack2<BF16>(x - z.x, y - z.y) : 0u;
+            }
+          }
           *reinterpret_cast<uint4*>(dst + (((((c & 32) >> 3) + i) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
@@ -339,11 +347,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
           const int32_t at[5] = {c * 64, q0 + quarter * 32, h, b, 0};
-          ptx::tma_store_nd(4, &a.o, at, q_smem + t * TILE + c * kBoxBytes + quarter * 4096);
+          ptx::tma_store_nd(4, low ? &a.o_low : &a.o, at, q_smem + t * TILE + c * kBoxBytes + quarter * 4096);
         }
         ptx::bulk_commit_group();
         ptx::bulk_wait_group_read<0>();
       }
+      __syncwarp();
     }
   }
 
@@ -384,12 +393,13 @@ int32_t launch_fwd_scores(const FwdArgs& a, int device, cudaStream_t s) {
 using namespace lego;
 
 extern "C" int32_t lego_attention_fwd(const lego_attention_t* d, const void* q, const void* k, const void* v, void* o,
-                                      float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+                                      void* o_low, float* lse, void* workspace, int64_t workspace_bytes,
+                                      void* stream) {
   FwdArgs a = {};
   int32_t st = attention_problem(d, &a.p);
   if (st != LEGO_OK) return st;
   if (!q || !k || !v || !o || !lse) return LEGO_ERR_NULL;
-  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)workspace) & 15) return LEGO_ERR_ALIGN;
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)o_low | (uintptr_t)workspace) & 15) return LEGO_ERR_ALIGN;
   const int64_t need = lego_attention_workspace_bytes(d, 0);
   if (need && !workspace) return LEGO_ERR_NULL;
   if (workspace_bytes < need) return LEGO_ERR_SIZE;
@@ -403,8 +413,10 @@ extern "C" int32_t lego_attention_fwd(const lego_attention_t* d, const void* q, 
   if (make_tmap_heads(enc, &a.q, bf16, q, p.dim, p.q_len, p.q_heads, p.batch, p.q_stride, kTile) != LEGO_OK ||
       make_tmap_heads(enc, &a.k, bf16, k, p.dim, p.k_len, p.k_heads, p.batch, p.k_stride, kTile) != LEGO_OK ||
       make_tmap_heads(enc, &a.v, bf16, v, p.dim, p.k_len, p.k_heads, p.batch, p.v_stride, kTile) != LEGO_OK ||
-      make_tmap_heads(enc, &a.o, bf16, o, p.dim, p.q_len, p.q_heads, p.batch, o_stride, 32) != LEGO_OK)
+      make_tmap_heads(enc, &a.o, bf16, o, p.dim, p.q_len, p.q_heads, p.batch, o_stride, 32) != LEGO_OK ||
+      (o_low && make_tmap_heads(enc, &a.o_low, bf16, o_low, p.dim, p.q_len, p.q_heads, p.batch, o_stride, 32) != LEGO_OK))
     return LEGO_ERR_UNSUPPORTED;
+  a.low = o_low != nullptr;
   cudaStream_t s = (cudaStream_t)stream;
   st = attention_docs(&a.p, workspace, s);
   if (st != LEGO_OK) return st;

@@ -570,7 +570,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
           }
           if (chunks > 1 && back) ptx::tmem_st_wait();
           if (!CAP && !BIAS) mt *= by;     // by > 0 in this instance
-          follow_maximum<DP>(mt, i == t, &m, &sum, o_tmem);
+          float unused = 0.f;
+          follow_maximum<DP>(mt, i == t, &m, &sum, &unused, o_tmem);
           const float mu = m == -INFINITY ? 0.f : m;
           const float2 by2 = make_float2(by, by), mu2 = make_float2(-mu, -mu);
           for (int x = 0; x < 4; ++x) {
@@ -585,9 +586,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
               for (int c = 0; c < 32; c += 2) {
                 float2 z = make_float2(s[c], s[c + 1]);
                 z = CAP || BIAS ? ptx::add2(z, mu2) : ptx::fma2(z, by2, mu2);
-                const float2 e = make_float2(ex2(z.x), ex2(z.y));
-                add[(c >> 1) & 1] = ptx::add2(add[(c >> 1) & 1], e);
-                w[c >> 1] = pack2<BF16>(e.x, e.y);
+                w[c >> 1] = pack2<BF16>(ex2(z.x), ex2(z.y));
+                add[(c >> 1) & 1] = ptx::add2(add[(c >> 1) & 1], unpack2<BF16>(w[c >> 1]));     // as they count in O
               }
               sum += (add[0].x + add[0].y) + (add[1].x + add[1].y);
             }

@@ -19,6 +19,7 @@ op raises; there is no CPU implementation behind them.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 from typing import List, Optional, Sequence
@@ -784,16 +785,26 @@ _ATTN_TYPES = {torch.float16: _abi.F16, torch.bfloat16: _abi.BF16}
 _ROTARY_TYPES = {**_ATTN_TYPES, torch.float32: _abi.F32}
 
 
-def _same_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
+def _same_device(*tensors: Optional[torch.Tensor]) -> torch.device:
     """The device of a call: that of its CUDA tensors, which have to share one (host tensors are
     staged to it); the current device when all are host tensors."""
-    dev = None
-    for t in (first, *others):
-        if t is not None and t.is_cuda:
-            if dev is not None and t.device != dev:
-                raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-            dev = t.device
-    return dev if dev is not None else _device()
+    at = -1
+    for t in tensors:
+        if t is not None:
+            n = t.get_device()
+            if n != at and n >= 0:
+                if at >= 0:
+                    raise ValueError(f"tensors on different devices: cuda:{at} and cuda:{n}")
+                at = n
+    return torch.device("cuda", at) if at >= 0 else _device()
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev: torch.device):
+    """The call's device made current, where it is not."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _ready(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
@@ -806,20 +817,27 @@ def _dense(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _strided(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
-    """On the device in a form the kernels read in place: last axis contiguous, the other strides
-    whole 16-byte steps, the first value on such a boundary; a copy where it is not."""
-    t = _ready(t, dev)
-    steps = 16 // t.element_size()
-    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0 and all(
-            n == 1 or (s > 0 and s % steps == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])):
-        return t
-    return _dense(t, dev)
+def _strided(t: torch.Tensor, dev: torch.device):
+    """A tensor ``[a, b, c, D]`` on the device in a form the kernels read in place -- last axis
+    contiguous, the other strides whole 16-byte steps, the first value on such a boundary; a copy
+    where it is not -- and the strides of its leading axes in elements."""
+    if not t.is_cuda:
+        t = t.to(dev, non_blocking=True)
+    _, b, c, d = t.shape
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t, (b * c * d, c * d, d)
+        steps = 16 // t.element_size()
+        if t.stride(-1) == 1 and all(n == 1 or (s > 0 and s % steps == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])):
+            return t, _strides(t)
+    return _dense(t, dev), (b * c * d, c * d, d)
 
 
 def _strides(t: torch.Tensor):
-    """Strides of the leading axes in elements; an axis of one has none of its own."""
-    return tuple(t.shape[-1] if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+    """Strides of the leading axes of ``[a, b, c, D]`` in elements; an axis of one has none of its own."""
+    a, b, c, d = t.shape
+    s = t.stride()
+    return (s[0] if a != 1 else d, s[1] if b != 1 else d, s[2] if c != 1 else d)
 
 
 def _check_int32(t: Optional[torch.Tensor], name: str, shape) -> None:
@@ -897,21 +915,21 @@ def _rotary(xs, positions, freqs, pairs, scale, inverse):
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
     dev = _same_device(*xs, positions, freqs)
-    with torch.cuda.device(dev):
-        src = [_ready(t, dev) for t in xs]
-        src = [t if t.stride(-1) == 1 or D == 1 else t.contiguous() for t in src]
+    with _on(dev):
         pos, fr = _ready(positions, dev), _ready(freqs, dev).contiguous()
-        out = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in src]
-        d = _abi.Rotary(dtype=_ROTARY_TYPES[x.dtype], pairs=kind, inverse=int(inverse), position_bytes=pos.element_size(),
-                        batch=B, length=S, head_dim=D, rotary_dim=2 * fr.numel(), scale=float(scale))
-        d.position_stride[:] = (0 if pos.dim() == 1 else pos.stride(0), pos.stride(-1))
-        for i, t in enumerate(src):
-            d.heads[i] = t.shape[2]
-            d.stride[i][:] = _strides(t)
-        two = len(src) > 1
-        _abi.check(_abi.lib().lego_rotary(C.byref(d), src[0].data_ptr(), src[1].data_ptr() if two else None,
-                                          out[0].data_ptr(), out[1].data_ptr() if two else None, pos.data_ptr(),
-                                          fr.data_ptr(), _stream()), "lego_rotary")
+        src, out = [], []
+        for t in xs:
+            t = _ready(t, dev)
+            src.append(t if t.stride(3) == 1 or D == 1 else t.contiguous())
+            out.append(torch.empty(t.shape, dtype=t.dtype, device=dev))
+        one, two = src[0], src[1] if len(src) > 1 else None
+        d = _abi.Rotary(_ROTARY_TYPES[x.dtype], kind, inverse, pos.element_size(), B, S, D, 2 * fr.numel(),
+                        (one.shape[2], 0 if two is None else two.shape[2]),
+                        (_strides(one), (0, 0, 0) if two is None else _strides(two)),
+                        (0 if pos.dim() == 1 else pos.stride(0), pos.stride(-1)), scale)
+        _abi.check(_abi.lib().lego_rotary(C.byref(d), one.data_ptr(), _ptr(two), out[0].data_ptr(),
+                                          None if two is None else out[1].data_ptr(), pos.data_ptr(), fr.data_ptr(),
+                                          _stream()), "lego_rotary")
         return [_like_input(o, t) for o, t in zip(out, xs)]
 
 
@@ -973,12 +991,13 @@ def _attention_desc(q, k, v, causal, prefix, documents, softcap, slopes, scale):
     _check_slopes(slopes, Hq)
     scale, softcap = _scores(scale, softcap, D)
     dev = _same_device(q, k, v, prefix, documents, slopes)
-    keep = [_strided(q, dev), _strided(k, dev), _strided(v, dev), _optional(prefix, dev), _optional(documents, dev),
-            _optional(slopes, dev)]
-    d = _abi.Attention(dtype=_ATTN_TYPES[q.dtype], causal=int(bool(causal)), batch=B, q_len=Sq, k_len=Sk, q_heads=Hq,
-                       k_heads=Hk, head_dim=D, scale=scale, softcap=softcap, prefix=_ptr(keep[3]),
-                       documents=_ptr(keep[4]), slopes=_ptr(keep[5]))
-    d.q_stride[:], d.k_stride[:], d.v_stride[:] = (_strides(t) for t in keep[:3])
+    (qd, q_st), (kd, k_st), (vd, v_st) = _strided(q, dev), _strided(k, dev), _strided(v, dev)
+    keep = [qd, kd, vd]
+    d = _abi.Attention(_ATTN_TYPES[q.dtype], 1 if causal else 0, B, Sq, Sk, Hq, Hk, D, q_st, k_st, v_st, scale, softcap)
+    for name, t in (("slopes", slopes), ("prefix", prefix), ("documents", documents)):
+        if t is not None:
+            keep.append(_ready(t, dev).contiguous())
+            setattr(d, name, keep[-1].data_ptr())
     return dev, d, keep
 
 
@@ -988,44 +1007,61 @@ def _attention_workspace(d, backward, dev):
     return torch.empty(max(n, 16), dtype=torch.uint8, device=dev), n
 
 
-def attention_fwd(q, k, v, causal=False, prefix=None, documents=None, softcap=0.0, slopes=None, scale=None):
-    """Attention forward: ``(o, lse)``, see ``attention``; lse is float32 ``[B, Hq, Sq]``."""
+def _attention_fwd(q, k, v, causal, prefix, documents, softcap, slopes, scale, low):
+    """``(o, lse, what o's rounding left or None)``."""
     dev, d, keep = _attention_desc(q, k, v, causal, prefix, documents, softcap, slopes, scale)
-    B, Sq, Hq, _ = q.shape
-    with torch.cuda.device(dev):
-        o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    B, Sq, Hq, _ = shape = q.shape
+    with _on(dev):
+        o = torch.empty(shape, dtype=q.dtype, device=dev)
         lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=dev)
+        o_low = torch.empty(shape, dtype=q.dtype, device=dev) if low else None
         if k.shape[1] == 0:
             o.zero_()
             lse.fill_(-math.inf)
+            o_low = None
         elif o.numel():
-            ws, n = _attention_workspace(d, 0, dev)
-            _abi.check(_abi.lib().lego_attention_fwd(C.byref(d), *(t.data_ptr() for t in keep[:3]), o.data_ptr(),
-                                                     lse.data_ptr(), ws.data_ptr(), n, _stream()), "lego_attention_fwd")
-        return _like_input(o, q), _like_input(lse, q)
+            # only document summaries need a workspace
+            ws, n = _attention_workspace(d, 0, dev) if documents is not None else (None, 0)
+            _abi.check(_abi.lib().lego_attention_fwd(C.byref(d), keep[0].data_ptr(), keep[1].data_ptr(), keep[2].data_ptr(),
+                                                     o.data_ptr(), _ptr(o_low), lse.data_ptr(), _ptr(ws), n, _stream()),
+                       "lego_attention_fwd")
+        if q.is_cuda:
+            return o, lse, o_low
+        return _to_host(o), _to_host(lse), None if o_low is None else _to_host(o_low)
 
 
-def attention_bwd(do, q, k, v, o, lse, causal=False, prefix=None, documents=None, softcap=0.0, slopes=None, scale=None):
+def attention_fwd(q, k, v, causal=False, prefix=None, documents=None, softcap=0.0, slopes=None, scale=None):
+    """Attention forward: ``(o, lse)``, see ``attention``; lse is float32 ``[B, Hq, Sq]``."""
+    return _attention_fwd(q, k, v, causal, prefix, documents, softcap, slopes, scale, False)[:2]
+
+
+def attention_bwd(do, q, k, v, o, lse, causal=False, prefix=None, documents=None, softcap=0.0, slopes=None, scale=None,
+                  o_low=None):
     """Attention backward from what ``attention_fwd`` took and gave: ``(dq, dk, dv)``, contiguous,
-    the same bits on every run."""
+    the same bits on every run.  ``o_low``: what the rounding of o left, as ``LEGOAttention`` keeps it;
+    without it the gradients of rows with one large weight carry that rounding too."""
     dev, d, keep = _attention_desc(q, k, v, causal, prefix, documents, softcap, slopes, scale)
-    _same_device(do, o, lse, keep[0])
+    _same_device(do, o, lse, o_low, keep[0])
     B, Sq, Hq, _ = q.shape
-    if do.shape != q.shape or o.shape != q.shape or tuple(lse.shape) != (B, Hq, Sq):
+    if do.shape != q.shape or o.shape != q.shape or tuple(lse.shape) != (B, Hq, Sq) or (
+            o_low is not None and o_low.shape != q.shape):
         raise ValueError("do and o must have q's shape, lse [B, Hq, Sq]")
-    if do.dtype != q.dtype or o.dtype != q.dtype or lse.dtype != torch.float32:
+    if do.dtype != q.dtype or o.dtype != q.dtype or lse.dtype != torch.float32 or (
+            o_low is not None and o_low.dtype != q.dtype):
         raise ValueError("do and o must have q's type, lse float32")
-    with torch.cuda.device(dev):
+    with _on(dev):
         dod, od, lsed = _dense(do, dev), _dense(o, dev), _dense(lse, dev)
+        lowd = None if o_low is None else _dense(o_low, dev)
         dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=dev) for t in (q, k, v))
         if dq.numel() == 0 or dk.numel() == 0:
             for g in (dq, dk, dv):
                 g.zero_()
         else:
             ws, n = _attention_workspace(d, 1, dev)
-            _abi.check(_abi.lib().lego_attention_bwd(C.byref(d), *(t.data_ptr() for t in keep[:3]), od.data_ptr(),
-                                                     lsed.data_ptr(), dod.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-                                                     dv.data_ptr(), ws.data_ptr(), n, _stream()), "lego_attention_bwd")
+            _abi.check(_abi.lib().lego_attention_bwd(C.byref(d), keep[0].data_ptr(), keep[1].data_ptr(), keep[2].data_ptr(),
+                                                     od.data_ptr(), _ptr(lowd), lsed.data_ptr(), dod.data_ptr(), dq.data_ptr(),
+                                                     dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n, _stream()),
+                       "lego_attention_bwd")
         return _like_input(dq, q), _like_input(dk, k), _like_input(dv, v)
 
 
@@ -1034,10 +1070,10 @@ class LEGOAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, causal, prefix, documents, softcap, slopes, scale):
-        o, lse = attention_fwd(q, k, v, causal, prefix, documents, softcap, slopes, scale)
+        o, lse, o_low = _attention_fwd(q, k, v, causal, prefix, documents, softcap, slopes, scale, True)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(lse)
-        ctx.save_for_backward(q, k, v, o, lse, prefix, documents, slopes)
+        ctx.save_for_backward(q, k, v, o, lse, o_low, prefix, documents, slopes)
         ctx.rest = (causal, softcap, scale)
         return o, lse
 
@@ -1046,9 +1082,9 @@ class LEGOAttention(torch.autograd.Function):
     def backward(ctx, do, _):
         if do is None:
             return (None,) * 9
-        q, k, v, o, lse, prefix, documents, slopes = ctx.saved_tensors
+        q, k, v, o, lse, o_low, prefix, documents, slopes = ctx.saved_tensors
         causal, softcap, scale = ctx.rest
-        return (*attention_bwd(do, q, k, v, o, lse, causal, prefix, documents, softcap, slopes, scale), *(None,) * 6)
+        return (*attention_bwd(do, q, k, v, o, lse, causal, prefix, documents, softcap, slopes, scale, o_low), *(None,) * 6)
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False,
@@ -1111,21 +1147,21 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _check_slopes(slopes, Hq)
     scale, softcap = _scores(scale, softcap, D)
     dev = _same_device(q, k_cache, v_cache, page_table, lengths, parents, slopes)
-    with torch.cuda.device(dev):
-        table, lens, par, sl = (_optional(t, dev) for t in (page_table, lengths, parents, slopes))
-        qd, kd, vd = _strided(q, dev), _strided(k_cache, dev), _strided(v_cache, dev)
+    with _on(dev):
+        table, lens = _ready(page_table, dev).contiguous(), _ready(lengths, dev).contiguous()
+        par, sl = _optional(parents, dev), _optional(slopes, dev)
+        (qd, q_st), (kd, k_st), (vd, v_st) = _strided(q, dev), _strided(k_cache, dev), _strided(v_cache, dev)
         o = torch.empty(q.shape, dtype=q.dtype, device=dev)
         if B == 0 or Hq == 0:
             return _like_input(o, q)
-        d = _abi.TreeAttention(dtype=_ATTN_TYPES[q.dtype], batch=B, drafted=T, q_heads=Hq, k_heads=Hk, head_dim=D,
-                               pages=pages, page_size=page_size, max_pages=table.shape[1], table_stride=table.shape[1],
-                               scale=scale, softcap=softcap)
-        d.q_stride[:], d.k_stride[:], d.v_stride[:] = _strides(qd), _strides(kd), _strides(vd)
-        lib = _abi.lib()
-        n = lib.lego_tree_attention_workspace_bytes(C.byref(d))
+        n_table = table.shape[1]
+        d = _abi.TreeAttention(_ATTN_TYPES[q.dtype], 0, B, T, Hq, Hk, D, pages, page_size, n_table, n_table, q_st, k_st, v_st,
+                               scale, softcap)
+        lib, ref = _abi.lib(), C.byref(d)
+        n = lib.lego_tree_attention_workspace_bytes(ref)
         _abi.check(min(n, 0), "lego_tree_attention_workspace_bytes")
-        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
-        _abi.check(lib.lego_tree_attention(C.byref(d), qd.data_ptr(), kd.data_ptr(), vd.data_ptr(), table.data_ptr(),
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        _abi.check(lib.lego_tree_attention(ref, qd.data_ptr(), kd.data_ptr(), vd.data_ptr(), table.data_ptr(),
                                            lens.data_ptr(), _ptr(par), _ptr(sl), o.data_ptr(), ws.data_ptr(), n,
                                            _stream()), "lego_tree_attention")
         return _like_input(o, q)

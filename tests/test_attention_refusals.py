@@ -103,11 +103,11 @@ def test_the_c_entry_points_return_their_reasons():
     odd.k_stride[1] = 65
     assert lib.lego_attention_workspace_bytes(C.byref(odd), 0) == -7
     d = attention_desc()
-    args = [4096] * 5
+    args = [4096] * 6
     assert lib.lego_attention_fwd(C.byref(d), 0, *args[1:], 4096, 1 << 20, None) == -1
     assert lib.lego_attention_fwd(C.byref(d), 4098, *args[1:], 4096, 1 << 20, None) == -7
-    assert lib.lego_attention_bwd(C.byref(d), *[4096] * 10, 0, None) == -6
-    assert lib.lego_attention_bwd(C.byref(d), *[4096] * 9, None, 1 << 30, None) == -1
+    assert lib.lego_attention_bwd(C.byref(d), *[4096] * 11, 0, None) == -6
+    assert lib.lego_attention_bwd(C.byref(d), *[4096] * 10, None, 1 << 30, None) == -1
 
     r = _abi.Rotary(dtype=_abi.F16, pairs=0, position_bytes=4, batch=1, length=4, head_dim=64, rotary_dim=64, scale=1.0)
     r.heads[:] = (1, 0)
