@@ -128,11 +128,18 @@ __device__ __forceinline__ void mask_documents(uint32_t (&m)[W], const int (&oth
 // swizzle: as a K-major operand its 16-value steps are 32 bytes apart inside a box, as an
 // MN-major one 16 tokens are 2 KiB and 64 values one box apart.
 template <int DP> constexpr int tile_bytes() { return DP / 64 * kBoxBytes; }
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t tile, int step) {   // step: 16 values
-  return ptx::smem_desc_sw128(tile + (step >> 2) * kBoxBytes + (step & 3) * 32, 16, 1024);
+// The descriptors of a tile differ in the low word only, by a constant per step: one addition.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t low) {
+  constexpr uint32_t high = (1024u >> 4) | (1u << 14) | (2u << 29);    // smem_desc_sw128: stride 1024, swizzle
+  return (uint64_t)high << 32 | low;
 }
-__device__ __forceinline__ uint64_t desc_mn_major(uint32_t tile, int step) {  // step: 16 tokens
-  return ptx::smem_desc_sw128(tile + step * 2048, kBoxBytes, 1024);
+__device__ __forceinline__ uint32_t low_k_major(uint32_t tile) { return (tile >> 4) + (1u << 16); }
+__device__ __forceinline__ uint32_t low_mn_major(uint32_t tile) { return (tile >> 4) + ((uint32_t)(kBoxBytes >> 4) << 16); }
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t low, int step) {    // step: 16 values
+  return tile_desc(low + (((step >> 2) * kBoxBytes + (step & 3) * 32) >> 4));
+}
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t low, int step) {   // step: 16 tokens
+  return tile_desc(low + ((step * 2048) >> 4));
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t idesc_of(int n, bool b_mn) {

@@ -365,12 +365,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
       };
       auto score_product = [&](uint32_t d, uint32_t own, uint32_t other, uint64_t* bar) {
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) ptx::mma_f16_ss(d, desc_k_major(own, s), desc_k_major(other, s), id_s, s != 0);
+        for (int s = 0; s < DP / 16; ++s) ptx::mma_f16_ss(d, desc_k_major(low_k_major(own), s), desc_k_major(low_k_major(other), s), id_s, s != 0);
         ptx::mma_commit(ptx::smem_u32(bar));
       };
       auto sum_product = [&](uint32_t d, uint32_t w, uint32_t other, bool add, uint64_t* bar) {
 #pragma unroll
-        for (int s = 0; s < kTile / 16; ++s) ptx::mma_f16_ts(d, w + packed_at(s), desc_mn_major(other, s), id_d, add || s != 0);
+        for (int s = 0; s < kTile / 16; ++s) ptx::mma_f16_ts(d, w + packed_at(s), desc_mn_major(low_mn_major(other), s), id_d, add || s != 0);
         ptx::mma_commit(ptx::smem_u32(bar));
       };
       wait(&sh->kv_full[0], 0, 0x520000u);
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
         if (!ok) return;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
-          ptx::mma_f16_ss(s_at + (n & 1) * kTile, desc_k_major(q_smem, s), desc_k_major(k_smem + (n % NK) * TILE, s), id_s, s != 0);
+          ptx::mma_f16_ss(s_at + (n & 1) * kTile, desc_k_major(low_k_major(q_smem), s), desc_k_major(low_k_major(k_smem + (n % NK) * TILE), s), id_s, s != 0);
         ptx::mma_commit(ptx::smem_u32(&sh->s_full[n & 1]));
       };
       auto grad = [&](int n) {         // dP(n) = dO V(n)
@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
         if (!ok) return;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
-          ptx::mma_f16_ss(dp_at, desc_k_major(do_smem, s), desc_k_major(v_smem + (n % NV) * TILE, s), id_s, s != 0);
+          ptx::mma_f16_ss(dp_at, desc_k_major(low_k_major(do_smem), s), desc_k_major(low_k_major(v_smem + (n % NV) * TILE), s), id_s, s != 0);
         ptx::mma_commit(ptx::smem_u32(&sh->dp_full));
         ptx::mma_commit(ptx::smem_u32(&sh->v_empty[n % NV]));
       };
@@ -729,7 +729,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
         if (!ok) break;
 #pragma unroll
         for (int s = 0; s < kTile / 16; ++s)
-          ptx::mma_f16_ts(dq_at, dp_at + packed_at(s), desc_mn_major(k_smem + (n % NK) * TILE, s), id_d, (n | s) != 0);
+          ptx::mma_f16_ts(dq_at, dp_at + packed_at(s), desc_mn_major(low_mn_major(k_smem + (n % NK) * TILE), s), id_d, (n | s) != 0);
         ptx::mma_commit(ptx::smem_u32(&sh->k_empty[n % NK]));
         grad(n + 1);
         if (ok) score(n + 2);

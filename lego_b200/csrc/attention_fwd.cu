@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
             wait(&sh->p_full[t], done[t] & 1, 0x430000u | t);
             if (!ok) break;
             ptx::tc_fence_after();
-            const uint32_t v_tile = kv_smem + (nv % NS) * TILE;
+            const uint32_t v_tile = low_mn_major(kv_smem + (nv % NS) * TILE);
 #pragma unroll
             for (int s = 0; s < kTile / 16; ++s)
               ptx::mma_f16_ts(o_tmem, s_tmem + s * 8, desc_mn_major(v_tile, s), id_o, (done[t] | s) != 0);
@@ -218,10 +218,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
               have_q[t] = true;
               ptx::tc_fence_after();
             }
-            const uint32_t k_tile = kv_smem + (nk % NS) * TILE;
+            const uint32_t k_tile = low_k_major(kv_smem + (nk % NS) * TILE), q_tile = low_k_major(q_smem + t * TILE);
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s)
-              ptx::mma_f16_ss(s_tmem, desc_k_major(q_smem + t * TILE, s), desc_k_major(k_tile, s), id_s, s != 0);
+              ptx::mma_f16_ss(s_tmem, desc_k_major(q_tile, s), desc_k_major(k_tile, s), id_s, s != 0);
             ptx::mma_commit(ptx::smem_u32(&sh->s_full[t]));
           }
         }

@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
               ptx::fence_proxy_async();      // so did these keys
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s)
-              ptx::mma_f16_ss(tmem + (i & 1) * kTile, desc_k_major(q_tile, s), desc_k_major(kv_smem + slot * TILE, s), id_s, s != 0);
+              ptx::mma_f16_ss(tmem + (i & 1) * kTile, desc_k_major(low_k_major(q_tile), s), desc_k_major(low_k_major(kv_smem + slot * TILE), s), id_s, s != 0);
             ptx::mma_commit(ptx::smem_u32(&sh->s_full[i & 1]));
             ptx::mma_commit(ptx::smem_u32(&sh->empty[slot]));
             if (i == count - 1) ptx::mma_commit(ptx::smem_u32(&sh->q_empty[n & 1]));
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             ++weighed[t];
 #pragma unroll
             for (int s = 0; s < kTile / 16; ++s)
-              ptx::mma_f16_ts(tmem + 2 * kTile + t * DP, tmem + t * kTile + s * 8, desc_mn_major(kv_smem + slot * TILE, s), id_o,
+              ptx::mma_f16_ts(tmem + 2 * kTile + t * DP, tmem + t * kTile + s * 8, desc_mn_major(low_mn_major(kv_smem + slot * TILE), s), id_o,
                               i > 2 || s != 0);
             ptx::mma_commit(ptx::smem_u32(&sh->empty[slot]));
             if (i >= count - 1) ptx::mma_commit(ptx::smem_u32(&sh->o_full[t]));
