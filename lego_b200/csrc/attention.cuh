@@ -75,6 +75,47 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// 2^z for z < 128 on the FMA pipe: z = n + r with |r| <= 1/2, a polynomial of degree 5 for 2^r
+// (fitted for the least relative error with p(0) = 1: 9.2e-8, 1.9e-7 in 32 bits), n added to the
+// exponent.  Zero from 2^-127 down, -inf among them.  An SM takes 16 ex2 per cycle, 1024 cycles
+// for a tile of scores, and the issue slots are idle meanwhile: some of the weights go this way.
+__device__ __forceinline__ float2 ex2_fma(float2 z) {
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(z.x));      // -127; a NaN stays one
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(z.y));
+  const float2 big = make_float2(12582912.f, 12582912.f);   // 1.5 2^23: rounds to an integer in the low bits
+  const float2 t = ptx::add2(z, big);
+  const float2 n = ptx::add2(t, make_float2(-12582912.f, -12582912.f));
+  const float2 r = ptx::fma2(n, make_float2(-1.f, -1.f), z);
+  float2 p = make_float2(1.326472848e-03f, 1.326472848e-03f);
+  p = ptx::fma2(p, r, make_float2(9.671512991e-03f, 9.671512991e-03f));
+  p = ptx::fma2(p, r, make_float2(5.550733581e-02f, 5.550733581e-02f));
+  p = ptx::fma2(p, r, make_float2(2.402224243e-01f, 2.402224243e-01f));
+  p = ptx::fma2(p, r, make_float2(6.931470037e-01f, 6.931470037e-01f));
+  p = ptx::fma2(p, r, make_float2(1.f, 1.f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+// tanh(u) for |u| <= 1: an odd polynomial of degree 13, off by 2e-8 (1e-7 in 32 bits).  Scores under
+// a cap rarely reach it, and the exact way below takes two of the 16 per cycle.
+__device__ __forceinline__ float2 tanh_near(float2 u) {
+  const float2 w = ptx::mul2(u, u);
+  float2 p = make_float2(9.637710173e-04f, 9.637710173e-04f);
+  p = ptx::fma2(p, w, make_float2(-5.951276980e-03f, -5.951276980e-03f));
+  p = ptx::fma2(p, w, make_float2(1.997327805e-02f, 1.997327805e-02f));
+  p = ptx::fma2(p, w, make_float2(-5.326583236e-02f, -5.326583236e-02f));
+  p = ptx::fma2(p, w, make_float2(1.331958324e-01f, 1.331958324e-01f));
+  p = ptx::fma2(p, w, make_float2(-3.333213031e-01f, -3.333213031e-01f));
+  p = ptx::fma2(p, w, make_float2(9.999997020e-01f, 9.999997020e-01f));
+  return ptx::mul2(p, u);
+}
+// Whether tanh_near does for all scores of the warp's rows.
+template <int N>
+__device__ __forceinline__ bool all_near(const float (&s)[N], float to_u) {
+  float top[2] = {fabsf(s[0]), fabsf(s[1])};
+#pragma unroll
+  for (int c = 2; c < N; ++c) top[c & 1] = fmaxf(top[c & 1], fabsf(s[c]));
+  return __all_sync(~0u, fmaxf(top[0], top[1]) * fabsf(to_u) <= 1.f);
+}
 // tanh(u), given 2 log2(e) u: 1 - 2 / (1 + e^2u), off by a few 2^-24 absolutely.
 __device__ __forceinline__ float tanh_of(float twice_log2e_u) { return fmaf(-2.f, rcp(1.f + ex2(twice_log2e_u)), 1.f); }
 
@@ -169,6 +210,8 @@ __device__ __forceinline__ void copy_tile_clean(uint8_t* tile, const uint16_t* b
 // log2 of the growth a row's reference value may lag behind its maximum: weights stay below
 // 2^8, their sum is kept in 32 bits, and O in TMEM is rarely rescaled.
 constexpr float kRescale = 8.f;
+// One pair of weights in so many goes to the FMA pipe.
+constexpr int kFmaEvery = 3;
 
 // A row's reference value m for a tile whose maximum is mt (log2 units).  Not the first tile:
 // where some row of the warp outgrew its reference value, its sums, in two registers and over DP
@@ -195,41 +238,94 @@ __device__ __forceinline__ void follow_maximum(float mt, bool first, float* m, f
   }
 }
 
+// Raw scores to log2 units: z = cap tanh(scale s / cap) - slope distance, times log2(e).  first:
+// position minus that of the first key.
+struct Scores {
+  float by;              // scale log2(e)
+  float to_u, cap_by;    // scale / cap, cap log2(e)
+  float slope;           // slope log2(e)
+};
+template <bool CAP>
+__device__ __forceinline__ Scores scores_of(float scale, float softcap, const float* slopes, int h) {
+  Scores s;
+  s.by = scale * kLog2e;
+  s.to_u = CAP ? scale / softcap : 0.f;
+  s.cap_by = softcap * kLog2e;
+  s.slope = slopes ? slopes[h] * kLog2e : 0.f;
+  return s;
+}
+template <int N, bool CAP, bool BIAS>
+__device__ __forceinline__ void score(float (&s)[N], const Scores& sc, int first) {
+  if (CAP) {
+    if (all_near(s, sc.to_u)) {
+#pragma unroll
+      for (int c = 0; c < N; c += 2) {
+        const float2 z = ptx::mul2(tanh_near(ptx::mul2(make_float2(s[c], s[c + 1]), make_float2(sc.to_u, sc.to_u))),
+                                   make_float2(sc.cap_by, sc.cap_by));
+        s[c] = z.x;
+        s[c + 1] = z.y;
+      }
+    } else {
+      const float by = 2.f * kLog2e * sc.to_u;
+#pragma unroll
+      for (int c = 0; c < N; ++c) s[c] = sc.cap_by * tanh_of(s[c] * by);
+    }
+  }
+  if (BIAS) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) s[c] = fmaf(-sc.slope, fabsf((float)(first - c)), CAP ? s[c] : s[c] * sc.by);
+  }
+}
+
 // One thread per row: the row's 128 scores s (hidden ones -inf) become weights
 // 2^(s by - m) (SCALED: s is in log2 units already), packed to 16 bits over columns 0 .. 63 of
-// s_tmem.  `sum` takes the weights as they are, for the row's logarithm; `packed_sum` as they
-// were rounded: divided by it, the result's weights add up to one, so an error all of them
-// share, above all that of a row's one large weight, falls out.  by > 0.
+// s_tmem; ready[i] gets the warp's arrival when 64 of them are in place.  `sum` takes the weights as
+// they are, for the row's logarithm; with BOTH `packed_sum` takes them as they were rounded:
+// divided by it, the result's weights add up to one, so an error all of them share, above all
+// that of a row's one large weight, falls out.  by > 0.
+template <bool BF16, bool SCALED, bool BOTH>
+__device__ __forceinline__ void weigh(const float (&s)[kTile], float by, float m, float* sum, float* packed_sum,
+                                      uint32_t s_tmem, uint64_t* ready, int lane) {
+  const float mu = m == -INFINITY ? 0.f : m;
+  float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, packed_add[2] = {add[0], add[0]};
+  const float2 by2 = make_float2(by, by), mu2 = make_float2(-mu, -mu);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int c = half * 64; c < half * 64 + 64; c += 32) {
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        float2 z = make_float2(s[c + i], s[c + i + 1]);
+        z = SCALED ? ptx::add2(z, mu2) : ptx::fma2(z, by2, mu2);
+        const float2 x = (i >> 1) % kFmaEvery == 1 ? ex2_fma(z) : make_float2(ex2(z.x), ex2(z.y));
+        const int k = (i >> 1) & 1;
+        add[k] = ptx::add2(add[k], x);
+        w[i >> 1] = pack2<BF16>(x.x, x.y);
+        if (BOTH) packed_add[k] = ptx::add2(packed_add[k], unpack2<BF16>(w[i >> 1]));
+      }
+      ptx::tmem_st_32x16(s_tmem + c / 2, w);
+    }
+    ptx::tmem_st_wait();
+    ptx::tc_fence_before();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ready[half]));
+  }
+  *sum += (add[0].x + add[0].y) + (add[1].x + add[1].y);
+  if (BOTH) *packed_sum += (packed_add[0].x + packed_add[0].y) + (packed_add[1].x + packed_add[1].y);
+}
 template <int DP, bool BF16, bool SCALED>
 __device__ __forceinline__ void weigh_tile(const float (&s)[kTile], float by, bool first, float* m, float* sum,
-                                           float* packed_sum, uint32_t s_tmem, uint32_t o_tmem) {
+                                           float* packed_sum, bool both, uint32_t s_tmem, uint32_t o_tmem,
+                                           uint64_t* ready, int lane) {
   float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
   for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
   float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   if (!SCALED) mt *= by;
   follow_maximum<DP>(mt, first, m, sum, packed_sum, o_tmem);
-  const float mu = *m == -INFINITY ? 0.f : *m;
-  float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, packed_add[2] = {add[0], add[0]};
-  const float2 by2 = make_float2(by, by), mu2 = make_float2(-mu, -mu);
-#pragma unroll
-  for (int c = 0; c < kTile; c += 32) {
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      float2 z = make_float2(s[c + i], s[c + i + 1]);
-      z = SCALED ? ptx::add2(z, mu2) : ptx::fma2(z, by2, mu2);
-      const float2 x = make_float2(ex2(z.x), ex2(z.y));
-      const int k = (i >> 1) & 1;
-      add[k] = ptx::add2(add[k], x);
-      w[i >> 1] = pack2<BF16>(x.x, x.y);
-      packed_add[k] = ptx::add2(packed_add[k], unpack2<BF16>(w[i >> 1]));
-    }
-    ptx::tmem_st_32x16(s_tmem + c / 2, w);
-  }
-  *sum += (add[0].x + add[0].y) + (add[1].x + add[1].y);
-  *packed_sum += (packed_add[0].x + packed_add[0].y) + (packed_add[1].x + packed_add[1].y);
-  ptx::tmem_st_wait();
+  if (both) weigh<BF16, SCALED, true>(s, by, *m, sum, packed_sum, s_tmem, ready, lane);
+  else weigh<BF16, SCALED, false>(s, by, *m, sum, packed_sum, s_tmem, ready, lane);
 }
 
 __device__ __forceinline__ void attn_fail(uint32_t* status, volatile uint32_t* abort_flag, uint32_t code) {

@@ -24,6 +24,8 @@
 // both are taken out of the 32-bit sums at the end.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "attention.cuh"
 #include "tma_host.cuh"
 
@@ -130,27 +132,16 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __grid_constan
 
 // ---- shared by the two product kernels ---------------------------------------------------------
 
-struct Scores {      // log2 units, as in the forward pass
-  float by, u_by, cap_by, slope;
-};
-template <bool CAP>
-__device__ __forceinline__ Scores scores_of(const AttnProblem& p, int h) {
-  Scores s;
-  s.by = p.scale * kLog2e;
-  s.u_by = CAP ? 2.f * kLog2e * p.scale / p.softcap : 0.f;
-  s.cap_by = p.softcap * kLog2e;
-  s.slope = p.slopes ? p.slopes[h] * kLog2e : 0.f;
-  return s;
-}
-
 // A pair of raw scores -> weights x = 2^(z + nl) and what the score gradient is multiplied by,
-// w = x (1 - tanh^2).  far: distances.
-template <bool CAP, bool BIAS>
+// w = x (1 - tanh^2).  far: distances; NEAR: tanh_near does.
+template <bool CAP, bool BIAS, bool NEAR>
 __device__ __forceinline__ void weights(float2 s, float2 nl, const Scores& sc, float2 far, float2* x, float2* w) {
   float2 z;
   float2 bend = make_float2(1.f, 1.f);
   if (CAP) {
-    const float2 t = make_float2(tanh_of(s.x * sc.u_by), tanh_of(s.y * sc.u_by));
+    const float by = 2.f * kLog2e * sc.to_u;
+    const float2 t = NEAR ? tanh_near(ptx::mul2(s, make_float2(sc.to_u, sc.to_u)))
+                          : make_float2(tanh_of(s.x * by), tanh_of(s.y * by));
     z = ptx::fma2(t, make_float2(sc.cap_by, sc.cap_by), nl);
     bend = ptx::fma2(make_float2(-t.x, -t.y), t, bend);
   } else {
@@ -226,7 +217,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
   const uint32_t k_smem = ptx::smem_u32(smem), v_smem = k_smem + TILE, q_smem = v_smem + TILE, do_smem = q_smem + NS * TILE;
   const AttnProblem& p = a.p;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int heads = p.batch * p.k_heads;
   const int kt = (int)(blockIdx.x / heads);      // the first keys, which most queries see, come first
   const int b = blockIdx.x % heads / p.k_heads, hk = blockIdx.x % heads % p.k_heads;
@@ -286,9 +277,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = sh->tmem_base;
+  const uint32_t tmem = ptx::uniform(sh->tmem_base);
   const uint32_t s_at = tmem, dp_at = tmem + kTile, dv_at = tmem + 2 * kTile, dk_at = dv_at + DP;
-  const int lo = sh->lo, per_head = sh->hi - lo, steps = per_head * p.group;
+  const int lo = ptx::uniform(sh->lo), per_head = ptx::uniform(sh->hi) - lo, steps = per_head * p.group;
 
   if (warp >= 8) {
     ptx::regs_less<kBwdOtherRegs>();
@@ -352,26 +343,27 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
             ptx::mbar_wait_bounded(ptx::smem_u32(&sh->do_full[s]), ((n - 1 - s) / NS) & 1, &never, kAttnWait);
           }
       }
-    } else if (warp == 9 && lane == 0 && steps > 0) {
+    } else if (warp == 9 && steps > 0) {
       // ---------------- MMA issue ----------------
+      const uint32_t leader = ptx::elect_one();
       const uint32_t id_s = idesc_of<BF16>(kTile, false), id_d = idesc_of<BF16>(DP, true);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
-        if (ok && !ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait)) {
-          attn_fail(a.status, abort_flag, code);
+        if (ok && !__all_sync(~0u, ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait))) {
+          if (leader) attn_fail(a.status, abort_flag, code);
           ok = false;
         }
         ptx::tc_fence_after();
       };
       auto score_product = [&](uint32_t d, uint32_t own, uint32_t other, uint64_t* bar) {
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) ptx::mma_f16_ss(d, desc_k_major(low_k_major(own), s), desc_k_major(low_k_major(other), s), id_s, s != 0);
-        ptx::mma_commit(ptx::smem_u32(bar));
+        for (int s = 0; s < DP / 16; ++s) ptx::mma_f16_ss_by(leader, d, desc_k_major(low_k_major(own), s), desc_k_major(low_k_major(other), s), id_s, s != 0);
+        ptx::mma_commit_by(leader, ptx::smem_u32(bar));
       };
       auto sum_product = [&](uint32_t d, uint32_t w, uint32_t other, bool add, uint64_t* bar) {
 #pragma unroll
-        for (int s = 0; s < kTile / 16; ++s) ptx::mma_f16_ts(d, w + packed_at(s), desc_mn_major(low_mn_major(other), s), id_d, add || s != 0);
-        ptx::mma_commit(ptx::smem_u32(bar));
+        for (int s = 0; s < kTile / 16; ++s) ptx::mma_f16_ts_by(leader, d, w + packed_at(s), desc_mn_major(low_mn_major(other), s), id_d, add || s != 0);
+        ptx::mma_commit_by(leader, ptx::smem_u32(bar));
       };
       wait(&sh->kv_full[0], 0, 0x520000u);
       wait(&sh->q_full[0], 0, 0x520001u);
@@ -399,7 +391,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
           score_product(dp_at, v_smem, do_smem + next * TILE, &sh->dp_full);
         }
       }
-      if (ok) ptx::mma_commit(ptx::smem_u32(&sh->acc_full));
+      if (ok) ptx::mma_commit_by(leader, ptx::smem_u32(&sh->acc_full));
     }
   } else {
     ptx::regs_more<kMathRegs>();
@@ -434,7 +426,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
     for (int n = 0; n < steps; ++n) {
       const int h = hk * p.group + n / per_head, i0 = (lo + n % per_head) * kTile;
       const uint32_t slot = n % NS;
-      const Scores sc = scores_of<CAP>(p, h);
+      const Scores sc = scores_of<CAP>(p.scale, p.softcap, p.slopes, h);
       // seen whole: the first query sees the last key (queries past the end have weight zero)
       bool masked = p.causal && last_key(p, prefix, i0 + p.offset) < j0 + kTile - 1;
       if (qd) masked = masked || !docs_same(qd[lo + n % per_head], tile_docs);
@@ -463,6 +455,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
           mask_documents(see, other, own_doc);
         }
       }
+      auto weigh = [&](auto near_tag) {
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         uint32_t packed[16];
@@ -479,7 +472,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
           for (int x = 0; x < 2; ++x) {
             const int at = c + e + 2 * x;
             float2 px, pw;
-            weights<CAP, BIAS>(make_float2(w[at], w[at + 1]), x ? make_float2(nl.z, nl.w) : make_float2(nl.x, nl.y), sc,
+            weights<CAP, BIAS, decltype(near_tag)::value>(make_float2(w[at], w[at + 1]), x ? make_float2(nl.z, nl.w) : make_float2(nl.x, nl.y), sc,
                                far[x], &px, &pw);
             if (masked) {
               if (!((see[at >> 5] >> (at & 31)) & 1u)) px.x = pw.x = 0.f;
@@ -492,6 +485,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
         }
         ptx::tmem_st_32x16(s_tmem + c / 2, packed);
       }
+      };
+      if (CAP && all_near(w, sc.to_u)) weigh(std::true_type{});
+      else weigh(std::false_type{});
       ptx::tmem_st_wait();
       ptx::tc_fence_before();
       __syncwarp();
@@ -577,7 +573,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
   const uint32_t q_smem = ptx::smem_u32(smem), do_smem = q_smem + TILE, k_smem = do_smem + TILE, v_smem = k_smem + NK * TILE;
   const AttnProblem& p = a.p;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int heads = p.batch * p.q_heads;
   const int qt = tiles_of(p.q_len) - 1 - (int)(blockIdx.x / heads);
   const int b = blockIdx.x % heads / p.q_heads, h = blockIdx.x % heads % p.q_heads, hk = h / p.group;
@@ -637,9 +633,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = sh->tmem_base;
+  const uint32_t tmem = ptx::uniform(sh->tmem_base);
   const uint32_t s_at = tmem, dp_at = tmem + 2 * kTile, dq_at = tmem + 3 * kTile;
-  const int lo = sh->lo, steps = sh->hi - lo;
+  const int lo = ptx::uniform(sh->lo), steps = ptx::uniform(sh->hi) - lo;
 
   if (warp >= 8) {
     ptx::regs_less<kBwdOtherRegs>();
@@ -689,13 +685,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
         for (int s = 0; s < NV; ++s)
           if (n > s) ptx::mbar_wait_bounded(ptx::smem_u32(&sh->v_full[s]), ((n - 1 - s) / NV) & 1, &never, kAttnWait);
       }
-    } else if (warp == 9 && lane == 0 && steps > 0) {
+    } else if (warp == 9 && steps > 0) {
       // ---------------- MMA issue ----------------
+      const uint32_t leader = ptx::elect_one();
       const uint32_t id_s = idesc_of<BF16>(kTile, false), id_d = idesc_of<BF16>(DP, true);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
-        if (ok && !ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait)) {
-          attn_fail(a.status, abort_flag, code);
+        if (ok && !__all_sync(~0u, ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait))) {
+          if (leader) attn_fail(a.status, abort_flag, code);
           ok = false;
         }
         ptx::tc_fence_after();
@@ -706,8 +703,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
         if (!ok) return;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
-          ptx::mma_f16_ss(s_at + (n & 1) * kTile, desc_k_major(low_k_major(q_smem), s), desc_k_major(low_k_major(k_smem + (n % NK) * TILE), s), id_s, s != 0);
-        ptx::mma_commit(ptx::smem_u32(&sh->s_full[n & 1]));
+          ptx::mma_f16_ss_by(leader, s_at + (n & 1) * kTile, desc_k_major(low_k_major(q_smem), s), desc_k_major(low_k_major(k_smem + (n % NK) * TILE), s), id_s, s != 0);
+        ptx::mma_commit_by(leader, ptx::smem_u32(&sh->s_full[n & 1]));
       };
       auto grad = [&](int n) {         // dP(n) = dO V(n)
         if (n >= steps) return;
@@ -715,9 +712,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
         if (!ok) return;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
-          ptx::mma_f16_ss(dp_at, desc_k_major(low_k_major(do_smem), s), desc_k_major(low_k_major(v_smem + (n % NV) * TILE), s), id_s, s != 0);
-        ptx::mma_commit(ptx::smem_u32(&sh->dp_full));
-        ptx::mma_commit(ptx::smem_u32(&sh->v_empty[n % NV]));
+          ptx::mma_f16_ss_by(leader, dp_at, desc_k_major(low_k_major(do_smem), s), desc_k_major(low_k_major(v_smem + (n % NV) * TILE), s), id_s, s != 0);
+        ptx::mma_commit_by(leader, ptx::smem_u32(&sh->dp_full));
+        ptx::mma_commit_by(leader, ptx::smem_u32(&sh->v_empty[n % NV]));
       };
       wait(&sh->q_full[0], 0, 0x620002u);
       if (ok) score(0);
@@ -729,12 +726,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
         if (!ok) break;
 #pragma unroll
         for (int s = 0; s < kTile / 16; ++s)
-          ptx::mma_f16_ts(dq_at, dp_at + packed_at(s), desc_mn_major(low_mn_major(k_smem + (n % NK) * TILE), s), id_d, (n | s) != 0);
-        ptx::mma_commit(ptx::smem_u32(&sh->k_empty[n % NK]));
+          ptx::mma_f16_ts_by(leader, dq_at, dp_at + packed_at(s), desc_mn_major(low_mn_major(k_smem + (n % NK) * TILE), s), id_d, (n | s) != 0);
+        ptx::mma_commit_by(leader, ptx::smem_u32(&sh->k_empty[n % NK]));
         grad(n + 1);
         if (ok) score(n + 2);
       }
-      if (ok) ptx::mma_commit(ptx::smem_u32(&sh->acc_full));
+      if (ok) ptx::mma_commit_by(leader, ptx::smem_u32(&sh->acc_full));
     }
   } else {
     ptx::regs_more<kMathRegs>();
@@ -744,7 +741,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
     const uint32_t dp_tmem = dp_at + lanes + half * 64;
     const int row = q0 + quarter * 32 + lane, pos = row + p.offset;
     const int last = last_key(p, prefix, pos), last_first = last_key(p, prefix, q0 + p.offset);
-    const Scores sc = scores_of<CAP>(p, h);
+    const Scores sc = scores_of<CAP>(p.scale, p.softcap, p.slopes, h);
     const float ds_factor = BF16 ? 1.f : score_factor(a, b, hk);
     const float w_by = BF16 ? 1.f : ldexpf(ds_factor, -kWeightShift);
     const long long slot = row_slot(p, b, h) + row;
@@ -778,6 +775,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
 #pragma unroll
       for (int c = 0; c < 64; c += 32) ptx::tmem_ld_32x32(s_tmem + c, reinterpret_cast<uint32_t*>(w) + c);
       ptx::tmem_ld_wait();
+      auto weigh = [&](auto near_tag) {
 #pragma unroll
       for (int c = 0; c < 64; c += 2) {
         float2 far, px, pw;
@@ -785,11 +783,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
           const float d = (float)(pos - j0 - half * 64 - c);
           far = make_float2(fabsf(d), fabsf(d - 1.f));
         }
-        weights<CAP, BIAS>(make_float2(w[c], w[c + 1]), nl2, sc, far, &px, &pw);
+        weights<CAP, BIAS, decltype(near_tag)::value>(make_float2(w[c], w[c + 1]), nl2, sc, far, &px, &pw);
         if (!BF16) pw = ptx::mul2(pw, make_float2(w_by, w_by));
         w[c] = pw.x;
         w[c + 1] = pw.y;
       }
+      };
+      if (CAP && all_near(w, sc.to_u)) weigh(std::true_type{});
+      else weigh(std::false_type{});
       uint32_t see[2] = {~0u, ~0u};
       if (masked) {
         see[0] = bits_upto(last - j0 - half * 64, 0);

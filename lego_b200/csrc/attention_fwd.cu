@@ -37,7 +37,7 @@ template <int DP> constexpr int fwd_smem() { return (2 + fwd_stages<DP>()) * til
 
 struct FwdArgs {
   CUtensorMap q, k, v, o, o_low;
-  int low;              // o_low is wanted
+  bool low;             // o_low is wanted
   AttnProblem p;
   const uint16_t* v_raw;
   float* lse;
@@ -46,7 +46,7 @@ struct FwdArgs {
 };
 
 struct FwdShared {
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2];      // p_full: by halves of the keys
   uint64_t kv_full[8], kv_empty[8];
   int lo[2], hi[2];     // tiles of keys that row tile t sees
   uint32_t tmem_base, abort_flag;
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
   const uint32_t q_smem = ptx::smem_u32(smem), kv_smem = q_smem + 2 * TILE;
   const AttnProblem& p = a.p;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // the last queries, which see the most keys of a causal mask, come first
   const int heads = p.batch * p.q_heads;
   const int qt = a.q_tiles - 1 - (int)(blockIdx.x / heads);
@@ -73,7 +73,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(ptx::smem_u32(&sh->q_full[t]), 1);
       ptx::mbar_init(ptx::smem_u32(&sh->s_full[t]), 1);
-      ptx::mbar_init(ptx::smem_u32(&sh->p_full[t]), 4);
+      ptx::mbar_init(ptx::smem_u32(&sh->p_full[t][0]), 4);
+      ptx::mbar_init(ptx::smem_u32(&sh->p_full[t][1]), 4);
       ptx::mbar_init(ptx::smem_u32(&sh->o_full[t]), 1);
     }
     for (int s = 0; s < NS; ++s) {
@@ -122,8 +123,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = sh->tmem_base;
-  const int lo0 = sh->lo[0], hi0 = sh->hi[0], lo1 = sh->lo[1], hi1 = sh->hi[1];
+  const uint32_t tmem = ptx::uniform(sh->tmem_base);
+  const int lo0 = ptx::uniform(sh->lo[0]), hi0 = ptx::uniform(sh->hi[0]);
+  const int lo1 = ptx::uniform(sh->lo[1]), hi1 = ptx::uniform(sh->hi[1]);
   const bool any0 = lo0 < hi0, any1 = lo1 < hi1;
   const int lo = !any0 ? lo1 : !any1 ? lo0 : lo0 < lo1 ? lo0 : lo1;
   const int hi = !any0 ? hi1 : !any1 ? hi0 : hi0 > hi1 ? hi0 : hi1;
@@ -180,36 +182,41 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
     }
   } else if (warp == 9) {
     // ---------------- MMA issue ----------------
-    if (lane == 0) {
+    {
+      const uint32_t leader = ptx::elect_one();
       const uint32_t id_s = idesc_of<BF16>(kTile, false), id_o = idesc_of<BF16>(DP, true);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
-        if (ok && !ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait)) {
-          attn_fail(a.status, abort_flag, code);
+        if (ok && !__all_sync(~0u, ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait))) {
+          if (leader) attn_fail(a.status, abort_flag, code);
           ok = false;
         }
       };
-      uint32_t done[2] = {0, 0};     // weight tiles multiplied so far
+      uint32_t slot = 0, phase = 0, v_slot = 0, v_phase = 0;     // ring: the next tile's, V's of the step before
       bool have_q[2] = {false, false};
       for (int j = lo; ok && j <= hi && lo < hi; ++j) {
-        const uint32_t nk = 2 * (j - lo), nv = nk - 1;   // ring positions of K(j), V(j - 1)
-        if (j < hi) wait(&sh->kv_full[nk % NS], (nk / NS) & 1, 0x420000u);
-        if (j > lo) wait(&sh->kv_full[nv % NS], (nv / NS) & 1, 0x420001u);
+        const uint32_t k_slot = slot;
+        if (j < hi) wait(&sh->kv_full[slot], phase, 0x420000u);
+        if (j > lo) wait(&sh->kv_full[v_slot], v_phase, 0x420001u);
+        if (!ok) break;
         ptx::tc_fence_after();
+        const uint32_t v_tile = low_mn_major(kv_smem + v_slot * TILE), k_tile = low_k_major(kv_smem + k_slot * TILE);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int l = t ? lo1 : lo0, e = t ? hi1 : hi0;
           const uint32_t s_tmem = tmem + t * kTile, o_tmem = tmem + 2 * kTile + t * DP;
           if (j - 1 >= l && j - 1 < e) {     // O += P V(j - 1)
-            wait(&sh->p_full[t], done[t] & 1, 0x430000u | t);
-            if (!ok) break;
-            ptx::tc_fence_after();
-            const uint32_t v_tile = low_mn_major(kv_smem + (nv % NS) * TILE);
 #pragma unroll
-            for (int s = 0; s < kTile / 16; ++s)
-              ptx::mma_f16_ts(o_tmem, s_tmem + s * 8, desc_mn_major(v_tile, s), id_o, (done[t] | s) != 0);
-            ++done[t];
-            if (j == e) ptx::mma_commit(ptx::smem_u32(&sh->o_full[t]));
+            for (int half = 0; half < 2; ++half) {
+              wait(&sh->p_full[t][half], (j - 1 - l) & 1, 0x430000u | t);
+              if (!ok) break;
+              ptx::tc_fence_after();
+#pragma unroll
+              for (int s = half * 4; s < half * 4 + 4; ++s)
+                ptx::mma_f16_ts_by(leader, o_tmem, s_tmem + s * 8, desc_mn_major(v_tile, s), id_o, j - 1 != l || s != 0);
+            }
+            if (!ok) break;
+            if (j == e) ptx::mma_commit_by(leader, ptx::smem_u32(&sh->o_full[t]));
           }
           if (j >= l && j < e) {             // S = Q K(j)
             if (!have_q[t]) {
@@ -218,16 +225,21 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
               have_q[t] = true;
               ptx::tc_fence_after();
             }
-            const uint32_t k_tile = low_k_major(kv_smem + (nk % NS) * TILE), q_tile = low_k_major(q_smem + t * TILE);
+            const uint32_t q_tile = low_k_major(q_smem + t * TILE);
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s)
-              ptx::mma_f16_ss(s_tmem, desc_k_major(q_tile, s), desc_k_major(k_tile, s), id_s, s != 0);
-            ptx::mma_commit(ptx::smem_u32(&sh->s_full[t]));
+              ptx::mma_f16_ss_by(leader, s_tmem, desc_k_major(q_tile, s), desc_k_major(k_tile, s), id_s, s != 0);
+            ptx::mma_commit_by(leader, ptx::smem_u32(&sh->s_full[t]));
           }
         }
         if (!ok) break;
-        if (j > lo) ptx::mma_commit(ptx::smem_u32(&sh->kv_empty[nv % NS]));
-        if (j < hi) ptx::mma_commit(ptx::smem_u32(&sh->kv_empty[nk % NS]));
+        if (j > lo) ptx::mma_commit_by(leader, ptx::smem_u32(&sh->kv_empty[v_slot]));
+        if (j < hi) ptx::mma_commit_by(leader, ptx::smem_u32(&sh->kv_empty[k_slot]));
+        // K, V alternate in the ring
+        v_slot = slot + 1 == NS ? 0 : slot + 1;
+        v_phase = slot + 1 == NS ? phase ^ 1 : phase;
+        slot = v_slot + 1 == NS ? 0 : v_slot + 1;
+        phase = v_slot + 1 == NS ? v_phase ^ 1 : v_phase;
       }
     }
   }
@@ -252,10 +264,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
       if (row < p.q_len) own_doc = docs[pos];
       tile_docs = p.query_docs[(long long)b * tiles_of(p.q_len) + q0 / kTile];
     }
-    // log2 units: z = raw * by, or cap_by * tanh(raw * u_by / (2 log2 e)); minus slope * distance
-    const float by = p.scale * kLog2e;
-    const float u_by = CAP ? 2.f * kLog2e * p.scale / p.softcap : 0.f, cap_by = p.softcap * kLog2e;
-    const float slope = BIAS && p.slopes ? p.slopes[h] * kLog2e : 0.f;
+    const Scores sc = scores_of<CAP>(p.scale, p.softcap, p.slopes, h);
     float m = -INFINITY, sum = 0.f, packed_sum = 0.f;
     bool ok = true;
     for (int j = l; j < e; ++j) {
@@ -275,14 +284,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
 #pragma unroll
       for (int c = 0; c < kTile; c += 32) ptx::tmem_ld_32x32(s_tmem + c, reinterpret_cast<uint32_t*>(s) + c);
       ptx::tmem_ld_wait();
-      if (CAP || BIAS) {
-#pragma unroll
-        for (int c = 0; c < kTile; ++c) {
-          float z = CAP ? cap_by * tanh_of(s[c] * u_by) : s[c] * by;
-          if (BIAS) z = fmaf(-slope, fabsf((float)(pos - j0 - c)), z);
-          s[c] = z;
-        }
-      }
+      score<kTile, CAP, BIAS>(s, sc, pos - j0);
       if (masked) {
         uint32_t see[4];
 #pragma unroll
@@ -299,13 +301,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
 #pragma unroll
         for (int c = 0; c < kTile; ++c) s[c] = (see[c >> 5] >> (c & 31)) & 1u ? s[c] : -INFINITY;
       }
-      weigh_tile<DP, BF16, CAP || BIAS>(s, by, j == l, &m, &sum, &packed_sum, s_tmem, o_tmem);
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->p_full[t]));
+      weigh_tile<DP, BF16, CAP || BIAS>(s, sc.by, j == l, &m, &sum, &packed_sum, a.low, s_tmem, o_tmem, sh->p_full[t], lane);
     }
     // result
     const bool has = sum > 0.f || sum != sum;
+    if (!a.low) packed_sum = sum;
     const float inv = packed_sum > 0.f || sum != sum ? 1.f / packed_sum : 0.f;
     if (row < p.q_len && ok)
       a.lse[((long long)b * p.q_heads + h) * p.q_len + row] = has ? (m + log2f(sum)) * kLn2 : -INFINITY;
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
       }
       ptx::tc_fence_after();
     }
-    for (int low = 0; ok && low <= a.low && q0 + quarter * 32 < p.q_len; ++low) {   // the tile's own queries are no longer needed: stage there
+    for (int low = 0; ok && low <= (a.low ? 1 : 0) && q0 + quarter * 32 < p.q_len; ++low) {   // the tile's own queries are no longer needed: stage there
 #pragma unroll
       for (int c = 0; c < DP; c += 32) {
         uint32_t o[32];

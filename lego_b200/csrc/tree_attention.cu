@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
   TreeShared* sh = reinterpret_cast<TreeShared*>(smem + (2 + NS) * TILE);
   volatile uint32_t* abort_flag = &sh->abort_flag;
   const uint32_t q_smem = ptx::smem_u32(smem), kv_smem = q_smem + 2 * TILE;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
@@ -296,18 +296,19 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = sh->tmem_base;
+  const uint32_t tmem = ptx::uniform(sh->tmem_base);
   Piece pc;
 
   if (warp >= 12) {
     ptx::regs_less<kTreeOtherRegs>();
-    if (warp == 12 && lane == 0) {
+    if (warp == 12) {
       // ---------------- MMA issue ----------------
+      const uint32_t leader = ptx::elect_one();
       const uint32_t id_s = idesc_of<BF16>(kTile, false), id_o = idesc_of<BF16>(DP, true);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
-        if (ok && !ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait)) {
-          attn_fail(p.status, abort_flag, code);
+        if (ok && !__all_sync(~0u, ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait))) {
+          if (leader) attn_fail(p.status, abort_flag, code);
           ok = false;
         }
         ptx::tc_fence_after();
@@ -334,10 +335,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
               ptx::fence_proxy_async();      // so did these keys
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s)
-              ptx::mma_f16_ss(tmem + (i & 1) * kTile, desc_k_major(low_k_major(q_tile), s), desc_k_major(low_k_major(kv_smem + slot * TILE), s), id_s, s != 0);
-            ptx::mma_commit(ptx::smem_u32(&sh->s_full[i & 1]));
-            ptx::mma_commit(ptx::smem_u32(&sh->empty[slot]));
-            if (i == count - 1) ptx::mma_commit(ptx::smem_u32(&sh->q_empty[n & 1]));
+              ptx::mma_f16_ss_by(leader, tmem + (i & 1) * kTile, desc_k_major(low_k_major(q_tile), s), desc_k_major(low_k_major(kv_smem + slot * TILE), s), id_s, s != 0);
+            ptx::mma_commit_by(leader, ptx::smem_u32(&sh->s_full[i & 1]));
+            ptx::mma_commit_by(leader, ptx::smem_u32(&sh->empty[slot]));
+            if (i == count - 1) ptx::mma_commit_by(leader, ptx::smem_u32(&sh->q_empty[n & 1]));
           }
           if (i > 0) {
             const uint32_t t = (i - 1) & 1, vpos = pos - 1, slot = vpos % NS;
@@ -348,10 +349,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             ++weighed[t];
 #pragma unroll
             for (int s = 0; s < kTile / 16; ++s)
-              ptx::mma_f16_ts(tmem + 2 * kTile + t * DP, tmem + t * kTile + s * 8, desc_mn_major(low_mn_major(kv_smem + slot * TILE), s), id_o,
+              ptx::mma_f16_ts_by(leader, tmem + 2 * kTile + t * DP, tmem + t * kTile + s * 8, desc_mn_major(low_mn_major(kv_smem + slot * TILE), s), id_o,
                               i > 2 || s != 0);
-            ptx::mma_commit(ptx::smem_u32(&sh->empty[slot]));
-            if (i >= count - 1) ptx::mma_commit(ptx::smem_u32(&sh->o_full[t]));
+            ptx::mma_commit_by(leader, ptx::smem_u32(&sh->empty[slot]));
+            if (i >= count - 1) ptx::mma_commit_by(leader, ptx::smem_u32(&sh->o_full[t]));
           }
         }
         pos -= 2;     // the last turn had no K
@@ -486,7 +487,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_tmem = tmem + lanes + t * kTile, o_tmem = tmem + lanes + 2 * kTile + t * DP;
     const float by = p.scale * kLog2e;
-    const float u_by = CAP ? 2.f * kLog2e * p.scale / p.softcap : 0.f, cap_by = p.softcap * kLog2e;
     const int per_copy = kTile / p.copies, chunks = 4 / p.copies;     // rows; chunks of 32 columns a copy weighs
     const int in_copy = (quarter * 32 + lane) & (per_copy - 1), copy = quarter * 32 / per_copy, chunk0 = copy * chunks;
     bool ok = true;
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
       const int len = pc.len;
       const unsigned long long seen = real ? tree->seen[tok] : 0;
       const int depth = tree->depth[tok];
-      const float slope = BIAS && p.slopes ? p.slopes[h] * kLog2e : 0.f;
+      const Scores sc = scores_of<CAP>(p.scale, p.softcap, p.slopes, h);
       float m = -INFINITY, sum = 0.f;
       for (int i = t; i < count; i += 2) {
         const int j0 = (pc.first + i) * kTile;
@@ -538,18 +538,19 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             }
             ptx::tmem_ld_wait();
             if (CAP || BIAS) {
+              // cached tokens: none is ahead.  (A place past 2^24 is rounded, its distance by as little.)
+              score<32, CAP, false>(s, sc, 0);
+              if (BIAS) {
 #pragma unroll
-              for (int c = 0; c < 32; ++c) {
-                float z = CAP ? cap_by * tanh_of(s[c] * u_by) : s[c] * by;
-                if (BIAS) z = fmaf(-slope, (float)(at - c) + (float)depth, z);     // cached tokens: none is ahead
-                s[c] = z;
+                for (int c = 0; c < 32; ++c)
+                  s[c] = fmaf(-sc.slope, (float)(at - c) + (float)depth, CAP ? s[c] : s[c] * by);
               }
               if (BIAS && at < 32) {     // drafted tokens stand where their depth says, not their place
 #pragma unroll
                 for (int c = 0; c < 32; ++c) {
                   const int d = c - at;
                   if (d >= 0 && d < p.drafted)
-                    s[c] = fmaf(-slope, fabsf((float)(depth - tree->depth[d])) - (float)(depth - d), s[c]);
+                    s[c] = fmaf(-sc.slope, fabsf((float)(depth - tree->depth[d])) - (float)(depth - d), s[c]);
                 }
               }
             }
