@@ -68,63 +68,89 @@ __device__ __forceinline__ void raise_peak(uint32_t* at, uint32_t bits) {
 
 // ---- preparation -----------------------------------------------------------------------------
 
-// A warp per row, four values a lane: delta, the negated log-sum, and in fp16 the peaks of dO
-// and V.  Rows past q_len (whole tiles) and padding get weight zero: -inf.  Memory bound; the
-// peaks are maxima, so the order of the atomics does not matter.
+// Per row delta and the negated log-sum, and in fp16 the peaks of dO and V.  Rows past q_len (whole
+// tiles) and padding get weight zero: -inf.  A warp takes 32 tokens of one head, a block the same
+// tokens of eight heads, which lie together in memory; four rows are under way at a time, and lane i
+// keeps token i's results so they leave as one line.  Memory bound.  The peaks are maxima, so the
+// order of the atomics, one per warp that raises a peak, does not matter.
+struct PrepGrid {
+  int q_chunks, q_blocks, k_blocks;     // of 32 tokens; of 8 heads x 32 tokens
+};
+__host__ __device__ inline PrepGrid prep_grid(const AttnProblem& p, bool peaks) {
+  PrepGrid g;
+  g.q_chunks = tiles_of(p.q_len) * 4;
+  g.q_blocks = p.batch * g.q_chunks * ((p.q_heads + 7) / 8);
+  g.k_blocks = peaks ? p.batch * ((p.k_len + 31) / 32) * ((p.k_heads + 7) / 8) : 0;
+  return g;
+}
 template <bool BF16>
 __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __grid_constant__ BwdArgs a) {
   const AttnProblem& p = a.p;
+  const PrepGrid g = prep_grid(p, !BF16);
   ptx::grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int padded = tiles_of(p.q_len) * kTile;
-  const long long rows = (long long)p.batch * padded * p.q_heads;
-  if (id < rows) {
-    const int h = (int)(id % p.q_heads), i = (int)(id / p.q_heads % padded), b = (int)(id / p.q_heads / padded);
-    float delta = 0.f, peak = 0.f, nl = -INFINITY;
-    const bool real = i < p.q_len &&
-                      (!p.documents || p.documents[(long long)b * p.k_len + p.offset + i] >= 0);
-    if (real) {
-      const long long at = (((long long)b * p.q_len + i) * p.q_heads + h) * p.dim;
-      if (lane * 4 < p.dim) {
-        const uint2 x = *reinterpret_cast<const uint2*>(a.o_raw + at + lane * 4);
-        const uint2 g = *reinterpret_cast<const uint2*>(a.do_raw + at + lane * 4);
-        float2 x0 = unpack2<BF16>(x.x), x1 = unpack2<BF16>(x.y);
-        const float2 g0 = unpack2<BF16>(g.x), g1 = unpack2<BF16>(g.y);
-        if (a.low_raw) {
-          const uint2 y = *reinterpret_cast<const uint2*>(a.low_raw + at + lane * 4);
-          x0 = ptx::add2(x0, unpack2<BF16>(y.x));
-          x1 = ptx::add2(x1, unpack2<BF16>(y.y));
-        }
-        delta = fmaf(x0.x, g0.x, fmaf(x0.y, g0.y, fmaf(x1.x, g1.x, x1.y * g1.y)));
-        peak = fmaxf(fmaxf(fabsf(g0.x), fabsf(g0.y)), fmaxf(fabsf(g1.x), fabsf(g1.y)));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool mine = lane * 4 < p.dim;
+  if ((int)blockIdx.x < g.q_blocks) {
+    const int groups = (p.q_heads + 7) / 8;
+    const int h = (int)(blockIdx.x % groups) * 8 + warp, chunk = (int)(blockIdx.x / groups) % g.q_chunks;
+    const int b = (int)(blockIdx.x / groups) / g.q_chunks;
+    if (h >= p.q_heads) return;
+    const int i0 = chunk * 32, own = i0 + lane;
+    const bool real = own < p.q_len && (!p.documents || p.documents[(long long)b * p.k_len + p.offset + own] >= 0);
+    const uint32_t rows = __ballot_sync(~0u, real);
+    float kept = 0.f, peak = 0.f;
+    const long long stride = (long long)p.q_heads * p.dim;
+    const long long at0 = ((long long)b * p.q_len + i0) * stride + (long long)h * p.dim + lane * 4;
+    for (int r = 0; r < 32; r += 4) {
+      if (((rows >> r) & 15u) == 0) continue;
+      uint2 x[4], d[4], y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const bool load = mine && ((rows >> (r + k)) & 1u);
+        const long long at = at0 + (r + k) * stride;
+        x[k] = load ? __ldg(reinterpret_cast<const uint2*>(a.o_raw + at)) : make_uint2(0, 0);
+        d[k] = load ? __ldg(reinterpret_cast<const uint2*>(a.do_raw + at)) : make_uint2(0, 0);
+        y[k] = load && a.low_raw ? __ldg(reinterpret_cast<const uint2*>(a.low_raw + at)) : make_uint2(0, 0);
       }
 #pragma unroll
-      for (int o = 16; o; o >>= 1) delta += __shfl_xor_sync(~0u, delta, o);
-      const float ls = a.lse[((long long)b * p.q_heads + h) * p.q_len + i];
-      if (ls > -INFINITY) nl = -ls * kLog2e + (BF16 ? 0.f : (float)kWeightShift);
-      if (!BF16) {
-        const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(peak));
-        if (lane == 0) raise_peak(a.peak + ((long long)b * p.k_heads + h / p.group) * 2, top);
+      for (int k = 0; k < 4; ++k) {
+        const float2 x0 = ptx::add2(unpack2<BF16>(x[k].x), unpack2<BF16>(y[k].x));
+        const float2 x1 = ptx::add2(unpack2<BF16>(x[k].y), unpack2<BF16>(y[k].y));
+        const float2 d0 = unpack2<BF16>(d[k].x), d1 = unpack2<BF16>(d[k].y);
+        float delta = fmaf(x0.x, d0.x, fmaf(x0.y, d0.y, fmaf(x1.x, d1.x, x1.y * d1.y)));
+        if (!BF16) peak = fmaxf(peak, fmaxf(fmaxf(fabsf(d0.x), fabsf(d0.y)), fmaxf(fabsf(d1.x), fabsf(d1.y))));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) delta += __shfl_xor_sync(~0u, delta, o);
+        if (lane == r + k) kept = delta;
       }
     }
-    if (lane == 0) {
-      const long long at = row_slot(p, b, h) + i;
-      a.neg_lse[at] = nl;
-      a.neg_delta[at] = -delta;
+    float nl = -INFINITY;
+    if (real) {
+      const float ls = a.lse[((long long)b * p.q_heads + h) * p.q_len + own];
+      if (ls > -INFINITY) nl = -ls * kLog2e + (BF16 ? 0.f : (float)kWeightShift);
+    }
+    const long long at = row_slot(p, b, h) + own;
+    a.neg_lse[at] = nl;
+    a.neg_delta[at] = -kept;
+    if (!BF16) {
+      const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(peak));
+      if (lane == 0) raise_peak(a.peak + ((long long)b * p.k_heads + h / p.group) * 2, top);
     }
     return;
   }
   if (BF16) return;
-  const long long key = id - rows;
-  if (key >= (long long)p.batch * p.k_len * p.k_heads) return;
-  const int h = (int)(key % p.k_heads), j = (int)(key / p.k_heads % p.k_len), b = (int)(key / p.k_heads / p.k_len);
-  if (p.documents && p.documents[(long long)b * p.k_len + j] < 0) return;
+  const int id = (int)blockIdx.x - g.q_blocks, groups = (p.k_heads + 7) / 8, chunks = (p.k_len + 31) / 32;
+  const int h = id % groups * 8 + warp, i0 = id / groups % chunks * 32, b = id / groups / chunks;
+  if (h >= p.k_heads) return;
   float peak = 0.f;
-  if (lane * 4 < p.dim) {
-    const uint2 x = *reinterpret_cast<const uint2*>(a.v_raw + b * p.v_stride[0] + j * p.v_stride[1] + h * p.v_stride[2] + lane * 4);
+#pragma unroll 4
+  for (int r = 0; r < 32; ++r) {
+    const int j = i0 + r;
+    const bool real = j < p.k_len && (!p.documents || p.documents[(long long)b * p.k_len + j] >= 0);
+    if (!real || !mine) continue;
+    const uint2 x = __ldg(reinterpret_cast<const uint2*>(a.v_raw + b * p.v_stride[0] + j * p.v_stride[1] + h * p.v_stride[2] + lane * 4));
     const float2 x0 = unpack2<BF16>(x.x), x1 = unpack2<BF16>(x.y);
-    peak = fmaxf(fmaxf(fabsf(x0.x), fabsf(x0.y)), fmaxf(fabsf(x1.x), fabsf(x1.y)));
+    peak = fmaxf(peak, fmaxf(fmaxf(fabsf(x0.x), fabsf(x0.y)), fmaxf(fabsf(x1.x), fabsf(x1.y))));
   }
   const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(peak));
   if (lane == 0) raise_peak(a.peak + ((long long)b * p.k_heads + h) * 2 + 1, top);
@@ -356,13 +382,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
         ptx::tc_fence_after();
       };
       auto score_product = [&](uint32_t d, uint32_t own, uint32_t other, uint64_t* bar) {
+        const uint32_t a_low = low_k_major(own), b_low = low_k_major(other);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) ptx::mma_f16_ss_by(leader, d, desc_k_major(low_k_major(own), s), desc_k_major(low_k_major(other), s), id_s, s != 0);
+        for (int s = 0; s < DP / 16; ++s) ptx::mma_f16_ss_by(leader, d, desc_k_major(a_low, s), desc_k_major(b_low, s), id_s, s != 0);
         ptx::mma_commit_by(leader, ptx::smem_u32(bar));
       };
       auto sum_product = [&](uint32_t d, uint32_t w, uint32_t other, bool add, uint64_t* bar) {
+        const uint32_t b_low = low_mn_major(other);
 #pragma unroll
-        for (int s = 0; s < kTile / 16; ++s) ptx::mma_f16_ts_by(leader, d, w + packed_at(s), desc_mn_major(low_mn_major(other), s), id_d, add || s != 0);
+        for (int s = 0; s < kTile / 16; ++s) ptx::mma_f16_ts_by(leader, d, w + packed_at(s), desc_mn_major(b_low, s), id_d, add || s != 0);
         ptx::mma_commit_by(leader, ptx::smem_u32(bar));
       };
       wait(&sh->kv_full[0], 0, 0x520000u);
@@ -371,8 +399,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
       wait(&sh->kv_full[1], 0, 0x520002u);
       wait(&sh->do_full[0], 0, 0x520003u);
       if (ok) score_product(dp_at, v_smem, do_smem, &sh->dp_full);
+      uint32_t slot = 0, parity = 0;
       for (int n = 0; ok && n < steps; ++n) {
-        const uint32_t slot = n % NS, next = (n + 1) % NS, next_parity = ((n + 1) / NS) & 1;
+        const uint32_t next = slot + 1 == NS ? 0 : slot + 1, next_parity = slot + 1 == NS ? parity ^ 1 : parity;
         const bool more = n + 1 < steps;
         wait(&sh->p_full, n & 1, 0x530000u);
         if (!ok) break;
@@ -390,6 +419,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
           if (!ok) break;
           score_product(dp_at, v_smem, do_smem + next * TILE, &sh->dp_full);
         }
+        slot = next;
+        parity = next_parity;
       }
       if (ok) ptx::mma_commit_by(leader, ptx::smem_u32(&sh->acc_full));
     }
@@ -697,37 +728,51 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
         }
         ptx::tc_fence_after();
       };
+      uint32_t k_slot = 0, k_parity = 0, v_slot = 0, v_parity = 0;      // of the next K, V
       auto score = [&](int n) {        // S(n) = Q K(n)
         if (n >= steps) return;
-        wait(&sh->k_full[n % NK], (n / NK) & 1, 0x620000u);
+        wait(&sh->k_full[k_slot], k_parity, 0x620000u);
         if (!ok) return;
+        const uint32_t a_low = low_k_major(q_smem), b_low = low_k_major(k_smem + k_slot * TILE);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
-          ptx::mma_f16_ss_by(leader, s_at + (n & 1) * kTile, desc_k_major(low_k_major(q_smem), s), desc_k_major(low_k_major(k_smem + (n % NK) * TILE), s), id_s, s != 0);
+          ptx::mma_f16_ss_by(leader, s_at + (n & 1) * kTile, desc_k_major(a_low, s), desc_k_major(b_low, s), id_s, s != 0);
         ptx::mma_commit_by(leader, ptx::smem_u32(&sh->s_full[n & 1]));
+        if (++k_slot == NK) {
+          k_slot = 0;
+          k_parity ^= 1;
+        }
       };
       auto grad = [&](int n) {         // dP(n) = dO V(n)
         if (n >= steps) return;
-        wait(&sh->v_full[n % NV], (n / NV) & 1, 0x620001u);
+        wait(&sh->v_full[v_slot], v_parity, 0x620001u);
         if (!ok) return;
+        const uint32_t a_low = low_k_major(do_smem), b_low = low_k_major(v_smem + v_slot * TILE);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
-          ptx::mma_f16_ss_by(leader, dp_at, desc_k_major(low_k_major(do_smem), s), desc_k_major(low_k_major(v_smem + (n % NV) * TILE), s), id_s, s != 0);
+          ptx::mma_f16_ss_by(leader, dp_at, desc_k_major(a_low, s), desc_k_major(b_low, s), id_s, s != 0);
         ptx::mma_commit_by(leader, ptx::smem_u32(&sh->dp_full));
-        ptx::mma_commit_by(leader, ptx::smem_u32(&sh->v_empty[n % NV]));
+        ptx::mma_commit_by(leader, ptx::smem_u32(&sh->v_empty[v_slot]));
+        if (++v_slot == NV) {
+          v_slot = 0;
+          v_parity ^= 1;
+        }
       };
       wait(&sh->q_full[0], 0, 0x620002u);
       if (ok) score(0);
       wait(&sh->q_full[1], 0, 0x620003u);
       if (ok) grad(0);
       if (ok) score(1);
+      uint32_t slot = 0;               // of K(n)
       for (int n = 0; ok && n < steps; ++n) {
         wait(&sh->ds_full, n & 1, 0x630000u);
         if (!ok) break;
+        const uint32_t b_low = low_mn_major(k_smem + slot * TILE);
 #pragma unroll
         for (int s = 0; s < kTile / 16; ++s)
-          ptx::mma_f16_ts_by(leader, dq_at, dp_at + packed_at(s), desc_mn_major(low_mn_major(k_smem + (n % NK) * TILE), s), id_d, (n | s) != 0);
-        ptx::mma_commit_by(leader, ptx::smem_u32(&sh->k_empty[n % NK]));
+          ptx::mma_f16_ts_by(leader, dq_at, dp_at + packed_at(s), desc_mn_major(b_low, s), id_d, n != 0 || s != 0);
+        ptx::mma_commit_by(leader, ptx::smem_u32(&sh->k_empty[slot]));
+        if (++slot == NK) slot = 0;
         grad(n + 1);
         if (ok) score(n + 2);
       }
@@ -940,8 +985,10 @@ int32_t lego_attention_bwd(const lego_attention_t* d, const void* q, const void*
   a.neg_delta = reinterpret_cast<float*>(ws + l.neg_delta);
   a.peak = reinterpret_cast<uint32_t*>(ws + l.peak);
   a.status = ctx->status_word;
-  const long long rows = l.rows + (bf16 ? 0 : (long long)p.batch * p.k_len * p.k_heads), blocks = (rows + 7) / 8;
-  if (blocks > 0x7fffffffLL) return LEGO_ERR_SIZE;
+  if ((int64_t)p.batch * (tiles_of(p.q_len) * 4LL * ((p.q_heads + 7) / 8) + (p.k_len / 32 + 1LL) * ((p.k_heads + 7) / 8)) > 0x7fffffffLL)
+    return LEGO_ERR_SIZE;
+  const PrepGrid grid = prep_grid(p, !bf16);
+  const int blocks = grid.q_blocks + grid.k_blocks;
   st = attention_docs(&a.p, workspace, s);
   if (st != LEGO_OK) return st;
   if (bf16) {
