@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 
 MAX_RANK = 12
@@ -111,6 +112,15 @@ class TreeAttention(C.Structure):
                 ("table_stride", C.c_int64),
                 ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
                 ("scale", C.c_float), ("softcap", C.c_float)]
+
+
+# The same layouts for struct: filling a descriptor field by field through ctypes takes longer
+# than a launch.
+ROTARY_FORMAT = struct.Struct("4i4q2q6q2qfi")
+ATTENTION_FORMAT = struct.Struct("2i6q9q2f3P")
+TREE_ATTENTION_FORMAT = struct.Struct("2i9q9q2f")
+assert (ROTARY_FORMAT.size, ATTENTION_FORMAT.size, TREE_ATTENTION_FORMAT.size) == (
+    C.sizeof(Rotary), C.sizeof(Attention), C.sizeof(TreeAttention))
 
 
 LayoutP = C.POINTER(Layout)

@@ -48,6 +48,11 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def _stream_on(dev: torch.device) -> int:
+    """``_stream()`` of a device by its number, without making a Stream object for it."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
 def _to_device(t: torch.Tensor) -> torch.Tensor:
     if t.is_cuda:
         return t
@@ -833,6 +838,12 @@ def _strided(t: torch.Tensor, dev: torch.device):
     return _dense(t, dev), (b * c * d, c * d, d)
 
 
+def _rows(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """On the device, the last axis contiguous."""
+    t = _ready(t, dev)
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
 def _strides(t: torch.Tensor):
     """Strides of the leading axes of ``[a, b, c, D]`` in elements; an axis of one has none of its own."""
     a, b, c, d = t.shape
@@ -840,15 +851,13 @@ def _strides(t: torch.Tensor):
     return (s[0] if a != 1 else d, s[1] if b != 1 else d, s[2] if c != 1 else d)
 
 
-def _check_int32(t: Optional[torch.Tensor], name: str, shape) -> None:
-    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != tuple(shape)):
+def _check_int32(t: torch.Tensor, name: str, shape) -> None:
+    if t.dtype != torch.int32 or t.shape != shape:
         raise ValueError(f"{name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
 
 
-def _check_slopes(t: Optional[torch.Tensor], heads: int) -> None:
-    if t is None:
-        return
-    if t.dtype != torch.float32 or tuple(t.shape) != (heads,):
+def _check_slopes(t: torch.Tensor, heads: int) -> None:
+    if t.dtype != torch.float32 or t.shape != (heads,):
         raise ValueError(f"slopes must be float32 [{heads}], got {t.dtype} {list(t.shape)}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("slopes are constants of the bias: no gradient is computed for them")
@@ -902,35 +911,39 @@ def _rotary(xs, positions, freqs, pairs, scale, inverse):
     if kind is None:
         raise ValueError(f"pairs must be 'half' or 'interleaved', got {pairs!r}")
     x = xs[0]
-    for t in xs:
-        if t.dim() != 4 or t.dtype not in _ROTARY_TYPES or t.dtype != x.dtype:
+    code = _ROTARY_TYPES.get(x.dtype)
+    if x.dim() != 4 or code is None:
+        raise ValueError("rotary takes [B, S, H, D] tensors of one type: float16, bfloat16 or float32")
+    B, S, H, D = x.shape
+    two = xs[1] if len(xs) > 1 else None
+    H2 = 0
+    if two is not None:
+        if two.dim() != 4 or two.dtype != x.dtype:
             raise ValueError("rotary takes [B, S, H, D] tensors of one type: float16, bfloat16 or float32")
-        if t.shape[:2] != x.shape[:2] or t.shape[3] != x.shape[3]:
+        B2, S2, H2, D2 = two.shape
+        if B2 != B or S2 != S or D2 != D:
             raise ValueError("the tensors must agree in batch, length and head size")
-    B, S, _, D = x.shape
-    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((B, S), (S,)):
+    at = positions.shape
+    if positions.dtype not in (torch.int32, torch.int64) or len(at) not in (1, 2) or at[-1] != S or at[0] != (B if len(at) == 2 else S):
         raise ValueError(f"positions must be int32 or int64 [{B}, {S}] or [{S}]")
-    if freqs.dtype != torch.float64 or freqs.dim() != 1 or freqs.numel() < 1 or 2 * freqs.numel() > D:
+    turns = freqs.numel()
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or turns < 1 or 2 * turns > D:
         raise ValueError(f"freqs must be float64 of 1 .. {D // 2} pairs")
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
-    dev = _same_device(*xs, positions, freqs)
+    dev = _same_device(x, two, positions, freqs)
     with _on(dev):
         pos, fr = _ready(positions, dev), _ready(freqs, dev).contiguous()
-        src, out = [], []
-        for t in xs:
-            t = _ready(t, dev)
-            src.append(t if t.stride(3) == 1 or D == 1 else t.contiguous())
-            out.append(torch.empty(t.shape, dtype=t.dtype, device=dev))
-        one, two = src[0], src[1] if len(src) > 1 else None
-        d = _abi.Rotary(_ROTARY_TYPES[x.dtype], kind, inverse, pos.element_size(), B, S, D, 2 * fr.numel(),
-                        (one.shape[2], 0 if two is None else two.shape[2]),
-                        (_strides(one), (0, 0, 0) if two is None else _strides(two)),
-                        (0 if pos.dim() == 1 else pos.stride(0), pos.stride(-1)), scale)
-        _abi.check(_abi.lib().lego_rotary(C.byref(d), one.data_ptr(), _ptr(two), out[0].data_ptr(),
-                                          None if two is None else out[1].data_ptr(), pos.data_ptr(), fr.data_ptr(),
-                                          _stream()), "lego_rotary")
-        return [_like_input(o, t) for o, t in zip(out, xs)]
+        one, y1, ptr2, y2, st2 = _rows(x, dev), torch.empty((B, S, H, D), dtype=x.dtype, device=dev), None, None, (0, 0, 0)
+        if two is not None:
+            second, y2 = _rows(two, dev), torch.empty((B, S, H2, D), dtype=x.dtype, device=dev)
+            ptr2, st2 = second.data_ptr(), _strides(second)
+        d = _abi.Rotary.from_buffer_copy(_abi.ROTARY_FORMAT.pack(
+            code, kind, inverse, pos.element_size(), B, S, D, 2 * turns, H, H2, *_strides(one), *st2,
+            0 if len(at) == 1 else pos.stride(0), pos.stride(-1), scale, 0))
+        _abi.check(_abi.lib().lego_rotary(C.byref(d), one.data_ptr(), ptr2, y1.data_ptr(), _ptr(y2), pos.data_ptr(),
+                                          fr.data_ptr(), _stream_on(dev)), "lego_rotary")
+        return [_like_input(y1, x)] if two is None else [_like_input(y1, x), _like_input(y2, two)]
 
 
 class LEGORotary(torch.autograd.Function):
@@ -970,34 +983,40 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
 
 def _attention_desc(q, k, v, causal, prefix, documents, softcap, slopes, scale):
     """Checks of an attention call; ``(device, descriptor, tensors it refers to)`` with q, k, v first."""
+    code = _ATTN_TYPES.get(q.dtype)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("attention takes q [B, Sq, Hq, D] and k, v [B, Sk, Hk, D]")
-    if q.dtype not in _ATTN_TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+    if code is None or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("attention takes float16 or bfloat16 tensors of one type")
     B, Sq, Hq, D = q.shape
-    Sk, Hk = k.shape[1], k.shape[2]
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+    Bk, Sk, Hk, Dk = k.shape
+    if Bk != B or Dk != D or k.shape != v.shape:
         raise ValueError("q, k, v must agree in batch and head size, k and v in shape")
     if Hk < 1 or Hq % Hk:
         raise ValueError(f"{Hq} query heads cannot share {Hk} key heads evenly")
     if D % 8 or not 8 <= D <= 128:
         raise ValueError("head size must be a multiple of 8 up to 128")
-    if prefix is not None and not causal:
-        raise ValueError("a prefix needs causal=True")
-    if documents is not None and Sq > Sk:
-        raise ValueError("documents need as many keys as queries at least")
-    _check_int32(prefix, "prefix", (B,))
-    _check_int32(documents, "documents", (B, Sk))
-    _check_slopes(slopes, Hq)
+    if prefix is not None:
+        if not causal:
+            raise ValueError("a prefix needs causal=True")
+        _check_int32(prefix, "prefix", (B,))
+    if documents is not None:
+        if Sq > Sk:
+            raise ValueError("documents need as many keys as queries at least")
+        _check_int32(documents, "documents", (B, Sk))
+    if slopes is not None:
+        _check_slopes(slopes, Hq)
     scale, softcap = _scores(scale, softcap, D)
     dev = _same_device(q, k, v, prefix, documents, slopes)
     (qd, q_st), (kd, k_st), (vd, v_st) = _strided(q, dev), _strided(k, dev), _strided(v, dev)
     keep = [qd, kd, vd]
-    d = _abi.Attention(_ATTN_TYPES[q.dtype], 1 if causal else 0, B, Sq, Sk, Hq, Hk, D, q_st, k_st, v_st, scale, softcap)
-    for name, t in (("slopes", slopes), ("prefix", prefix), ("documents", documents)):
-        if t is not None:
-            keep.append(_ready(t, dev).contiguous())
-            setattr(d, name, keep[-1].data_ptr())
+    options = (0, 0, 0)
+    if slopes is not None or prefix is not None or documents is not None:
+        given = [_optional(t, dev) for t in (slopes, prefix, documents)]
+        options = [t.data_ptr() if t is not None else 0 for t in given]
+        keep += given
+    d = _abi.Attention.from_buffer_copy(_abi.ATTENTION_FORMAT.pack(
+        code, 1 if causal else 0, B, Sq, Sk, Hq, Hk, D, *q_st, *k_st, *v_st, scale, softcap, *options))
     return dev, d, keep
 
 
@@ -1023,7 +1042,7 @@ def _attention_fwd(q, k, v, causal, prefix, documents, softcap, slopes, scale, l
             # only document summaries need a workspace
             ws, n = _attention_workspace(d, 0, dev) if documents is not None else (None, 0)
             _abi.check(_abi.lib().lego_attention_fwd(C.byref(d), keep[0].data_ptr(), keep[1].data_ptr(), keep[2].data_ptr(),
-                                                     o.data_ptr(), _ptr(o_low), lse.data_ptr(), _ptr(ws), n, _stream()),
+                                                     o.data_ptr(), _ptr(o_low), lse.data_ptr(), _ptr(ws), n, _stream_on(dev)),
                        "lego_attention_fwd")
         if q.is_cuda:
             return o, lse, o_low
@@ -1060,7 +1079,7 @@ def attention_bwd(do, q, k, v, o, lse, causal=False, prefix=None, documents=None
             ws, n = _attention_workspace(d, 1, dev)
             _abi.check(_abi.lib().lego_attention_bwd(C.byref(d), keep[0].data_ptr(), keep[1].data_ptr(), keep[2].data_ptr(),
                                                      od.data_ptr(), _ptr(lowd), lsed.data_ptr(), dod.data_ptr(), dq.data_ptr(),
-                                                     dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n, _stream()),
+                                                     dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n, _stream_on(dev)),
                        "lego_attention_bwd")
         return _like_input(dq, q), _like_input(dk, k), _like_input(dv, v)
 
@@ -1125,7 +1144,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     place is not used.  No gradient."""
     if q.dim() != 4 or k_cache.dim() != 4 or v_cache.dim() != 4:
         raise ValueError("tree_attention takes q [B, T, Hq, D] and caches [pages, page_size, Hk, D]")
-    if q.dtype not in _ATTN_TYPES or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    code = _ATTN_TYPES.get(q.dtype)
+    if code is None or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
         raise ValueError("tree_attention takes float16 or bfloat16 tensors of one type")
     B, T, Hq, D = q.shape
     pages, page_size, Hk, _ = k_cache.shape
@@ -1139,12 +1159,14 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         raise ValueError(f"1 .. {_abi.MAX_DRAFT} drafted tokens per sequence")
     if page_table.dim() != 2 or pages < 1 or page_size < 1 or page_table.shape[1] < 1:
         raise ValueError("page_table must be int32 [B, pages of a sequence], the cache must not be empty")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_cache, v_cache)):
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise ValueError("tree_attention has no gradient: call it under torch.no_grad()")
     _check_int32(page_table, "page_table", (B, page_table.shape[1]))
     _check_int32(lengths, "lengths", (B,))
-    _check_int32(parents, "parents", (B, T))
-    _check_slopes(slopes, Hq)
+    if parents is not None:
+        _check_int32(parents, "parents", (B, T))
+    if slopes is not None:
+        _check_slopes(slopes, Hq)
     scale, softcap = _scores(scale, softcap, D)
     dev = _same_device(q, k_cache, v_cache, page_table, lengths, parents, slopes)
     with _on(dev):
@@ -1155,13 +1177,13 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         if B == 0 or Hq == 0:
             return _like_input(o, q)
         n_table = table.shape[1]
-        d = _abi.TreeAttention(_ATTN_TYPES[q.dtype], 0, B, T, Hq, Hk, D, pages, page_size, n_table, n_table, q_st, k_st, v_st,
-                               scale, softcap)
+        d = _abi.TreeAttention.from_buffer_copy(_abi.TREE_ATTENTION_FORMAT.pack(
+            code, 0, B, T, Hq, Hk, D, pages, page_size, n_table, n_table, *q_st, *k_st, *v_st, scale, softcap))
         lib, ref = _abi.lib(), C.byref(d)
         n = lib.lego_tree_attention_workspace_bytes(ref)
         _abi.check(min(n, 0), "lego_tree_attention_workspace_bytes")
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         _abi.check(lib.lego_tree_attention(ref, qd.data_ptr(), kd.data_ptr(), vd.data_ptr(), table.data_ptr(),
                                            lens.data_ptr(), _ptr(par), _ptr(sl), o.data_ptr(), ws.data_ptr(), n,
-                                           _stream()), "lego_tree_attention")
+                                           _stream_on(dev)), "lego_tree_attention")
         return _like_input(o, q)
