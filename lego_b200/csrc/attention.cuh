@@ -34,10 +34,24 @@ struct AttnProblem {
 
 inline __host__ __device__ int tiles_of(int n) { return (n + kTile - 1) / kTile; }
 
+// Pieces a long loop is cut into when a call has fewer CTAs than SMs: enough to fill one wave, or,
+// where a causal or document mask makes the loops unequal, two CTAs per SM; none shorter than four
+// steps (a piece costs its start and its sums' way through memory).  148 SMs whatever the device,
+// so that the workspace follows from the call alone.  Measured: backward, 16384 causal tokens on one
+// key head (128 CTAs), 2392 -> 1580 us; equal loops of that number cut the same way were slower
+// (2944 -> 3322 us), and so was a forward pass of 192 CTAs (81 -> 116 us).
+inline int pieces_of(const AttnProblem& p, long long ctas, long long steps) {
+  if (ctas >= 148) return 1;
+  const long long want = p.causal || p.documents ? (2 * 148 + ctas - 1) / ctas : 148 / ctas, most = steps / 4;
+  return (int)(want < most ? want : most > 1 ? most : 1);
+}
+
 // Refuses what the attention kernels do not take and fills in the device's view of the rest.
 int32_t attention_problem(const lego_attention_t* d, AttnProblem* out);
 // Bytes of the document summaries; 0 without documents.
 int64_t attention_docs_bytes(const AttnProblem& p);
+// Workspace of the forward pass.
+int64_t attention_fwd_bytes(const AttnProblem& p);
 // Enqueues the kernel that writes them to `where` and points the problem at them.
 int32_t attention_docs(AttnProblem* p, void* where, cudaStream_t s);
 

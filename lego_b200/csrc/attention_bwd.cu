@@ -12,6 +12,10 @@
 // addition depends on the order in which CTAs happen to run, and there is no dQ in 32 bits to
 // clear, add to and convert.
 //
+// Where the tiles are too few to load the SMs alike (short or shared key heads; few queries), a
+// CTA's loop is cut into pieces whose sums go through the workspace in 32 bits and are added in
+// order by one more launch.
+//
 // Key kernel: S^T = K Q^T and dP^T = V dO^T into TMEM, one thread per key and half the
 // columns (two warpgroups); P^T and dS^T go back over them as 16-bit pairs and are the TMEM
 // operands of dV += P^T dO and dK += dS^T Q.  The order of issue is dV(n), S(n + 1), dK(n),
@@ -47,6 +51,9 @@ struct BwdArgs {
   float *neg_lse, *neg_delta;        // [batch][q_heads][q_len up to whole tiles], log2 units
   uint32_t* peak;                    // fp16: [batch][k_heads][2] bits of max|dO|, max|V|
   uint32_t* status;
+  int key_pieces, query_pieces;
+  float *key_part, *query_part;      // [piece][tile CTA](dV, dK)[128][DP]; [piece][tile CTA][128][DP]
+  uint16_t *dq_raw, *dk_raw, *dv_raw;
 };
 
 __device__ __forceinline__ long long row_slot(const AttnProblem& p, int b, int h) {
@@ -212,6 +219,52 @@ __device__ __forceinline__ void store_rows(const CUtensorMap* map, uint32_t tmem
   }
 }
 
+// The same rows in 32 bits, to the workspace.
+template <int DP>
+__device__ __forceinline__ void keep_rows(float* to, uint32_t tmem, bool any, float by, int lane) {
+#pragma unroll 1
+  for (int c = 0; c < DP; c += 32) {
+    uint32_t o[32];
+    if (any) {
+      ptx::tmem_ld_32x32(tmem + c, o);
+      ptx::tmem_ld_wait();
+    }
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+      *reinterpret_cast<float4*>(to + lane * DP + c + i) =
+          any ? make_float4(__uint_as_float(o[i]) * by, __uint_as_float(o[i + 1]) * by, __uint_as_float(o[i + 2]) * by,
+                            __uint_as_float(o[i + 3]) * by)
+              : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+}
+
+// The pieces of one result added up in order.  Tiles are numbered [tile][batch][head], `sums` of
+// them side by side (dV, dK); a thread takes four values of a row.
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(256) attn_add_kernel(const float* part, int pieces, int sums, int batch, int heads, int len,
+                                                       int dim, bool reversed, uint16_t* out0, uint16_t* out1) {
+  ptx::grid_dependency_wait();
+  const long long tiles = (long long)tiles_of(len) * batch * heads * sums, per = tiles * kTile * (DP / 4);
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= per) return;
+  const int c = (int)(id % (DP / 4)) * 4, r = (int)(id / (DP / 4) % kTile);
+  const long long slot = id / (DP / 4) / kTile;
+  const int which = (int)(slot % sums);
+  const long long cta = slot / sums;
+  const int h = (int)(cta % heads), b = (int)(cta / heads % batch), n = (int)(cta / heads / batch);
+  const int row = (reversed ? tiles_of(len) - 1 - n : n) * kTile + r;
+  if (row >= len || c >= dim) return;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int x = 0; x < pieces; ++x) {
+    const float4 v = __ldcs(reinterpret_cast<const float4*>(part) + per * x + id);
+    sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+  }
+  uint16_t* out = which ? out1 : out0;
+  *reinterpret_cast<uint2*>(out + (((long long)b * len + row) * heads + h) * dim + c) =
+      make_uint2(pack2<BF16>(sum.x, sum.y), pack2<BF16>(sum.z, sum.w));
+}
+
 // TMEM column of 16 tokens' packed pairs: a warpgroup's half of the columns lies over the
 // scores that this warpgroup has read, the first half at 0, the second at 64.
 __device__ __forceinline__ uint32_t packed_at(int step) { return (step < 4 ? 0 : 64) + (step & 3) * 8; }
@@ -245,8 +298,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
 
   const int warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int heads = p.batch * p.k_heads;
-  const int kt = (int)(blockIdx.x / heads);      // the first keys, which most queries see, come first
-  const int b = blockIdx.x % heads / p.k_heads, hk = blockIdx.x % heads % p.k_heads;
+  const int piece = a.key_pieces > 1 ? (int)(blockIdx.x % a.key_pieces) : 0;
+  const int cta = a.key_pieces > 1 ? (int)(blockIdx.x / a.key_pieces) : (int)blockIdx.x;
+  const int kt = cta / heads;      // the first keys, which most queries see, come first
+  const int b = cta % heads / p.k_heads, hk = cta % heads % p.k_heads;
   const int j0 = kt * kTile;
 
   if (threadIdx.x == 0) {
@@ -305,7 +360,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
   ptx::tc_fence_after();
   const uint32_t tmem = ptx::uniform(sh->tmem_base);
   const uint32_t s_at = tmem, dp_at = tmem + kTile, dv_at = tmem + 2 * kTile, dk_at = dv_at + DP;
-  const int lo = ptx::uniform(sh->lo), per_head = ptx::uniform(sh->hi) - lo, steps = per_head * p.group;
+  const int lo = ptx::uniform(sh->lo), per_head = ptx::uniform(sh->hi) - lo, all_steps = per_head * p.group;
+  const int step0 = (int)((long long)all_steps * piece / a.key_pieces);      // this CTA's steps
+  const int steps = (int)((long long)all_steps * (piece + 1) / a.key_pieces) - step0;
 
   if (warp >= 8) {
     ptx::regs_less<kBwdOtherRegs>();
@@ -324,7 +381,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
       const int4* qd = p.documents ? p.query_docs + (long long)b * tiles_of(p.q_len) : nullptr;
       int n = 0;
       for (; ok && n < steps; ++n) {
-        const int h = hk * p.group + n / per_head, i = lo + n % per_head;
+        const int h = hk * p.group + (step0 + n) / per_head, i = lo + (step0 + n) % per_head;
         const uint32_t slot = n % NS, parity = ((n / NS) & 1) ^ 1;
         const bool dirty = qd && qd[i].z;
         for (int g = 0; g < 2; ++g) {       // Q with the rows' sums, then dO
@@ -455,12 +512,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
       return ok;
     };
     for (int n = 0; n < steps; ++n) {
-      const int h = hk * p.group + n / per_head, i0 = (lo + n % per_head) * kTile;
+      const int h = hk * p.group + (step0 + n) / per_head, i = lo + (step0 + n) % per_head, i0 = i * kTile;
       const uint32_t slot = n % NS;
       const Scores sc = scores_of<CAP>(p.scale, p.softcap, p.slopes, h);
       // seen whole: the first query sees the last key (queries past the end have weight zero)
       bool masked = p.causal && last_key(p, prefix, i0 + p.offset) < j0 + kTile - 1;
-      if (qd) masked = masked || !docs_same(qd[lo + n % per_head], tile_docs);
+      if (qd) masked = masked || !docs_same(qd[i], tile_docs);
       const float4* nl4 = reinterpret_cast<const float4*>(stats + slot * 256 + half * 64);
       const float4* nd4 = nl4 + 32;
       // the row sums arrive with Q, before the scores made from it
@@ -561,12 +618,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
     }
     if (ok && steps > 0) wait(&sh->acc_full, 0, 0x550000u);
     const int row0 = j0 + quarter * 32;
-    if (ok && row0 < p.k_len) {      // staged where K and V were
+    const float dv_by = BF16 ? 1.f : ldexpf(1.f, -kWeightShift), dk_by = p.scale / ds_factor;
+    if (ok && a.key_pieces > 1) {
+      const long long slot = ((long long)piece * (gridDim.x / a.key_pieces) + cta) * 2 + half;
+      keep_rows<DP>(a.key_part + (slot * kTile + quarter * 32) * DP, (half ? dk_at : dv_at) + lanes, steps > 0,
+                    half ? dk_by : dv_by, lane);
+    } else if (ok && row0 < p.k_len) {      // staged where K and V were
       if (half == 0)
-        store_rows<DP, BF16>(&a.dv, dv_at + lanes, steps > 0, BF16 ? 1.f : ldexpf(1.f, -kWeightShift),
+        store_rows<DP, BF16>(&a.dv, dv_at + lanes, steps > 0, dv_by,
                              smem + TILE + quarter * 4096, row0, hk, b, lane);
       else
-        store_rows<DP, BF16>(&a.dk, dk_at + lanes, steps > 0, p.scale / ds_factor, smem + quarter * 4096, row0, hk, b, lane);
+        store_rows<DP, BF16>(&a.dk, dk_at + lanes, steps > 0, dk_by, smem + quarter * 4096, row0, hk, b, lane);
     }
   }
 
@@ -606,8 +668,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
 
   const int warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int heads = p.batch * p.q_heads;
-  const int qt = tiles_of(p.q_len) - 1 - (int)(blockIdx.x / heads);
-  const int b = blockIdx.x % heads / p.q_heads, h = blockIdx.x % heads % p.q_heads, hk = h / p.group;
+  const int piece = a.query_pieces > 1 ? (int)(blockIdx.x % a.query_pieces) : 0;
+  const int cta = a.query_pieces > 1 ? (int)(blockIdx.x / a.query_pieces) : (int)blockIdx.x;
+  const int qt = tiles_of(p.q_len) - 1 - cta / heads;
+  const int b = cta % heads / p.q_heads, h = cta % heads % p.q_heads, hk = h / p.group;
   const int q0 = qt * kTile;
 
   if (threadIdx.x == 0) {
@@ -666,7 +730,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
   ptx::tc_fence_after();
   const uint32_t tmem = ptx::uniform(sh->tmem_base);
   const uint32_t s_at = tmem, dp_at = tmem + 2 * kTile, dq_at = tmem + 3 * kTile;
-  const int lo = ptx::uniform(sh->lo), steps = ptx::uniform(sh->hi) - lo;
+  const int lo_all = ptx::uniform(sh->lo), all_steps = ptx::uniform(sh->hi) - lo_all;
+  const int lo = lo_all + (int)((long long)all_steps * piece / a.query_pieces);      // this CTA's tiles
+  const int steps = lo_all + (int)((long long)all_steps * (piece + 1) / a.query_pieces) - lo;
 
   if (warp >= 8) {
     ptx::regs_less<kBwdOtherRegs>();
@@ -877,7 +943,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
     }
     if (ok && steps > 0) wait(&sh->acc_full, 0, 0x650000u);
     const int row0 = q0 + quarter * 32;
-    if (ok && half == 0 && row0 < p.q_len)      // staged where Q was
+    if (ok && half == 0 && a.query_pieces > 1) {
+      const long long slot = (long long)piece * (gridDim.x / a.query_pieces) + cta;
+      keep_rows<DP>(a.query_part + (slot * kTile + quarter * 32) * DP, dq_at + lanes, steps > 0, p.scale / ds_factor, lane);
+    } else if (ok && half == 0 && row0 < p.q_len)      // staged where Q was
       store_rows<DP, BF16>(&a.dq, dq_at + lanes, steps > 0, p.scale / ds_factor, smem + quarter * 4096, row0, h, b, lane);
   }
 
@@ -904,8 +973,18 @@ int32_t launch_bwd(const BwdArgs& a, int device, cudaStream_t s) {
   const long long key_ctas = (long long)tiles_of(a.p.k_len) * a.p.batch * a.p.k_heads;
   const long long query_ctas = (long long)tiles_of(a.p.q_len) * a.p.batch * a.p.q_heads;
   if (key_ctas > 0x7fffffffLL || query_ctas > 0x7fffffffLL) return LEGO_ERR_SIZE;
-  LEGO_CUDA_TRY(launch_overlapped(keys, dim3((unsigned)key_ctas), dim3(kBwdThreads), key_smem<DP>(), s, a));
-  LEGO_CUDA_TRY(launch_overlapped(queries, dim3((unsigned)query_ctas), dim3(kBwdThreads), query_smem<DP>(), s, a));
+  // (pieces are only made of calls with few CTAs: the products below stay small)
+  auto add = [&](const float* part, int pieces, int sums, long long ctas, int heads, int len, bool reversed, uint16_t* o0, uint16_t* o1) {
+    const long long blocks = (ctas * sums * kTile * (DP / 4) + 255) / 256;
+    return launch_overlapped(attn_add_kernel<DP, BF16>, dim3((unsigned)blocks), dim3(256), 0, s, part, pieces, sums, a.p.batch,
+                             heads, len, a.p.dim, reversed, o0, o1);
+  };
+  LEGO_CUDA_TRY(launch_overlapped(keys, dim3((unsigned)(key_ctas * a.key_pieces)), dim3(kBwdThreads), key_smem<DP>(), s, a));
+  if (a.key_pieces > 1)
+    LEGO_CUDA_TRY(add(a.key_part, a.key_pieces, 2, key_ctas, a.p.k_heads, a.p.k_len, false, a.dv_raw, a.dk_raw));
+  LEGO_CUDA_TRY(launch_overlapped(queries, dim3((unsigned)(query_ctas * a.query_pieces)), dim3(kBwdThreads), query_smem<DP>(), s, a));
+  if (a.query_pieces > 1)
+    LEGO_CUDA_TRY(add(a.query_part, a.query_pieces, 1, query_ctas, a.p.q_heads, a.p.q_len, true, a.dq_raw, nullptr));
   return LEGO_OK;
 }
 
@@ -916,9 +995,11 @@ int32_t launch_bwd_scores(const BwdArgs& a, int device, cudaStream_t s) {
   return bias ? launch_bwd<DP, BF16, false, true>(a, device, s) : launch_bwd<DP, BF16, false, false>(a, device, s);
 }
 
-// Workspace of the backward pass: document summaries, row sums, peaks.
+// Workspace of the backward pass: document summaries, row sums, peaks, the pieces' sums (those of dQ
+// are written after those of dK, dV have been added up, and use their place).
 struct BwdLayout {
-  int64_t rows, neg_lse, neg_delta, peak, bytes;
+  int64_t rows, neg_lse, neg_delta, peak, part, bytes;
+  int key_pieces, query_pieces;
 };
 BwdLayout bwd_layout(const AttnProblem& p) {
   BwdLayout l;
@@ -926,7 +1007,14 @@ BwdLayout bwd_layout(const AttnProblem& p) {
   l.neg_lse = attention_docs_bytes(p);
   l.neg_delta = l.neg_lse + l.rows * 4;
   l.peak = l.neg_delta + l.rows * 4;
-  l.bytes = l.peak + ((int64_t)p.batch * p.k_heads * 8 + 15) / 16 * 16;
+  l.part = l.peak + ((int64_t)p.batch * p.k_heads * 8 + 15) / 16 * 16;
+  const int64_t key_ctas = (int64_t)tiles_of(p.k_len) * p.batch * p.k_heads, query_ctas = (int64_t)tiles_of(p.q_len) * p.batch * p.q_heads;
+  l.key_pieces = pieces_of(p, key_ctas, (int64_t)tiles_of(p.q_len) * p.group);
+  l.query_pieces = pieces_of(p, query_ctas, tiles_of(p.k_len));
+  const int64_t tile = (int64_t)kTile * (p.dim <= 64 ? 64 : 128) * 4;
+  const int64_t keys = l.key_pieces > 1 ? key_ctas * l.key_pieces * 2 * tile : 0;
+  const int64_t queries = l.query_pieces > 1 ? query_ctas * l.query_pieces * tile : 0;
+  l.bytes = l.part + (keys > queries ? keys : queries);
   return l;
 }
 
@@ -941,7 +1029,7 @@ int64_t lego_attention_workspace_bytes(const lego_attention_t* d, int32_t backwa
   AttnProblem p;
   const int32_t st = attention_problem(d, &p);
   if (st != LEGO_OK) return st;
-  return backward ? bwd_layout(p).bytes : attention_docs_bytes(p);
+  return backward ? bwd_layout(p).bytes : attention_fwd_bytes(p);
 }
 
 int32_t lego_attention_bwd(const lego_attention_t* d, const void* q, const void* k, const void* v, const void* o,
@@ -984,6 +1072,12 @@ int32_t lego_attention_bwd(const lego_attention_t* d, const void* q, const void*
   a.neg_lse = reinterpret_cast<float*>(ws + l.neg_lse);
   a.neg_delta = reinterpret_cast<float*>(ws + l.neg_delta);
   a.peak = reinterpret_cast<uint32_t*>(ws + l.peak);
+  a.key_pieces = l.key_pieces;
+  a.query_pieces = l.query_pieces;
+  a.key_part = a.query_part = reinterpret_cast<float*>(ws + l.part);
+  a.dq_raw = (uint16_t*)dq;
+  a.dk_raw = (uint16_t*)dk;
+  a.dv_raw = (uint16_t*)dv;
   a.status = ctx->status_word;
   if ((int64_t)p.batch * (tiles_of(p.q_len) * 4LL * ((p.q_heads + 7) / 8) + (p.k_len / 32 + 1LL) * ((p.k_heads + 7) / 8)) > 0x7fffffffLL)
     return LEGO_ERR_SIZE;
@@ -994,7 +1088,7 @@ int32_t lego_attention_bwd(const lego_attention_t* d, const void* q, const void*
   if (bf16) {
     LEGO_CUDA_TRY(launch_overlapped(attn_bwd_prep_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, s, a));
   } else {
-    LEGO_CUDA_TRY(cudaMemsetAsync(a.peak, 0, (size_t)(l.bytes - l.peak), s));
+    LEGO_CUDA_TRY(cudaMemsetAsync(a.peak, 0, (size_t)(l.part - l.peak), s));
     LEGO_CUDA_TRY(launch_overlapped(attn_bwd_prep_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, s, a));
   }
   if (p.dim <= 64)

@@ -9,6 +9,10 @@
 // tensor core works for the other.  Warps: 0-3 and 4-7 softmax of row tile 0 and 1 (and
 // their epilogue), 8 TMA loads, 9 MMA issue (10 and 11 fill up their warpgroup).
 //
+// Few queries and many keys: the tiles of keys are cut into pieces, a CTA each; a piece leaves its
+// sums in 32 bits and (m, sums) of its rows in the workspace, a second kernel joins them in the
+// order of the keys.
+//
 // Running maximum: the reference value m of a row moves only when a tile's maximum exceeds it
 // by more than 2^8 -- weights stay below 2^8, the row sum is kept in 32 bits -- so O in
 // TMEM is rarely rescaled.  The rounding of the weights to 16 bits, half a step of the type
@@ -43,7 +47,11 @@ struct FwdArgs {
   float* lse;
   uint32_t* status;
   int q_tiles;          // of 256 queries
+  int pieces;
+  float* part;          // pieces > 1: [piece][batch][q_heads][q_len][DP], then 4 floats for every row: m, sum, packed sum
+  uint16_t *o_raw, *low_raw;
 };
+__host__ __device__ inline long long part_rows(const AttnProblem& p) { return (long long)p.batch * p.q_heads * p.q_len; }
 
 struct FwdShared {
   uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2];      // p_full: by halves of the keys
@@ -66,8 +74,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
   const int warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // the last queries, which see the most keys of a causal mask, come first
   const int heads = p.batch * p.q_heads;
-  const int qt = a.q_tiles - 1 - (int)(blockIdx.x / heads);
-  const int bh = blockIdx.x % heads, b = bh / p.q_heads, h = bh % p.q_heads, hk = h / p.group;
+  const int piece = a.pieces > 1 ? (int)(blockIdx.x % a.pieces) : 0, cta = a.pieces > 1 ? (int)(blockIdx.x / a.pieces) : (int)blockIdx.x;
+  const int qt = a.q_tiles - 1 - cta / heads;
+  const int bh = cta % heads, b = bh / p.q_heads, h = bh % p.q_heads, hk = h / p.group;
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
@@ -124,11 +133,22 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = ptx::uniform(sh->tmem_base);
-  const int lo0 = ptx::uniform(sh->lo[0]), hi0 = ptx::uniform(sh->hi[0]);
-  const int lo1 = ptx::uniform(sh->lo[1]), hi1 = ptx::uniform(sh->hi[1]);
-  const bool any0 = lo0 < hi0, any1 = lo1 < hi1;
-  const int lo = !any0 ? lo1 : !any1 ? lo0 : lo0 < lo1 ? lo0 : lo1;
-  const int hi = !any0 ? hi1 : !any1 ? hi0 : hi0 > hi1 ? hi0 : hi1;
+  int lo0 = ptx::uniform(sh->lo[0]), hi0 = ptx::uniform(sh->hi[0]);
+  int lo1 = ptx::uniform(sh->lo[1]), hi1 = ptx::uniform(sh->hi[1]);
+  bool any0 = lo0 < hi0, any1 = lo1 < hi1;
+  int lo = !any0 ? lo1 : !any1 ? lo0 : lo0 < lo1 ? lo0 : lo1;
+  int hi = !any0 ? hi1 : !any1 ? hi0 : hi0 > hi1 ? hi0 : hi1;
+  if (a.pieces > 1) {     // this CTA's piece of them
+    const int first = lo, n = hi - lo;
+    lo = first + (int)((long long)n * piece / a.pieces);
+    hi = first + (int)((long long)n * (piece + 1) / a.pieces);
+    lo0 = lo0 > lo ? lo0 : lo;
+    lo1 = lo1 > lo ? lo1 : lo;
+    hi0 = hi0 < hi ? hi0 : hi;
+    hi1 = hi1 < hi ? hi1 : hi;
+    any0 = lo0 < hi0;
+    any1 = lo1 < hi1;
+  }
 
   if (warp >= 8) {
   ptx::regs_less<kOtherRegs>();
@@ -307,8 +327,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
     const bool has = sum > 0.f || sum != sum;
     if (!a.low) packed_sum = sum;
     const float inv = packed_sum > 0.f || sum != sum ? 1.f / packed_sum : 0.f;
-    if (row < p.q_len && ok)
-      a.lse[((long long)b * p.q_heads + h) * p.q_len + row] = has ? (m + log2f(sum)) * kLn2 : -INFINITY;
     if (ok && l < e) {
       if (!ptx::mbar_wait_bounded(ptx::smem_u32(&sh->o_full[t]), 0, abort_flag, kAttnWait)) ok = false;
       if (!__all_sync(~0u, ok)) {
@@ -317,6 +335,26 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
       }
       ptx::tc_fence_after();
     }
+    if (a.pieces > 1) {
+      const long long at = part_rows(p) * piece + ((long long)b * p.q_heads + h) * p.q_len + row;
+      if (ok && l < e && q0 + quarter * 32 < p.q_len) {
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          ptx::tmem_ld_32x32(o_tmem + c, o);
+          ptx::tmem_ld_wait();
+          if (row < p.q_len)
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<uint4*>(a.part + at * DP + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+      }
+      if (ok && row < p.q_len)
+        reinterpret_cast<float4*>(a.part + part_rows(p) * a.pieces * DP)[at] = make_float4(m, sum, packed_sum, 0.f);
+      ok = false;      // the second kernel writes the results
+    }
+    if (row < p.q_len && ok)
+      a.lse[((long long)b * p.q_heads + h) * p.q_len + row] = has ? (m + log2f(sum)) * kLn2 : -INFINITY;
     for (int low = 0; ok && low <= (a.low ? 1 : 0) && q0 + quarter * 32 < p.q_len; ++low) {   // the tile's own queries are no longer needed: stage there
 #pragma unroll
       for (int c = 0; c < DP; c += 32) {
@@ -364,6 +402,57 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
   }
 }
 
+// A warp per row: the pieces' sums brought to the largest reference value and added in order.
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ FwdArgs a) {
+  const AttnProblem& p = a.p;
+  ptx::grid_dependency_wait();
+  const long long rows = part_rows(p), row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const float4* stats = reinterpret_cast<const float4*>(a.part + rows * a.pieces * DP);
+  float top = -INFINITY;
+  for (int x = lane; x < a.pieces; x += 32) top = fmaxf(top, stats[rows * x + row].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  const float mu = top == -INFINITY ? 0.f : top;
+  constexpr int V = DP / 32;
+  float sum = 0.f, packed_sum = 0.f, acc[V] = {};
+#pragma unroll 4
+  for (int x = 0; x < a.pieces; ++x) {
+    const float4 st = stats[rows * x + row];
+    const float f = ex2(st.x - mu);
+    if (st.y == 0.f) continue;      // saw nothing: its sums were not written
+    sum = fmaf(st.y, f, sum);
+    packed_sum = fmaf(st.z, f, packed_sum);
+    const float* o = a.part + (rows * x + row) * DP + lane * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = fmaf(o[i], f, acc[i]);
+  }
+  const bool has = sum > 0.f || sum != sum;
+  const float inv = has ? 1.f / packed_sum : 0.f;
+  const int i = (int)(row % p.q_len), h = (int)(row / p.q_len % p.q_heads), b = (int)(row / p.q_len / p.q_heads);
+  const long long at = (((long long)b * p.q_len + i) * p.q_heads + h) * p.dim + lane * V;
+  if (lane * V < p.dim) {
+#pragma unroll
+    for (int k = 0; k < V; k += 2) {
+      const float x = acc[k] * inv, y = acc[k + 1] * inv;
+      const uint32_t w = has ? pack2<BF16>(x, y) : 0u;
+      *reinterpret_cast<uint32_t*>(a.o_raw + at + k) = w;
+      if (a.low) {
+        const float2 z = unpack2<BF16>(w);
+        *reinterpret_cast<uint32_t*>(a.low_raw + at + k) = has ? pack2<BF16>(x - z.x, y - z.y) : 0u;
+      }
+    }
+  }
+  if (lane == 0) a.lse[row] = has ? (top + log2f(sum)) * kLn2 : -INFINITY;
+}
+
+// Pieces of a call's loop over the keys, and the workspace they take.
+int fwd_pieces(const AttnProblem& p) {
+  return pieces_of(p, (long long)((p.q_len + 2 * kTile - 1) / (2 * kTile)) * p.batch * p.q_heads, tiles_of(p.k_len));
+}
+
 template <int DP, bool BF16, bool CAP, bool BIAS>
 int32_t launch_fwd(const FwdArgs& a, int device, cudaStream_t s) {
   static PerDeviceFlag ready;
@@ -372,9 +461,11 @@ int32_t launch_fwd(const FwdArgs& a, int device, cudaStream_t s) {
     LEGO_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, fwd_smem<DP>()));
     ready.set(device);
   }
-  const long long ctas = (long long)a.q_tiles * a.p.batch * a.p.q_heads;
+  const long long ctas = (long long)a.q_tiles * a.p.batch * a.p.q_heads * a.pieces;
   if (ctas > 0x7fffffffLL) return LEGO_ERR_SIZE;
   LEGO_CUDA_TRY(launch_overlapped(kernel, dim3((unsigned)ctas), dim3(kFwdThreads), fwd_smem<DP>(), s, a));
+  if (a.pieces > 1)
+    LEGO_CUDA_TRY(launch_overlapped(attn_join_kernel<DP, BF16>, dim3((unsigned)((part_rows(a.p) + 3) / 4)), dim3(128), 0, s, a));
   return LEGO_OK;
 }
 
@@ -388,6 +479,12 @@ int32_t launch_fwd_scores(const FwdArgs& a, int device, cudaStream_t s) {
 }
 
 }  // namespace
+
+int64_t attention_fwd_bytes(const AttnProblem& p) {
+  const int pieces = fwd_pieces(p);
+  return attention_docs_bytes(p) + (pieces > 1 ? part_rows(p) * pieces * ((p.dim <= 64 ? 64 : 128) + 4) * 4 : 0);
+}
+
 }  // namespace lego
 
 using namespace lego;
@@ -400,7 +497,7 @@ extern "C" int32_t lego_attention_fwd(const lego_attention_t* d, const void* q, 
   if (st != LEGO_OK) return st;
   if (!q || !k || !v || !o || !lse) return LEGO_ERR_NULL;
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)o_low | (uintptr_t)workspace) & 15) return LEGO_ERR_ALIGN;
-  const int64_t need = lego_attention_workspace_bytes(d, 0);
+  const int64_t need = attention_fwd_bytes(a.p);
   if (need && !workspace) return LEGO_ERR_NULL;
   if (workspace_bytes < need) return LEGO_ERR_SIZE;
   DeviceCtx* ctx = device_ctx(&st);
@@ -424,6 +521,10 @@ extern "C" int32_t lego_attention_fwd(const lego_attention_t* d, const void* q, 
   a.lse = lse;
   a.status = ctx->status_word;
   a.q_tiles = (p.q_len + 2 * kTile - 1) / (2 * kTile);
+  a.pieces = fwd_pieces(p);
+  a.part = reinterpret_cast<float*>((uint8_t*)workspace + attention_docs_bytes(p));
+  a.o_raw = (uint16_t*)o;
+  a.low_raw = (uint16_t*)o_low;
   if (p.dim <= 64)
     return bf16 ? launch_fwd_scores<64, true>(a, ctx->device, s) : launch_fwd_scores<64, false>(a, ctx->device, s);
   return bf16 ? launch_fwd_scores<128, true>(a, ctx->device, s) : launch_fwd_scores<128, false>(a, ctx->device, s);

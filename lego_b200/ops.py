@@ -1022,8 +1022,9 @@ def _attention_desc(q, k, v, causal, prefix, documents, softcap, slopes, scale):
 
 def _attention_workspace(d, backward, dev):
     n = _abi.lib().lego_attention_workspace_bytes(C.byref(d), backward)
-    _abi.check(min(n, 0), "lego_attention_workspace_bytes")
-    return torch.empty(max(n, 16), dtype=torch.uint8, device=dev), n
+    if n < 0:
+        _abi.check(n, "lego_attention_workspace_bytes")
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None, n
 
 
 def _attention_fwd(q, k, v, causal, prefix, documents, softcap, slopes, scale, low):
@@ -1039,8 +1040,7 @@ def _attention_fwd(q, k, v, causal, prefix, documents, softcap, slopes, scale, l
             lse.fill_(-math.inf)
             o_low = None
         elif o.numel():
-            # only document summaries need a workspace
-            ws, n = _attention_workspace(d, 0, dev) if documents is not None else (None, 0)
+            ws, n = _attention_workspace(d, 0, dev)
             _abi.check(_abi.lib().lego_attention_fwd(C.byref(d), keep[0].data_ptr(), keep[1].data_ptr(), keep[2].data_ptr(),
                                                      o.data_ptr(), _ptr(o_low), lse.data_ptr(), _ptr(ws), n, _stream_on(dev)),
                        "lego_attention_fwd")

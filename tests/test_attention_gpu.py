@@ -288,6 +288,21 @@ def test_empty_calls():
     assert ops.attention(z(0, 3, 2, 64), z(0, 5, 1, 64), z(0, 5, 1, 64)).shape == (0, 3, 2, 64)
 
 
+@pytest.mark.parametrize("Sq,Sk,Hq,Hk", [(1, 9000, 8, 2), (3, 5001, 2, 2), (130, 4097, 4, 1), (4097, 130, 4, 1)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_few_tiles_and_long_loops(Sq, Sk, Hq, Hk, causal):
+    """Calls whose loops are cut into pieces and joined: plain, with pieces a mask leaves empty, with scores that
+    grow from piece to piece."""
+    q, k, v, do = make(51, 1, Sq, Sk, Hq, Hk, 64, torch.bfloat16)
+    check(q, k, v, do, causal=causal)
+    if Sq <= Sk:
+        docs = torch.arange(Sk, dtype=torch.int32, device="cuda")[None] // 700
+        docs[:, -40:] = docs[0, 40]          # the last queries' document is one of the first, and these
+        check(q, k, v, do, causal=causal, documents=docs, softcap=9.0)
+    k = (k.float() * torch.linspace(0.1, 20, Sk, device="cuda")[None, :, None, None]).to(k.dtype)
+    check(q, k, v, do, causal=causal, slopes=slopes_of(Hq))
+
+
 @pytest.mark.parametrize("Sq,Sk,D,dtype", [(2047, 2047, 128, torch.bfloat16), (1025, 4100, 64, torch.float16)])
 def test_longer(Sq, Sk, D, dtype):
     q, k, v, do = make(50, 1, Sq, Sk, 4, 1, D, dtype)
