@@ -30,6 +30,7 @@ struct RotArgs {
   int pos64, inverse;
   float scale;
   int per_block;          // tokens per block
+  FastDiv by_units, by_heads;      // units of a head; heads of both tensors
 };
 
 // VEC values of T at once; VEC = 16 / sizeof(T) for aligned tensors, 1 otherwise.
@@ -53,15 +54,23 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, VEC>& r) {
 template <typename T, int VEC, bool HALF>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotArgs a) {
   extern __shared__ float2 turn[];   // [token][pair] (cos, sin), scaled
+  __shared__ long long row[2][kRotMaxTokens];      // where a token's heads start in either input
   ptx::launch_dependents();
   ptx::grid_dependency_wait();
   const long long t0 = (long long)blockIdx.x * a.per_block;
   const int nt = (int)(a.tokens - t0 < a.per_block ? a.tokens - t0 : a.per_block);
 
+  __shared__ long long place[kRotMaxTokens];
+  if (threadIdx.x < nt) {
+    const long long b = (t0 + threadIdx.x) / a.length, s = (t0 + threadIdx.x) - b * a.length;
+    row[0][threadIdx.x] = b * a.in_stride[0][0] + s * a.in_stride[0][1];
+    row[1][threadIdx.x] = b * a.in_stride[1][0] + s * a.in_stride[1][1];
+    place[threadIdx.x] = b * a.pos_stride[0] + s * a.pos_stride[1];
+  }
+  __syncthreads();
   for (int i = threadIdx.x; i < nt * a.half; i += kRotThreads) {
     const int t = i / a.half, p = i - t * a.half;
-    const long long b = (t0 + t) / a.length, s = (t0 + t) - b * a.length;
-    const long long at = b * a.pos_stride[0] + s * a.pos_stride[1];
+    const long long at = place[t];
     const double pos = a.pos64 ? (double)reinterpret_cast<const long long*>(a.positions)[at]
                                : (double)reinterpret_cast<const int*>(a.positions)[at];
     double turns = pos * a.freqs[p] * 0.15915494309189533577;   // 1 / (2 pi)
@@ -77,16 +86,15 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
   const int per_head = rot_units + copy_units;
   const int h0 = a.heads[0], heads = h0 + a.heads[1];
   const int units = nt * heads * per_head;
-#pragma unroll 2
+#pragma unroll 4
   for (int i = threadIdx.x; i < units; i += kRotThreads) {
-    const int head_id = i / per_head, u = i - head_id * per_head;
-    const int t = head_id / heads, hh = head_id - t * heads;
-    const int which = hh >= h0, h = which ? hh - h0 : hh;
-    const long long tok = t0 + t;
-    const long long b = tok / a.length, s = tok - b * a.length;
-    const T* x = reinterpret_cast<const T*>(a.x[which]) + b * a.in_stride[which][0] + s * a.in_stride[which][1] +
-                 h * a.in_stride[which][2];
-    T* y = reinterpret_cast<T*>(a.y[which]) + (tok * a.heads[which] + h) * a.dim;
+    const int head_id = (int)fd_div((uint32_t)i, a.by_units), u = i - head_id * per_head;
+    const int t = (int)fd_div((uint32_t)head_id, a.by_heads), hh = head_id - t * heads;
+    const bool second = hh >= h0;
+    const int h = second ? hh - h0 : hh;
+    const T* x = reinterpret_cast<const T*>(second ? a.x[1] : a.x[0]) + row[second ? 1 : 0][t] +
+                 h * (second ? a.in_stride[1][2] : a.in_stride[0][2]);
+    T* y = reinterpret_cast<T*>(second ? a.y[1] : a.y[0]) + ((t0 + t) * (second ? a.heads[1] : h0) + h) * a.dim;
     if (u >= rot_units) {
       const int c = 2 * a.half + (u - rot_units) * VEC;
       store_pack<T, VEC>(y + c, load_pack<T, VEC>(x + c));
@@ -188,6 +196,10 @@ extern "C" int32_t lego_rotary(const lego_rotary_t* d, const void* x0, const voi
   a.scale = d->scale;
   a.per_block = 1;
   while (a.per_block < kRotMaxTokens && a.tokens / (2 * a.per_block) >= 148 * 8) a.per_block *= 2;
+  const int vec_values = vec ? vec_elems : 1;
+  const int rot_units = half ? a.half / vec_values : (vec ? 2 * a.half / vec_values : a.half);
+  a.by_units = make_fastdiv((uint64_t)(rot_units + (a.dim - 2 * a.half) / vec_values));
+  a.by_heads = make_fastdiv((uint64_t)(a.heads[0] + a.heads[1]));
   const long long blocks = (a.tokens + a.per_block - 1) / a.per_block;
   if (blocks > 0x7fffffffLL) return LEGO_ERR_SIZE;
   const size_t smem = (size_t)a.per_block * a.half * sizeof(float2);   // at most 8 x 512 x 8 = 32 KiB
