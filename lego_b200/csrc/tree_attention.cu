@@ -24,12 +24,13 @@
 //
 // Warps: 0-3 and 4-7 weights of the even and the odd tiles of a piece (each with its own m, sum
 // and O, put together at the piece's end), 8-11 loads, 12 MMA issue (13-15 fill up their
-// warpgroup).  Each loading lane looks up the place of one row of a tile.  Tiles of cached
-// tokens come by TMA, in boxes of as many rows as stand together in a page (a common divisor
-// of the page size and 32, at least 8).  The last tiles of a sequence, which hold drafted tokens
-// and end somewhere, and pages of other sizes come as 16-byte copies.  Keys that do not exist
-// (past the end, of a page number outside the cache, of an unused drafted token) are zeros in
-// shared memory and hidden by a mask that the loads leave with the tile.
+// warpgroup).  Each loading lane looks up the place of one row of a tile.  Tiles come by TMA, in
+// boxes of as many rows as stand together in a page (a common divisor of the page size and 32, at
+// least 8); pages of other sizes come as 16-byte copies.  Keys that do not exist (past the end, of
+// a page number outside the cache, of an unused drafted token) are hidden by a mask that the loads
+// leave with the tile, and their values, which may be NaN and must not meet a zero weight, are
+// zeros in shared memory: a box past the cache reads as zeros, other rows are cleared by the
+// loading warp before it hands the tile on.
 #include <cuda.h>
 
 #include "attention.cuh"
@@ -118,12 +119,6 @@ __device__ __forceinline__ int tree_places(const TreeProblem& p, int len) {
   return len < room - p.drafted ? len + p.drafted : room;
 }
 __device__ __forceinline__ int run_begin(int total, int runs, int c) { return total / runs * c + total % runs * c / runs; }
-
-// Every key of a tile is a cached token within the table.
-__device__ __forceinline__ bool all_cached(int tile, int len, int places) {
-  const int end = (tile + 1) * kTile;
-  return end <= len && end <= places;
-}
 
 struct Piece {
   int b, hk, rt;         // sequence (-1: no more pieces), key head, row tile
@@ -216,7 +211,7 @@ struct TreeShared {
   Tree tree[2];
   Piece piece[2];
   uint32_t exist[kMaskRing][4];
-  uint64_t exist_full[kMaskRing], full[10], empty[10];
+  uint64_t exist_full[kMaskRing], full[10], empty[10], cleared[4];
   uint64_t piece_full[2], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], odd_done, o_free, merged;
   int words[16];
   int start_b, start_hr, start_tile, start_left;
@@ -253,6 +248,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
       ptx::mbar_init(ptx::smem_u32(&sh->empty[s]), 1);
     }
     for (int s = 0; s < kMaskRing; ++s) ptx::mbar_init(ptx::smem_u32(&sh->exist_full[s]), 4);
+    for (int s = 0; s < 4; ++s) ptx::mbar_init(ptx::smem_u32(&sh->cleared[s]), 1);
     sh->abort_flag = 0;
     sh->start_left = 0;
     ptx::fence_barrier_init();
@@ -331,7 +327,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             const uint32_t slot = pos % NS;
             wait(&sh->full[slot], (pos / NS) & 1, 0x720002u);
             if (!ok) break;
-            if (!(p.box_rows && all_cached(pc.first + i, pc.len, pc.places)))
+            if (!p.box_rows)
               ptx::fence_proxy_async();      // so did these keys
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s)
@@ -345,7 +341,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             wait(&sh->full[slot], (vpos / NS) & 1, 0x720003u);
             wait(&sh->p_full[t], weighed[t] & 1, 0x720004u);
             if (!ok) break;
-            if (!(p.box_rows && all_cached(pc.first + i - 1, pc.len, pc.places))) ptx::fence_proxy_async();
+            if (!p.box_rows) ptx::fence_proxy_async();
             ++weighed[t];
 #pragma unroll
             for (int s = 0; s < kTile / 16; ++s)
@@ -364,7 +360,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
     constexpr int CH = DP / 8, PER = 32 / CH;    // 16-byte pieces of a row; rows per instruction
     const int w = warp - 8, chunk = lane % CH, sub = lane / CH;
     const bool chunk_real = chunk * 8 < p.dim;
-    uint32_t issued = 0, tile_no = 0;
+    uint32_t issued = 0, tile_no = 0, clears = 0;
     bool ok = true;
     auto bounded = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
       if (lane == 0) ok = ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, abort_flag, kAttnWait);
@@ -420,22 +416,20 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
 
       const int places = pc.places;
       const int* table = p.table + pc.b * p.table_stride;
-      // page number of this lane's row of a tile, as the table has it; -1: the row does not exist
+      // page number of this lane's row of a tile, as the table has it; -1: past the end
       auto page_of = [&](int tile) {
         const int j = tile * kTile + w * 32 + lane;
-        if (tile >= pc.last || j >= places) return -1;
-        if (j >= pc.len && tree->seen[j - pc.len] == 0) return -1;
-        return table[fd_div((uint32_t)j, p.by_page)];
+        return tile < pc.last && j < places ? table[fd_div((uint32_t)j, p.by_page)] : -1;
       };
       int page = page_of(pc.first);
       for (int tile = pc.first; ok && tile < pc.last; ++tile, ++tile_no) {
-        const bool real = page >= 0 && page < p.pages;
-        const int here = real ? page : p.pages;     // past the cache: a TMA box of zeros
-        page = page_of(tile + 1);                   // on its way while this tile's copies are issued
         const int place = tile * kTile + w * 32 + lane;
         const int in_page = place - (int)fd_div((uint32_t)place, p.by_page) * p.page_size;
+        const bool paged = page >= 0 && page < p.pages;
+        const int here = paged ? page : p.pages;     // past the cache: a TMA box of zeros
+        const bool real = paged && (place < pc.len || tree->seen[place - pc.len] != 0);
+        page = page_of(tile + 1);                    // on its way while this tile's copies are issued
         const uint32_t word = __ballot_sync(~0u, real);
-        const bool boxes = p.box_rows && all_cached(tile, pc.len, places);
         for (int g = 0; g < 2; ++g, ++issued) {
           const uint32_t slot = issued % NS, full = ptx::smem_u32(&sh->full[slot]);
           if (!bounded(&sh->empty[slot], ((issued / NS) & 1) ^ 1, 0x710001u)) break;
@@ -447,10 +441,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             ptx::mbar_arrive(ptx::smem_u32(&sh->exist_full[tile_no % kMaskRing]));
           }
           const uint32_t dst = kv_smem + slot * TILE + w * 4096;     // this warp's rows in the first box
-          if (boxes) {
-            if (lane == 0) {      // for the 32 arrivals a warp's copies count as
-              ptx::mbar_arrive_expect_tx(full, TILE / 4);
-              ptx::mbar_arrive_n(full, 31);
+          if (p.box_rows) {
+            const bool clear = g == 1 && word != ~0u;
+            const uint32_t bar = clear ? ptx::smem_u32(&sh->cleared[w]) : full;
+            if (lane == 0) {
+              ptx::mbar_arrive_expect_tx(bar, TILE / 4);
+              if (!clear) ptx::mbar_arrive_n(full, 31);      // 32 arrivals, as of a warp's copies
             }
             __syncwarp();
             constexpr int WIDE = DP / 64;
@@ -458,7 +454,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             const int pg = __shfl_sync(~0u, here, r & 31), at_slot = __shfl_sync(~0u, in_page, r & 31);
             if (r < 32) {
               const int32_t at[5] = {c * 64, at_slot, pc.hk, pg, 0};
-              ptx::tma_load_nd(4, dst + c * kBoxBytes + r * 128, g ? &maps.v : &maps.k, at, full);
+              ptx::tma_load_nd(4, dst + c * kBoxBytes + r * 128, g ? &maps.v : &maps.k, at, bar);
+            }
+            if (clear) {
+              __syncwarp();
+              if (!bounded(&sh->cleared[w], clears++ & 1, 0x710003u)) break;
+              if (lane < CH)
+                for (uint32_t dead = ~word; dead; dead &= dead - 1)
+                  *reinterpret_cast<uint4*>(smem + (2 + slot) * TILE + (lane >> 3) * kBoxBytes + (w * 32 + __ffs(dead) - 1) * 128 +
+                                            ((lane & 7) << 4)) = make_uint4(0, 0, 0, 0);
+              ptx::fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) ptx::mbar_arrive_n(full, 32);
             }
             continue;
           }
@@ -479,7 +486,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
       }
       if (w > 0 && lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->q_empty[n & 1]));
     }
-    ptx::cp_async_wait_all();      // leave no copy in flight
+    ptx::cp_async_wait_all();
+    if (*abort_flag && lane == 0) {      // leave no copy in flight: a tenth of a second for each slot at most
+      uint32_t never = 0;
+      for (uint32_t s = 0; s < (uint32_t)NS; ++s)
+        if (issued > s) ptx::mbar_wait_bounded(ptx::smem_u32(&sh->full[s]), ((issued - 1 - s) / NS) & 1, &never, kAttnWait / 10);
+    }
   } else {
     ptx::regs_more<kTreeMathRegs>();
     // ---------------- weights, epilogue ----------------
