@@ -27,6 +27,16 @@ inline EncodeFn encode_fn(int32_t* err) {
     if (q != cudaDriverEntryPointSuccess || !p) { status = LEGO_ERR_UNSUPPORTED; return; }
     fn = (EncodeFn)p;
   });
+  // The driver call wants a current context, which a thread that has made no runtime call of its own
+  // (autograd's, say) does not have: make the device's primary context current.
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess) e = cudaSetDevice(device);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    if (err) *err = cuda_status(e);
+    return nullptr;
+  }
   if (err) *err = status;
   return fn;
 }

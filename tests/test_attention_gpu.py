@@ -265,6 +265,26 @@ def test_captured_and_replayed():
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_from_a_thread_of_its_own():
+    """A thread that has made no CUDA call yet, as autograd's is in a process that only trains: it has no
+    current context, which building the tensor maps needs."""
+    import threading
+    q, k, v, do = make(41, 1, 140, 140, 2, 1, 64, torch.bfloat16)
+    o, lse = ops.attention_fwd(q, k, v, True)
+    want = (o, lse, *ops.attention_bwd(do, q, k, v, o, lse, True))
+    got = []
+
+    def work():
+        got.extend(ops.attention_bwd(do, q, k, v, o, lse, True))
+        got.extend(ops.attention_fwd(q, k, v, True))
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert len(got) == 5 and all(torch.equal(a, b) for a, b in zip(got[3:] + got[:3], want))
+
+
 def test_host_tensors():
     q, k, v, do = (x.cpu() for x in make(40, 1, 60, 90, 2, 1, 64, torch.float16))
     o, lse = ops.attention_fwd(q, k, v, True)
