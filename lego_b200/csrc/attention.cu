@@ -4,6 +4,12 @@
 
 namespace lego {
 
+bool scores_ok(float scale, float softcap) {
+  const float most = 1e30f;      // what is made of them stays finite
+  if (!(softcap >= 0.f && softcap < most) || !(scale > -most && scale < most)) return false;
+  return softcap == 0.f || (scale < most * softcap && scale > -most * softcap);
+}
+
 int32_t attention_problem(const lego_attention_t* d, AttnProblem* p) {
   if (!d) return LEGO_ERR_NULL;
   if (d->dtype != LEGO_F16 && d->dtype != LEGO_BF16) return LEGO_ERR_UNSUPPORTED;
@@ -14,7 +20,7 @@ int32_t attention_problem(const lego_attention_t* d, AttnProblem* p) {
   if (d->batch * d->q_heads > (1LL << 31) / 64 ) return LEGO_ERR_SIZE;
   if (d->documents && d->q_len > d->k_len) return LEGO_ERR_SIZE;
   if (d->prefix && !d->causal) return LEGO_ERR_SIZE;
-  if (!(d->softcap >= 0.f) || d->softcap > 3e38f || !(d->scale >= -3e38f && d->scale <= 3e38f)) return LEGO_ERR_SIZE;
+  if (!scores_ok(d->scale, d->softcap)) return LEGO_ERR_SIZE;
   p->batch = (int)d->batch;
   p->q_len = (int)d->q_len;
   p->k_len = (int)d->k_len;

@@ -46,6 +46,8 @@ inline int pieces_of(const AttnProblem& p, long long ctas, long long steps) {
   return (int)(want < most ? want : most > 1 ? most : 1);
 }
 
+// Whether a scale and a cap (0: none) are numbers the kernels can work with.
+bool scores_ok(float scale, float softcap);
 // Refuses what the attention kernels do not take and fills in the device's view of the rest.
 int32_t attention_problem(const lego_attention_t* d, AttnProblem* out);
 // Bytes of the document summaries; 0 without documents.
@@ -90,11 +92,11 @@ __device__ __forceinline__ float rcp(float x) {
   return y;
 }
 // 2^z for z < 128 on the FMA pipe: z = n + r with |r| <= 1/2, a polynomial of degree 5 for 2^r
-// (fitted for the least relative error with p(0) = 1: 9.2e-8, 1.9e-7 in 32 bits), n added to the
-// exponent.  Zero from 2^-127 down, -inf among them.  An SM takes 16 ex2 per cycle, 1024 cycles
+// (fitted for the least relative error with p(0) = 1: 9.2e-8, 1.9e-7 in 32 bits), times 2^n.
+// Zero from 2^-127 down, -inf among them; a NaN stays one.  An SM takes 16 ex2 per cycle, 1024 cycles
 // for a tile of scores, and the issue slots are idle meanwhile: some of the weights go this way.
 __device__ __forceinline__ float2 ex2_fma(float2 z) {
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(z.x));      // -127; a NaN stays one
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(z.x));      // -127
   asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(z.y));
   const float2 big = make_float2(12582912.f, 12582912.f);   // 1.5 2^23: rounds to an integer in the low bits
   const float2 t = ptx::add2(z, big);
@@ -106,8 +108,9 @@ __device__ __forceinline__ float2 ex2_fma(float2 z) {
   p = ptx::fma2(p, r, make_float2(2.402224243e-01f, 2.402224243e-01f));
   p = ptx::fma2(p, r, make_float2(6.931470037e-01f, 6.931470037e-01f));
   p = ptx::fma2(p, r, make_float2(1.f, 1.f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+  const float2 scale = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),      // 2^n, 0 for -127
+                                   __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
+  return ptx::mul2(p, scale);
 }
 // tanh(u) for |u| <= 1: an odd polynomial of degree 13, off by 2e-8 (1e-7 in 32 bits).  Scores under
 // a cap rarely reach it, and the exact way below takes two of the 16 per cycle.

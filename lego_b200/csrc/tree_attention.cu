@@ -79,7 +79,7 @@ int32_t tree_problem(const lego_tree_attention_t* d, TreeProblem* p) {
   if (d->batch > 65535 || d->q_heads > 65535 || d->pages > 0x7fffffffLL || d->page_size > (1 << 30) ||
       d->max_pages > (1 << 30) / d->page_size || d->table_stride < d->max_pages)
     return LEGO_ERR_SIZE;
-  if (!(d->softcap >= 0.f) || d->softcap > 3e38f || !(d->scale >= -3e38f && d->scale <= 3e38f)) return LEGO_ERR_SIZE;
+  if (!scores_ok(d->scale, d->softcap)) return LEGO_ERR_SIZE;
   p->batch = (int)d->batch;
   p->drafted = (int)d->drafted;
   p->q_heads = (int)d->q_heads;

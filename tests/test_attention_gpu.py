@@ -265,6 +265,39 @@ def test_captured_and_replayed():
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_captured_training_step():
+    """Forward and gradients through autograd inside a capture, while another graph of the same leaves is alive."""
+    q, k, v, do = make(26, 1, 300, 300, 4, 2, 64, torch.bfloat16)
+    for x in (q, k, v):
+        x.requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = ops.attention(q, k, v, causal=True)
+        want = torch.autograd.grad(alive, (q, k, v), do, retain_graph=True)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = ops.attention(q, k, v, causal=True)
+        got = torch.autograd.grad(o, (q, k, v), do)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, alive) and all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(alive, (q, k, v), do), want))
+
+
+def test_a_nan_is_seen():
+    """A NaN in a key makes the rows that see it NaN, whichever column it stands in, and no row of an earlier tile."""
+    for at in (200, 201, 202, 203, 204, 205):
+        q, k, v, _ = make(27, 1, 260, 260, 1, 1, 64, torch.bfloat16)
+        k[0, at, 0, 5] = float("nan")
+        for how in (dict(), dict(softcap=9.0)):
+            o, lse = ops.attention_fwd(q, k, v, True, **how)
+            assert torch.isnan(o[0, at:]).all() and torch.isnan(lse[0, 0, at:]).all()
+            assert torch.isfinite(o[0, :at]).all() and torch.isfinite(lse[0, 0, :at]).all()
+
+
 def test_from_a_thread_of_its_own():
     """A thread that has made no CUDA call yet, as autograd's is in a process that only trains: it has no
     current context, which building the tensor maps needs."""

@@ -96,7 +96,8 @@ def test_the_c_entry_points_return_their_reasons():
     assert lib.lego_attention_workspace_bytes(None, 0) == -1
     for change, status in ((dict(dtype=2), -8), (dict(batch=0), -4), (dict(q_len=0), -4), (dict(head_dim=136), -6),
                            (dict(head_dim=12), -6), (dict(q_heads=3, k_heads=2), -6), (dict(softcap=-1.0), -6),
-                           (dict(scale=math.nan), -6), (dict(causal=0, prefix=4096), -6),
+                           (dict(scale=math.nan), -6), (dict(scale=1e38), -6), (dict(softcap=1e-35, scale=1.0), -6),
+                           (dict(causal=0, prefix=4096), -6),
                            (dict(q_len=5, documents=4096), -6), (dict(q_len=1 << 40), -6)):
         assert lib.lego_attention_workspace_bytes(C.byref(attention_desc(**change)), 0) == status, change
     odd = attention_desc()
