@@ -86,31 +86,23 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// The largest of N values: three to an instruction, four chains.
+template <int N>
+__device__ __forceinline__ float max_of(const float (&s)[N]) {
+  float top[4] = {max3(s[0], s[1], s[2]), max3(s[3], s[4], s[5]), max3(s[6], s[7], s[8]), max3(s[9], s[10], s[11])};
+#pragma unroll
+  for (int c = 12; c + 1 < N; c += 2) top[(c >> 1) & 3] = max3(top[(c >> 1) & 3], s[c], s[c + 1]);
+  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
 __device__ __forceinline__ float rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-// 2^z for z < 128 on the FMA pipe: z = n + r with |r| <= 1/2, a polynomial of degree 5 for 2^r
-// (fitted for the least relative error with p(0) = 1: 9.2e-8, 1.9e-7 in 32 bits), times 2^n.
-// Zero from 2^-127 down, -inf among them; a NaN stays one.  An SM takes 16 ex2 per cycle, 1024 cycles
-// for a tile of scores, and the issue slots are idle meanwhile: some of the weights go this way.
-__device__ __forceinline__ float2 ex2_fma(float2 z) {
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(z.x));      // -127
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(z.y));
-  const float2 big = make_float2(12582912.f, 12582912.f);   // 1.5 2^23: rounds to an integer in the low bits
-  const float2 t = ptx::add2(z, big);
-  const float2 n = ptx::add2(t, make_float2(-12582912.f, -12582912.f));
-  const float2 r = ptx::fma2(n, make_float2(-1.f, -1.f), z);
-  float2 p = make_float2(1.326472848e-03f, 1.326472848e-03f);
-  p = ptx::fma2(p, r, make_float2(9.671512991e-03f, 9.671512991e-03f));
-  p = ptx::fma2(p, r, make_float2(5.550733581e-02f, 5.550733581e-02f));
-  p = ptx::fma2(p, r, make_float2(2.402224243e-01f, 2.402224243e-01f));
-  p = ptx::fma2(p, r, make_float2(6.931470037e-01f, 6.931470037e-01f));
-  p = ptx::fma2(p, r, make_float2(1.f, 1.f));
-  const float2 scale = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),      // 2^n, 0 for -127
-                                   __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
-  return ptx::mul2(p, scale);
 }
 // tanh(u) for |u| <= 1: an odd polynomial of degree 13, off by 2e-8 (1e-7 in 32 bits).  Scores under
 // a cap rarely reach it, and the exact way below takes two of the 16 per cycle.
@@ -227,8 +219,6 @@ __device__ __forceinline__ void copy_tile_clean(uint8_t* tile, const uint16_t* b
 // log2 of the growth a row's reference value may lag behind its maximum: weights stay below
 // 2^8, their sum is kept in 32 bits, and O in TMEM is rarely rescaled.
 constexpr float kRescale = 8.f;
-// One pair of weights in so many goes to the FMA pipe.
-constexpr int kFmaEvery = 3;
 
 // A row's reference value m for a tile whose maximum is mt (log2 units).  Not the first tile:
 // where some row of the warp outgrew its reference value, its sums, in two registers and over DP
@@ -271,6 +261,23 @@ __device__ __forceinline__ Scores scores_of(float scale, float softcap, const fl
   s.slope = slopes ? slopes[h] * kLog2e : 0.f;
   return s;
 }
+// The bias where no key is ahead: linear in the column, and no conversion per key (an integer to a
+// float costs as much as an exponential); 8192 causal tokens of 16 heads of 128 355 -> 319 us.  The
+// product slope * from is rounded by 2^-24 of itself, that is of the bias 128 keys on at most, and
+// alike for all the columns.
+template <int N, bool CAP>
+__device__ __forceinline__ void bias_behind(float (&s)[N], const Scores& sc, float from) {
+  const float2 slope2 = make_float2(sc.slope, sc.slope), base2 = make_float2(-sc.slope * from, -sc.slope * from);
+  const float2 by2 = make_float2(sc.by, sc.by);
+#pragma unroll
+  for (int c = 0; c < N; c += 2) {
+    const float2 off = ptx::fma2(slope2, make_float2((float)c, (float)(c + 1)), base2);
+    const float2 z = make_float2(s[c], s[c + 1]);
+    const float2 r = CAP ? ptx::add2(z, off) : ptx::fma2(z, by2, off);
+    s[c] = r.x;
+    s[c + 1] = r.y;
+  }
+}
 template <int N, bool CAP, bool BIAS>
 __device__ __forceinline__ void score(float (&s)[N], const Scores& sc, int first) {
   if (CAP) {
@@ -289,8 +296,13 @@ __device__ __forceinline__ void score(float (&s)[N], const Scores& sc, int first
     }
   }
   if (BIAS) {
+    const float from = (float)first;      // past 2^24 a distance is rounded, by 2^-24 of itself
+    if (__all_sync(~0u, first >= N - 1)) {
+      bias_behind<N, CAP>(s, sc, from);
+    } else {
 #pragma unroll
-    for (int c = 0; c < N; ++c) s[c] = fmaf(-sc.slope, fabsf((float)(first - c)), CAP ? s[c] : s[c] * sc.by);
+      for (int c = 0; c < N; ++c) s[c] = fmaf(-sc.slope, fabsf(from - (float)c), CAP ? s[c] : s[c] * sc.by);
+    }
   }
 }
 
@@ -315,7 +327,7 @@ __device__ __forceinline__ void weigh(const float (&s)[kTile], float by, float m
       for (int i = 0; i < 32; i += 2) {
         float2 z = make_float2(s[c + i], s[c + i + 1]);
         z = SCALED ? ptx::add2(z, mu2) : ptx::fma2(z, by2, mu2);
-        const float2 x = (i >> 1) % kFmaEvery == 1 ? ex2_fma(z) : make_float2(ex2(z.x), ex2(z.y));
+        const float2 x = make_float2(ex2(z.x), ex2(z.y));
         const int k = (i >> 1) & 1;
         add[k] = ptx::add2(add[k], x);
         w[i >> 1] = pack2<BF16>(x.x, x.y);
@@ -335,10 +347,7 @@ template <int DP, bool BF16, bool SCALED>
 __device__ __forceinline__ void weigh_tile(const float (&s)[kTile], float by, bool first, float* m, float* sum,
                                            float* packed_sum, bool both, uint32_t s_tmem, uint32_t o_tmem,
                                            uint64_t* ready, int lane) {
-  float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-  for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
-  float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  float mt = max_of(s);
   if (!SCALED) mt *= by;
   follow_maximum<DP>(mt, first, m, sum, packed_sum, o_tmem);
   if (both) weigh<BF16, SCALED, true>(s, by, *m, sum, packed_sum, s_tmem, ready, lane);

@@ -552,11 +552,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
             if (CAP || BIAS) {
               // cached tokens: none is ahead.  (A place past 2^24 is rounded, its distance by as little.)
               score<32, CAP, false>(s, sc, 0);
-              if (BIAS) {
-#pragma unroll
-                for (int c = 0; c < 32; ++c)
-                  s[c] = fmaf(-sc.slope, (float)(at - c) + (float)depth, CAP ? s[c] : s[c] * by);
-              }
+              if (BIAS) bias_behind<32, CAP>(s, sc, (float)at + (float)depth);
               if (BIAS && at < 32) {     // drafted tokens stand where their depth says, not their place
 #pragma unroll
                 for (int c = 0; c < 32; ++c) {
@@ -571,10 +567,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
 #pragma unroll
               for (int c = 0; c < 32; ++c) s[c] = (see >> c) & 1u ? s[c] : -INFINITY;
             }
-            float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-            for (int c = 4; c < 32; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
-            mt = fmaxf(mt, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+            mt = fmaxf(mt, max_of(s));
             if (chunks > 1 && (CAP || BIAS || hide)) {
               ptx::tmem_st_32x16(s_tmem + c0, reinterpret_cast<uint32_t*>(s));
               ptx::tmem_st_32x16(s_tmem + c0 + 16, reinterpret_cast<uint32_t*>(s) + 16);
