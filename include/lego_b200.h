@@ -440,9 +440,12 @@ int32_t lego_rotary(const lego_rotary_t* desc, const void* x0, const void* x1, v
  * aligned; head_dim a multiple of 8 up to 128.  No counterpart in the reference.
  *
  * The backward pass takes o, o_low (or NULL), lse as the forward pass left them and d_o (contiguous like q)
- * and writes contiguous dq, dk, dv: same bits on every run, no atomics.
+ * and writes contiguous dq, dk, dv: same bits on every run, no sum by atomics.
  * workspace: lego_attention_workspace_bytes() bytes of device memory, 16-byte aligned, of
- * any contents, that no other call in flight uses.                              */
+ * any contents, that no other call in flight uses.
+ * LEGO_ERR_SIZE: a length above 2^30, more than 65535 query heads, batch * q_heads above 2^25,
+ * 2^31 or more tiles of 128 tokens and heads, |scale| or softcap of 1e30 or more, or a quotient of
+ * the two that large (what is made of them has to stay finite).                 */
 typedef struct lego_attention {
   int32_t dtype, causal;
   int64_t batch, q_len, k_len, q_heads, k_heads, head_dim;
@@ -473,7 +476,9 @@ int32_t lego_attention_bwd(const lego_attention_t* desc, const void* q, const vo
  * [0, pages), or a place at or past max_pages * page_size, holds nothing (its keys are
  * hidden).  Scores as in lego_attention.  q [batch, drafted, q_heads, head_dim]; o
  * contiguous.  Strides in elements (batch, token, head / page, slot, head), multiples of 8,
- * pointers 16-byte aligned; head_dim a multiple of 8 up to 128.  workspace as above.
+ * pointers 16-byte aligned; head_dim a multiple of 8 up to 128.  workspace as above, of
+ * lego_tree_attention_workspace_bytes().  LEGO_ERR_SIZE besides: max_pages * page_size above 2^30,
+ * or 2^31 or more tiles of 128 places, over all sequences, key heads and tiles of 128 rows.
  * No counterpart in the reference.                                              */
 typedef struct lego_tree_attention {
   int32_t dtype, reserved;
