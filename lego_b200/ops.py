@@ -1120,7 +1120,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     shows nothing and whose values are not used.  A query that sees no key gets zeros.
 
     Differentiable in q, k and v.  ``return_lse``: also the logarithm of each row's sum, float32
-    ``[B, Hq, Sq]`` (no gradient).  A key hidden from one query but seen by another has to be finite."""
+    ``[B, Hq, Sq]`` (no gradient).  Tokens that are not padding have to be finite, whoever sees them: a
+    hidden one meets a weight of zero.  To capture a backward pass into a CUDA graph take
+    ``torch.autograd.grad``, or keep no eager graph of the same leaves alive."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         o, lse = LEGOAttention.apply(q, k, v, causal, prefix, documents, softcap, slopes, scale)
     else:
