@@ -176,6 +176,22 @@ def test_small_and_large_gradients_in_fp16():
     check(q, k, (v.float() * 200).half(), do, causal=True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_capped_gradients_lose_little_more_than_their_rounding(dtype):
+    """Scores of deviation 4 under a cap, documents of many lengths.  In the norm over all values, dq's own
+    rounding is 1; the rounding of the weights in the forward pass, which reaches dq through o, makes it 1.07; score
+    gradients of 16 bits would make it 1.46 (sums of independent roundings, from the formulas in 64 bits)."""
+    q, k, v, do = make(28, 1, 2000, 2000, 4, 4, 64, dtype)
+    q = (4 * q.float()).to(dtype)
+    docs = documents_of(9, 1, 2000, "packed")
+    how = dict(causal=True, documents=docs, softcap=30.0)
+    o, lse, low = ops._attention_fwd(q, k, v, True, None, docs, 30.0, None, None, True)
+    dq, _, _ = ops.attention_bwd(do, q, k, v, o, lse, o_low=low, **how)
+    want = R.attention(q, k, v, do, **how)["dq"][0]
+    least = (want.to(dtype).double() - want).norm()
+    assert (dq.double() - want).norm() <= 1.25 * least
+
+
 def test_gradient_against_differences():
     """<dO, O(x + h r) - O(x - h r)> / 2h in 64 bits is the kernel's gradient along r, to the bound of its rounding."""
     q, k, v, do = make(13, 1, 90, 120, 2, 1, 64, torch.float16)
