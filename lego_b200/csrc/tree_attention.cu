@@ -23,8 +23,10 @@
 // at a piece's end.
 //
 // Warps: 0-3 and 4-7 weights of the even and the odd tiles of a piece (each with its own m, sum
-// and O, put together at the piece's end), 8-11 loads, 12 MMA issue (13-15 fill up their
-// warpgroup).  Each loading lane looks up the place of one row of a tile.  Tiles come by TMA, in
+// and O, put together at the piece's end), 8-11 loads of the cache, 12 MMA issue, 13-15 the run's
+// pieces with their trees and queries, one piece ahead (64 sequences 261 -> 257 us, 2 x 131072 tokens
+// 157 -> 156, against loads that did this in between; their waits are long suspends, polling took
+// slots from capped weights).  Each loading lane looks up the place of one row of a tile.  Tiles come by TMA, in
 // boxes of as many rows as stand together in a page (a common divisor of the page size and 32, at
 // least 8); pages of other sizes come as 16-byte copies.  Keys that do not exist (past the end, of
 // a page number outside the cache, of an unused drafted token) are hidden by a mask that the loads
@@ -234,8 +236,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(ptx::smem_u32(&sh->piece_full[t]), 1);
-      ptx::mbar_init(ptx::smem_u32(&sh->q_full[t]), 128);          // every loading thread's copies
-      ptx::mbar_init(ptx::smem_u32(&sh->q_empty[t]), 1 + 8 + 3);   // the MMAs; the warps done with the piece and its tree
+      ptx::mbar_init(ptx::smem_u32(&sh->q_full[t]), 96);           // the copies of three warps' threads
+      ptx::mbar_init(ptx::smem_u32(&sh->q_empty[t]), 1 + 8 + 4);   // the MMAs; the warps done with the piece and its tree
       ptx::mbar_init(ptx::smem_u32(&sh->s_full[t]), 1);
       ptx::mbar_init(ptx::smem_u32(&sh->p_full[t]), 4);
       ptx::mbar_init(ptx::smem_u32(&sh->o_full[t]), 1);
@@ -353,6 +355,63 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
         }
         pos -= 2;     // the last turn had no K
       }
+    } else {
+      // ---------------- pieces (warp 13) and their queries ----------------
+      constexpr int CH = DP / 8, PER = 32 / CH;    // 16-byte pieces of a row; rows per instruction
+      const int chunk = lane % CH, first_row = (warp - 13) * PER + lane / CH;
+      const bool chunk_real = chunk * 8 < p.dim;
+      int next_b = sh->start_b, next_hr = sh->start_hr, next_tile = sh->start_tile, left = sh->start_left;
+      int len = warp == 13 && left > 0 ? p.lengths[next_b] : 0;
+      bool ok = true;
+      auto bounded = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
+        if (lane == 0) ok = ptx::mbar_wait_bounded<true>(ptx::smem_u32(bar), parity, abort_flag, kAttnWait);
+        ok = __shfl_sync(~0u, ok ? 1 : 0, 0);
+        if (!ok && lane == 0) attn_fail(p.status, abort_flag, code);
+        return ok;
+      };
+      for (int n = 0; ok; ++n) {
+        if (warp == 13) {
+          if (!bounded(&sh->q_empty[n & 1], ((n >> 1) & 1) ^ 1, 0x710000u)) break;
+          pc.b = -1;
+          if (left > 0) {
+            pc.b = next_b;
+            pc.hk = next_hr / p.row_tiles;
+            pc.rt = next_hr - pc.hk * p.row_tiles;
+            pc.len = len;
+            pc.places = tree_places(p, len);
+            pc.first = next_tile;
+            const int tiles = tiles_of(pc.places);
+            pc.last = left < tiles - next_tile ? next_tile + left : tiles;
+            left -= pc.last - pc.first;
+            next_tile = 0;
+            grow_tree(p, pc.b, &sh->tree[n & 1], lane);
+          }
+          if (lane == 0) sh->piece[n & 1] = pc;
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->piece_full[n & 1]));
+        } else {
+          if (!bounded(&sh->piece_full[n & 1], (n >> 1) & 1, 0x710004u)) break;
+          pc = sh->piece[n & 1];
+        }
+        if (pc.b < 0) break;
+        const int per_copy = kTile / p.copies;
+#pragma unroll 4
+        for (int r = first_row; r < kTile; r += 3 * PER) {
+          const int row = pc.rt * kTile + (r & (per_copy - 1));
+          const bool copy = row < p.rows && chunk_real;
+          const int t = (int)fd_div((uint32_t)row, p.by_group), h = pc.hk * p.group + row - t * p.group;
+          const uint16_t* src = p.q + pc.b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2] + chunk * 8;
+          ptx::cp_async_16(q_smem + (n & 1) * TILE + (chunk >> 3) * kBoxBytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4),
+                           copy ? src : p.q, copy);
+        }
+        ptx::cp_async_arrive(ptx::smem_u32(&sh->q_full[n & 1]));
+        if (warp == 13 && ++next_hr == p.k_heads * p.row_tiles && left > 0) {
+          next_hr = 0;
+          do len = p.lengths[++next_b];      // units are left, so a sequence with tiles follows
+          while (len < 0);
+        }
+      }
+      ptx::cp_async_wait_all();
     }
   } else if (warp >= 8) {
     ptx::regs_less<kTreeOtherRegs>();
@@ -368,52 +427,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
       if (!ok && lane == 0) attn_fail(p.status, abort_flag, code);
       return ok;
     };
-    // warp 8 walks the run and publishes its pieces
-    int next_b = sh->start_b, next_hr = sh->start_hr, next_tile = sh->start_tile, left = sh->start_left;
-    int len = left > 0 ? p.lengths[next_b] : 0;
     for (int n = 0; ok; ++n) {
-      if (w == 0) {
-        if (!bounded(&sh->q_empty[n & 1], ((n >> 1) & 1) ^ 1, 0x710000u)) break;
-        pc.b = -1;
-        if (left > 0) {
-          pc.b = next_b;
-          pc.hk = next_hr / p.row_tiles;
-          pc.rt = next_hr - pc.hk * p.row_tiles;
-          pc.len = len;
-          pc.places = tree_places(p, len);
-          pc.first = next_tile;
-          const int tiles = tiles_of(pc.places);
-          pc.last = left < tiles - next_tile ? next_tile + left : tiles;
-          left -= pc.last - pc.first;
-          next_tile = 0;
-          if (++next_hr == p.k_heads * p.row_tiles && left > 0) {
-            next_hr = 0;
-            do len = p.lengths[++next_b];      // units are left, so a sequence with tiles follows
-            while (len < 0);
-          }
-          grow_tree(p, pc.b, &sh->tree[n & 1], lane);
-        }
-        if (lane == 0) sh->piece[n & 1] = pc;
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->piece_full[n & 1]));
-      } else {
-        if (!bounded(&sh->piece_full[n & 1], (n >> 1) & 1, 0x710002u)) break;
-        pc = sh->piece[n & 1];
-      }
+      if (!bounded(&sh->piece_full[n & 1], (n >> 1) & 1, 0x710002u)) break;
+      pc = sh->piece[n & 1];
       if (pc.b < 0) break;
       const Tree* tree = &sh->tree[n & 1];
-      const int per_copy = kTile / p.copies;
-#pragma unroll 4
-      for (int i = 0; i < 32; i += PER) {
-        const int r = w * 32 + i + sub, row = pc.rt * kTile + (r & (per_copy - 1));
-        const bool copy = row < p.rows && chunk_real;
-        const int t = (int)fd_div((uint32_t)row, p.by_group), h = pc.hk * p.group + row - t * p.group;
-        const uint16_t* src = p.q + pc.b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2] + chunk * 8;
-        ptx::cp_async_16(q_smem + (n & 1) * TILE + (chunk >> 3) * kBoxBytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4),
-                         copy ? src : p.q, copy);
-      }
-      ptx::cp_async_arrive(ptx::smem_u32(&sh->q_full[n & 1]));
-
       const int places = pc.places;
       const int* table = p.table + pc.b * p.table_stride;
       // page number of this lane's row of a tile, as the table has it; -1: past the end
@@ -484,7 +502,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
           ptx::cp_async_arrive(full);
         }
       }
-      if (w > 0 && lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->q_empty[n & 1]));
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->q_empty[n & 1]));
     }
     ptx::cp_async_wait_all();
     if (*abort_flag && lane == 0) {      // leave no copy in flight: a tenth of a second for each slot at most
