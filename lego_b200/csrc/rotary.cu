@@ -33,24 +33,36 @@ struct RotArgs {
   FastDiv by_units, by_heads;      // units of a head; heads of both tensors
 };
 
-// VEC values of T at once; VEC = 16 / sizeof(T) for aligned tensors, 1 otherwise.
-template <typename T, int VEC> struct Pack { T v[VEC]; };
+// VEC values of T at once: 16 bytes where the tensors' alignment and the borders inside a head allow it, else
+// 8 bytes of a 16-bit type (heads of 80 turned by half: 102 -> 48 us for 2 x 8192 tokens x 40 heads), else one value.
+template <typename T, int VEC> struct alignas(VEC * sizeof(T)) Pack { T v[VEC]; };
 template <typename T, int VEC>
 __device__ __forceinline__ Pack<T, VEC> load_pack(const T* p) {
   Pack<T, VEC> r;
   if constexpr (VEC * sizeof(T) == 16) *reinterpret_cast<uint4*>(&r) = __ldcs(reinterpret_cast<const uint4*>(p));
+  else if constexpr (VEC * sizeof(T) == 8) *reinterpret_cast<uint2*>(&r) = __ldcs(reinterpret_cast<const uint2*>(p));
   else r.v[0] = *p;
   return r;
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, VEC>& r) {
   if constexpr (VEC * sizeof(T) == 16) __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&r));
+  else if constexpr (VEC * sizeof(T) == 8) __stcs(reinterpret_cast<uint2*>(p), *reinterpret_cast<const uint2*>(&r));
   else *p = r.v[0];
 }
 
-// A unit of work is VEC values of the rotated part and their partners (half: two packs;
-// interleaved: one pack of whole pairs, or the two values of one pair when VEC is 1), or
-// one pack of the part that is copied.
+// A unit of work is two packs of VEC values, or one pack of whole pairs where neighbours turn together
+// (interleaved, VEC > 1): values of the rotated part and their partners, or of the part that is
+// copied (which ends with a pack twice where its packs are odd in number).  A thread has kRotUnits units
+// under way: all their loads, then the turns and stores; with a branch for copies before the
+// loads, heads turned by half moved 3.2 TB/s where whole ones moved 5.
+constexpr int kRotUnits = 4;
+constexpr __host__ __device__ bool rot_two_packs(bool half, int vec) { return half || vec == 1; }
+__host__ __device__ inline int rot_units(bool half, int vec, int pairs) { return rot_two_packs(half, vec) ? pairs / vec : 2 * pairs / vec; }
+__host__ __device__ inline int copy_units(bool half, int vec, int values) {
+  return rot_two_packs(half, vec) ? (values / vec + 1) / 2 : values / vec;
+}
+
 template <typename T, int VEC, bool HALF>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotArgs a) {
   extern __shared__ float2 turn[];   // [token][pair] (cos, sin), scaled
@@ -81,52 +93,63 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
   }
   __syncthreads();
 
-  const int rot_units = HALF ? a.half / VEC : (VEC > 1 ? 2 * a.half / VEC : a.half);
-  const int copy_units = (a.dim - 2 * a.half) / VEC;
-  const int per_head = rot_units + copy_units;
+  constexpr bool TWO = rot_two_packs(HALF, VEC);
+  const int turned = rot_units(HALF, VEC, a.half);
+  const int per_head = turned + copy_units(HALF, VEC, a.dim - 2 * a.half);
   const int h0 = a.heads[0], heads = h0 + a.heads[1];
   const int units = nt * heads * per_head;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < units; i += kRotThreads) {
-    const int head_id = (int)fd_div((uint32_t)i, a.by_units), u = i - head_id * per_head;
-    const int t = (int)fd_div((uint32_t)head_id, a.by_heads), hh = head_id - t * heads;
-    const bool second = hh >= h0;
-    const int h = second ? hh - h0 : hh;
-    const T* x = reinterpret_cast<const T*>(second ? a.x[1] : a.x[0]) + row[second ? 1 : 0][t] +
-                 h * (second ? a.in_stride[1][2] : a.in_stride[0][2]);
-    T* y = reinterpret_cast<T*>(second ? a.y[1] : a.y[0]) + ((t0 + t) * (second ? a.heads[1] : h0) + h) * a.dim;
-    if (u >= rot_units) {
-      const int c = 2 * a.half + (u - rot_units) * VEC;
-      store_pack<T, VEC>(y + c, load_pack<T, VEC>(x + c));
-      continue;
+  for (int i0 = threadIdx.x; i0 < units; i0 += kRotUnits * kRotThreads) {
+    Pack<T, VEC> x1[kRotUnits], x2[TWO ? kRotUnits : 1];
+    T* y1[kRotUnits];
+    int c2[kRotUnits], cs_at[kRotUnits];      // from the first pack to the second; angles, -1: a copy
+#pragma unroll
+    for (int k = 0; k < kRotUnits; ++k) {
+      const int i = i0 + k * kRotThreads;
+      if (i >= units) break;
+      const int head_id = (int)fd_div((uint32_t)i, a.by_units), u = i - head_id * per_head;
+      const int t = (int)fd_div((uint32_t)head_id, a.by_heads), hh = head_id - t * heads;
+      const bool second = hh >= h0, turn_it = u < turned;
+      const int h = second ? hh - h0 : hh;
+      int c1;
+      if (TWO) {
+        const int rest = 2 * a.half + 2 * (u - turned) * VEC;
+        c1 = !turn_it ? rest : HALF ? u * VEC : 2 * u;
+        c2[k] = !turn_it ? (rest + VEC < a.dim ? VEC : 0) : HALF ? a.half : 1;
+      } else {
+        c1 = u * VEC;
+      }
+      cs_at[k] = !turn_it ? -1 : t * a.half + (TWO ? u * VEC : u * (VEC / 2));
+      const T* x = reinterpret_cast<const T*>(second ? a.x[1] : a.x[0]) + row[second ? 1 : 0][t] +
+                   h * (second ? a.in_stride[1][2] : a.in_stride[0][2]) + c1;
+      y1[k] = reinterpret_cast<T*>(second ? a.y[1] : a.y[0]) + ((t0 + t) * (second ? a.heads[1] : h0) + h) * a.dim + c1;
+      x1[k] = load_pack<T, VEC>(x);
+      if constexpr (TWO) x2[k] = load_pack<T, VEC>(x + c2[k]);
     }
-    const float2* cs = turn + t * a.half;
-    if constexpr (HALF || VEC == 1) {
-      const int p = u * VEC;
-      const int c1 = HALF ? p : 2 * p, c2 = HALF ? p + a.half : 2 * p + 1;
-      const Pack<T, VEC> x1 = load_pack<T, VEC>(x + c1), x2 = load_pack<T, VEC>(x + c2);
-      Pack<T, VEC> y1, y2;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float2 k = cs[p + e];
-        const float f1 = to_f32(x1.v[e]), f2 = to_f32(x2.v[e]);
-        from_f32(f1 * k.x - f2 * k.y, &y1.v[e]);
-        from_f32(f2 * k.x + f1 * k.y, &y2.v[e]);
-      }
-      store_pack<T, VEC>(y + c1, y1);
-      store_pack<T, VEC>(y + c2, y2);
-    } else {
-      const int p = u * (VEC / 2);
-      const Pack<T, VEC> xv = load_pack<T, VEC>(x + 2 * p);
-      Pack<T, VEC> yv;
+    for (int k = 0; k < kRotUnits; ++k) {
+      if (i0 + k * kRotThreads >= units) break;
+      if (cs_at[k] >= 0) {
+        const float2* cs = turn + cs_at[k];
+        if constexpr (TWO) {
 #pragma unroll
-      for (int e = 0; e < VEC / 2; ++e) {
-        const float2 k = cs[p + e];
-        const float f1 = to_f32(xv.v[2 * e]), f2 = to_f32(xv.v[2 * e + 1]);
-        from_f32(f1 * k.x - f2 * k.y, &yv.v[2 * e]);
-        from_f32(f2 * k.x + f1 * k.y, &yv.v[2 * e + 1]);
+          for (int e = 0; e < VEC; ++e) {
+            const float2 w = cs[e];
+            const float f1 = to_f32(x1[k].v[e]), f2 = to_f32(x2[k].v[e]);
+            from_f32(f1 * w.x - f2 * w.y, &x1[k].v[e]);
+            from_f32(f2 * w.x + f1 * w.y, &x2[k].v[e]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC / 2; ++e) {
+            const float2 w = cs[e];
+            const float f1 = to_f32(x1[k].v[2 * e]), f2 = to_f32(x1[k].v[2 * e + 1]);
+            from_f32(f1 * w.x - f2 * w.y, &x1[k].v[2 * e]);
+            from_f32(f2 * w.x + f1 * w.y, &x1[k].v[2 * e + 1]);
+          }
+        }
       }
-      store_pack<T, VEC>(y + 2 * p, yv);
+      store_pack<T, VEC>(y1[k], x1[k]);
+      if constexpr (TWO) store_pack<T, VEC>(y1[k] + c2[k], x2[k]);
     }
   }
 }
@@ -138,9 +161,11 @@ cudaError_t launch_rotary(const RotArgs& a, bool half, long long blocks, size_t 
 }
 
 template <typename T>
-cudaError_t launch_rotary_type(const RotArgs& a, bool half, bool vec, long long blocks, size_t smem, cudaStream_t s) {
-  constexpr int VEC = 16 / sizeof(T);
-  return vec ? launch_rotary<T, VEC>(a, half, blocks, smem, s) : launch_rotary<T, 1>(a, half, blocks, smem, s);
+cudaError_t launch_rotary_type(const RotArgs& a, bool half, int vec, long long blocks, size_t smem, cudaStream_t s) {
+  if (vec == (int)(16 / sizeof(T))) return launch_rotary<T, 16 / sizeof(T)>(a, half, blocks, smem, s);
+  if constexpr (sizeof(T) == 2)
+    if (vec == 4) return launch_rotary<T, 4>(a, half, blocks, smem, s);
+  return launch_rotary<T, 1>(a, half, blocks, smem, s);
 }
 
 }  // namespace
@@ -166,23 +191,26 @@ extern "C" int32_t lego_rotary(const lego_rotary_t* d, const void* x0, const voi
   RotArgs a = {};
   const void* xs[2] = {x0, x1};
   void* ys[2] = {y0, y1};
-  const int eb = d->dtype == LEGO_F32 ? 4 : 2, vec_elems = 16 / eb;
+  const int eb = d->dtype == LEGO_F32 ? 4 : 2;
   const bool half = d->pairs == LEGO_PAIRS_HALF;
-  // whole 16-byte packs: every row of a head starts on such a boundary and no pack holds the
-  // border between the halves, or between the rotated and the copied part
-  bool vec = d->head_dim % vec_elems == 0 && (half ? d->rotary_dim / 2 : d->rotary_dim) % vec_elems == 0;
+  // whole packs: every row of a head starts on a pack's boundary and no pack holds the border
+  // between the halves, or between the rotated and the copied part
+  int64_t borders = d->head_dim | (half ? d->rotary_dim / 2 : d->rotary_dim);      // in values; their common powers of two count
+  uint64_t places = 0;                                                             // in bytes
   for (int i = 0; i < 2; ++i) {
     a.x[i] = xs[i];
     a.y[i] = ys[i];
     a.heads[i] = (int)d->heads[i];
     if (!d->heads[i]) continue;
     if (((uintptr_t)xs[i] | (uintptr_t)ys[i]) & (uintptr_t)(eb - 1)) return LEGO_ERR_ALIGN;
-    vec = vec && (((uintptr_t)xs[i] | (uintptr_t)ys[i]) & 15) == 0;
+    places |= (uintptr_t)xs[i] | (uintptr_t)ys[i];
     for (int k = 0; k < 3; ++k) {
       a.in_stride[i][k] = d->stride[i][k];
-      vec = vec && d->stride[i][k] % vec_elems == 0;
+      borders |= d->stride[i][k];
     }
   }
+  auto fits = [&](int values) { return borders % values == 0 && places % (uint64_t)(values * eb) == 0; };
+  const int vec = fits(16 / eb) ? 16 / eb : eb == 2 && fits(4) ? 4 : 1;
   a.positions = positions;
   a.pos_stride[0] = d->position_stride[0];
   a.pos_stride[1] = d->position_stride[1];
@@ -196,9 +224,7 @@ extern "C" int32_t lego_rotary(const lego_rotary_t* d, const void* x0, const voi
   a.scale = d->scale;
   a.per_block = 1;
   while (a.per_block < kRotMaxTokens && a.tokens / (2 * a.per_block) >= 148 * 8) a.per_block *= 2;
-  const int vec_values = vec ? vec_elems : 1;
-  const int rot_units = half ? a.half / vec_values : (vec ? 2 * a.half / vec_values : a.half);
-  a.by_units = make_fastdiv((uint64_t)(rot_units + (a.dim - 2 * a.half) / vec_values));
+  a.by_units = make_fastdiv((uint64_t)(rot_units(half, vec, a.half) + copy_units(half, vec, a.dim - 2 * a.half)));
   a.by_heads = make_fastdiv((uint64_t)(a.heads[0] + a.heads[1]));
   const long long blocks = (a.tokens + a.per_block - 1) / a.per_block;
   if (blocks > 0x7fffffffLL) return LEGO_ERR_SIZE;

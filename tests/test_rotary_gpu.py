@@ -101,6 +101,20 @@ def test_strides_and_alignment():
     assert torch.equal(ops.rotary(q, None, every_other, f), ops.rotary(q, None, every_other.clone(), f))
 
 
+@pytest.mark.parametrize("pairs", ["half", "interleaved"])
+@pytest.mark.parametrize("D,R", [(64, 64), (64, 32), (80, 40), (88, 8), (24, 16), (28, 20)])
+def test_every_width_of_loads(pairs, D, R):
+    """Starts on 2, 4, 8 and 16 byte boundaries, part of the head copied: the same bits as from a fresh tensor."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    pos, f = torch.arange(9, device="cuda"), ops.rotary_frequencies(R, device="cuda")
+    for dtype in (torch.bfloat16, torch.float32):
+        for off in (1, 2, 4, 8):
+            x = torch.randn(2 * 9 * 3 * D + off, generator=g, device="cuda").to(dtype)[off:].view(2, 9, 3, D)
+            y = ops.rotary(x, None, pos, f, pairs=pairs)
+            assert torch.equal(y, ops.rotary(x.clone(), None, pos, f, pairs=pairs))
+            assert torch.equal(y[..., R:], x[..., R:])
+
+
 def test_graph_stream_host_and_empty():
     x = torch.randn(1, 40, 2, 64, device="cuda").bfloat16()
     pos, f = torch.arange(40, device="cuda"), ops.rotary_frequencies(64, device="cuda")
