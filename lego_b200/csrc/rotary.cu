@@ -65,13 +65,19 @@ __host__ __device__ inline int copy_units(bool half, int vec, int values) {
 
 template <typename T, int VEC, bool HALF>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotArgs a) {
-  extern __shared__ float2 turn[];   // [token][pair] (cos, sin), scaled
+  extern __shared__ __align__(16) float2 turn[];   // [token][pair in the order below] (cos, sin), scaled
   __shared__ long long row[2][kRotMaxTokens];      // where a token's heads start in either input
   ptx::launch_dependents();
   ptx::grid_dependency_wait();
   const long long t0 = (long long)blockIdx.x * a.per_block;
   const int nt = (int)(a.tokens - t0 < a.per_block ? a.tokens - t0 : a.per_block);
 
+  // A unit's pairs, two at a time, stand as far apart as there are units: the lanes of a warp then read
+  // neighbouring 16 bytes, where a unit's own would be in four lanes' way (2 x 8192 tokens x 40 heads
+  // of 128, bf16: 65 -> 55.5 us, 6.05 TB/s).
+  constexpr bool TWO = rot_two_packs(HALF, VEC);
+  constexpr int PAIRS = TWO ? VEC : VEC / 2;
+  const int turned = rot_units(HALF, VEC, a.half);
   __shared__ long long place[kRotMaxTokens];
   if (threadIdx.x < nt) {
     const long long b = (t0 + threadIdx.x) / a.length, s = (t0 + threadIdx.x) - b * a.length;
@@ -89,12 +95,12 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
     turns -= rint(turns);
     float sn, cs;
     sincospif(2.0f * (float)turns, &sn, &cs);
-    turn[i] = make_float2(a.scale * cs, a.scale * (a.inverse ? -sn : sn));
+    const int u = p / PAIRS, e = p - u * PAIRS;
+    turn[t * a.half + (PAIRS > 1 ? ((e >> 1) * turned + u) * 2 + (e & 1) : p)] =
+        make_float2(a.scale * cs, a.scale * (a.inverse ? -sn : sn));
   }
   __syncthreads();
 
-  constexpr bool TWO = rot_two_packs(HALF, VEC);
-  const int turned = rot_units(HALF, VEC, a.half);
   const int per_head = turned + copy_units(HALF, VEC, a.dim - 2 * a.half);
   const int h0 = a.heads[0], heads = h0 + a.heads[1];
   const int units = nt * heads * per_head;
@@ -118,7 +124,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
       } else {
         c1 = u * VEC;
       }
-      cs_at[k] = !turn_it ? -1 : t * a.half + (TWO ? u * VEC : u * (VEC / 2));
+      cs_at[k] = !turn_it ? -1 : t * a.half + (PAIRS > 1 ? 2 * u : u);
       const T* x = reinterpret_cast<const T*>(second ? a.x[1] : a.x[0]) + row[second ? 1 : 0][t] +
                    h * (second ? a.in_stride[1][2] : a.in_stride[0][2]) + c1;
       y1[k] = reinterpret_cast<T*>(second ? a.y[1] : a.y[0]) + ((t0 + t) * (second ? a.heads[1] : h0) + h) * a.dim + c1;
@@ -130,22 +136,24 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
       if (i0 + k * kRotThreads >= units) break;
       if (cs_at[k] >= 0) {
         const float2* cs = turn + cs_at[k];
-        if constexpr (TWO) {
+        float2 w[PAIRS];
+        if constexpr (PAIRS > 1) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float2 w = cs[e];
-            const float f1 = to_f32(x1[k].v[e]), f2 = to_f32(x2[k].v[e]);
-            from_f32(f1 * w.x - f2 * w.y, &x1[k].v[e]);
-            from_f32(f2 * w.x + f1 * w.y, &x2[k].v[e]);
+          for (int e = 0; e < PAIRS; e += 2) {
+            const float4 z = *reinterpret_cast<const float4*>(cs + e * turned);
+            w[e] = make_float2(z.x, z.y);
+            w[e + 1] = make_float2(z.z, z.w);
           }
         } else {
+          w[0] = cs[0];
+        }
 #pragma unroll
-          for (int e = 0; e < VEC / 2; ++e) {
-            const float2 w = cs[e];
-            const float f1 = to_f32(x1[k].v[2 * e]), f2 = to_f32(x1[k].v[2 * e + 1]);
-            from_f32(f1 * w.x - f2 * w.y, &x1[k].v[2 * e]);
-            from_f32(f2 * w.x + f1 * w.y, &x1[k].v[2 * e + 1]);
-          }
+        for (int e = 0; e < PAIRS; ++e) {
+          T* v1 = TWO ? &x1[k].v[e] : &x1[k].v[2 * e];
+          T* v2 = TWO ? &x2[TWO ? k : 0].v[e] : &x1[k].v[2 * e + 1];
+          const float f1 = to_f32(*v1), f2 = to_f32(*v2);
+          from_f32(f1 * w[e].x - f2 * w[e].y, v1);
+          from_f32(f2 * w[e].x + f1 * w[e].y, v2);
         }
       }
       store_pack<T, VEC>(y1[k], x1[k]);
