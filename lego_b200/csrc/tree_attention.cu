@@ -33,6 +33,11 @@
 // leave with the tile, and their values, which may be NaN and must not meet a zero weight, are
 // zeros in shared memory: a box past the cache reads as zeros, other rows are cleared by the
 // loading warp before it hands the tile on.
+//
+// Measured: 64 sequences of 1024 .. 8192 tokens x 32/8 heads of 128, bf16, one token 257 us (5.1 TB/s); 8 of 8192 ..
+// 65536 tokens 260 us (5.8, what a plain sum reads here: the difference is the change of sequence);
+// 2 x 131072 tokens x 64 rows with a bias 156 us (4.7); 8 x 16384 x 37 tokens of 2 heads with a cap 99 us, bound by
+// the cap's arithmetic.  Slower: scores and weights of one copy in registers (drafts 95 -> 104 us).
 #include <cuda.h>
 
 #include "attention.cuh"
