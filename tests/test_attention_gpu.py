@@ -239,6 +239,20 @@ def test_autograd_through_the_public_call():
     assert ops.attention(q, k, v, return_lse=True)[1].grad_fn is None
 
 
+def test_gradients_of_gradients_are_refused():
+    """With a graph of the backward pass its results are the same, and going through it raises."""
+    q, k, v, do = make(29, 1, 40, 40, 2, 1, 64, torch.bfloat16)
+    pos, f = torch.arange(40, device="cuda"), ops.rotary_frequencies(64, device="cuda")
+    for x in (q, k, v):
+        x.requires_grad_()
+    for call in (lambda: ops.attention(q, k, v, causal=True), lambda: ops.rotary(q, None, pos, f)):
+        plain, = torch.autograd.grad(call(), q, do)
+        once, = torch.autograd.grad(call(), q, do, create_graph=True)
+        assert torch.equal(plain, once) and not plain.requires_grad
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(once.float().sum(), q)
+
+
 def test_same_bits_every_run_and_on_another_stream():
     q, k, v, do = make(15, 2, 700, 700, 4, 1, 128, torch.bfloat16)
     docs = documents_of(9, 2, 700, "packed")
