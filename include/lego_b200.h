@@ -432,7 +432,8 @@ int32_t lego_rotary(const lego_rotary_t* desc, const void* x0, const void* x1, v
  * (prefix, documents NULL: no such condition; documents needs q_len <= k_len; document
  * numbers may come in any order, runs of equal ones are what makes the call fast).  A query
  * that sees nothing gets zeros and lse = -inf, and no gradient passes it.  Values of keys
- * and queries with a negative document are not used at all, be they NaN.
+ * and queries with a negative document are not used at all, be they NaN; the others have to
+ * be finite, also where a query does not see them (their weight is zero, but counts).
  * o: contiguous like q; lse: dev float[batch, q_heads, q_len], the natural logarithm of the
  * sum of exp(s).  o_low (nullable, like o): what the rounding of o to its type left over, in
  * that type; given to the backward pass it keeps the gradients of rows with one large weight

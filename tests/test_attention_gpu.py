@@ -269,6 +269,32 @@ def test_same_bits_every_run_and_on_another_stream():
         assert all(torch.equal(a, b) for a, b in zip(first, got))
 
 
+def test_two_streams_at_once():
+    """Calls of two streams that overlap: each has its own workspace and gives the bits it gives alone."""
+    jobs = []
+    for n, (shape, how) in enumerate((((2, 900, 900, 4, 2, 64), dict(causal=True, softcap=20.0)),
+                                      ((1, 70, 5000, 2, 1, 128), dict(causal=True)))):
+        x = make(40 + n, *shape, torch.float16 if n else torch.bfloat16)
+        jobs.append((x, how, torch.cuda.Stream()))
+
+    def once(x, how):
+        q, k, v, do = x
+        o, lse = ops.attention_fwd(q, k, v, **how)
+        return (o, lse, *ops.attention_bwd(do, q, k, v, o, lse, **how))
+
+    alone = [once(x, how) for x, how, _ in jobs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for n, (x, how, stream) in enumerate(jobs):
+            with torch.cuda.stream(stream):
+                got[n].append(once(x, how))
+    torch.cuda.synchronize()
+    for n in range(2):
+        assert all(torch.equal(a, b) for out in got[n] for a, b in zip(alone[n], out))
+    assert ops.device_status() == 0
+
+
 def test_captured_and_replayed():
     """Forward and backward in a graph, replayed with new values in the same buffers, two graphs in turn."""
     shapes = [(1, 200, 200, 2, 1, 64), (2, 140, 300, 4, 2, 128)]
