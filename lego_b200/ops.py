@@ -859,8 +859,14 @@ def _check_int32(t: torch.Tensor, name: str, shape) -> None:
 def _check_slopes(t: torch.Tensor, heads: int) -> None:
     if t.dtype != torch.float32 or t.shape != (heads,):
         raise ValueError(f"slopes must be float32 [{heads}], got {t.dtype} {list(t.shape)}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError("slopes are constants of the bias: no gradient is computed for them")
+
+
+def _check_constants(**given) -> None:
+    """Refuses what takes no gradient and asks for one.  Called before an autograd function is entered:
+    inside its forward pass the grad mode is off."""
+    for name, t in given.items():
+        if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} is a constant of the operator: no gradient is computed for it")
 
 
 def _optional(t: Optional[torch.Tensor], dev: torch.device) -> Optional[torch.Tensor]:
@@ -960,6 +966,11 @@ def _first_order(backward):
 class LEGORotary(torch.autograd.Function):
     """``LEGORotary.apply(q, k, positions, freqs, pairs, scale)``; ``k`` may be None."""
 
+    @classmethod
+    def apply(cls, q, k, positions, freqs, pairs, scale):
+        _check_constants(freqs=freqs, scale=scale)
+        return super().apply(q, k, positions, freqs, pairs, scale)
+
     @staticmethod
     def forward(ctx, q, k, positions, freqs, pairs, scale):
         ctx.set_materialize_grads(False)
@@ -983,11 +994,12 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     pair ``p`` of the first ``2 len(freqs)`` values of every head by the angle ``position * freqs[p]``
     (``rotary_frequencies``), the rest copied.  ``pairs``: ``"half"`` pairs value p with value p + len(freqs),
     ``"interleaved"`` 2p with 2p + 1.  ``positions``: int32 or int64 ``[B, S]`` or ``[S]``.  ``scale``
-    multiplies the turned values.  Differentiable in q and k.  Returns ``(q, k)``, or q alone when
+    multiplies the turned values.  Differentiable in q and k (``freqs`` and ``scale`` are constants).  Returns ``(q, k)``, or q alone when
     ``k`` is None.  float16, bfloat16 or float32, any strides with a contiguous last axis."""
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         out = LEGORotary.apply(q, k, positions, freqs, pairs, scale)
         return out[0] if k is None else out
+    _check_constants(freqs=freqs, scale=scale)
     out = _rotary([q] if k is None else [q, k], positions, freqs, pairs, scale, False)
     return out[0] if k is None else tuple(out)
 
@@ -1062,6 +1074,7 @@ def _attention_fwd(q, k, v, causal, prefix, documents, softcap, slopes, scale, l
 
 def attention_fwd(q, k, v, causal=False, prefix=None, documents=None, softcap=0.0, slopes=None, scale=None):
     """Attention forward: ``(o, lse)``, see ``attention``; lse is float32 ``[B, Hq, Sq]``."""
+    _check_constants(slopes=slopes, softcap=softcap, scale=scale)
     return _attention_fwd(q, k, v, causal, prefix, documents, softcap, slopes, scale, False)[:2]
 
 
@@ -1070,6 +1083,7 @@ def attention_bwd(do, q, k, v, o, lse, causal=False, prefix=None, documents=None
     """Attention backward from what ``attention_fwd`` took and gave: ``(dq, dk, dv)``, contiguous,
     the same bits on every run.  ``o_low``: what the rounding of o left, as ``LEGOAttention`` keeps it;
     without it the gradients of rows with one large weight carry that rounding too."""
+    _check_constants(slopes=slopes, softcap=softcap, scale=scale)
     dev, d, keep = _attention_desc(q, k, v, causal, prefix, documents, softcap, slopes, scale)
     _same_device(do, o, lse, o_low, keep[0])
     B, Sq, Hq, _ = q.shape
@@ -1097,6 +1111,11 @@ def attention_bwd(do, q, k, v, o, lse, causal=False, prefix=None, documents=None
 
 class LEGOAttention(torch.autograd.Function):
     """``LEGOAttention.apply(q, k, v, causal, prefix, documents, softcap, slopes, scale)`` -> ``(o, lse)``."""
+
+    @classmethod
+    def apply(cls, q, k, v, causal, prefix, documents, softcap, slopes, scale):
+        _check_constants(slopes=slopes, softcap=softcap, scale=scale)
+        return super().apply(q, k, v, causal, prefix, documents, softcap, slopes, scale)
 
     @staticmethod
     def forward(ctx, q, k, v, causal, prefix, documents, softcap, slopes, scale):
@@ -1130,7 +1149,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     ``[B, Sk]``): only keys of the query's own document; negative numbers mark padding, which sees and
     shows nothing and whose values are not used.  A query that sees no key gets zeros.
 
-    Differentiable in q, k and v.  ``return_lse``: also the logarithm of each row's sum, float32
+    Differentiable in q, k and v (``slopes``, ``softcap`` and ``scale`` are constants).  ``return_lse``: also the logarithm of each row's sum, float32
     ``[B, Hq, Sq]`` (no gradient).  Tokens that are not padding have to be finite, whoever sees them: a
     hidden one meets a weight of zero.  To capture a backward pass into a CUDA graph take
     ``torch.autograd.grad``, or keep no eager graph of the same leaves alive."""
@@ -1174,6 +1193,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         raise ValueError("page_table must be int32 [B, pages of a sequence], the cache must not be empty")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise ValueError("tree_attention has no gradient: call it under torch.no_grad()")
+    _check_constants(slopes=slopes, softcap=softcap, scale=scale)
     _check_int32(page_table, "page_table", (B, page_table.shape[1]))
     _check_int32(lengths, "lengths", (B,))
     if parents is not None:

@@ -155,3 +155,43 @@ def test_frequencies():
                 dict(dim=8, scaling="bands", low=4.0, high=4.0), dict(dim=8, scaling="bands", original_length=0)):
         with pytest.raises(ValueError):
             ops.rotary_frequencies(**bad)
+
+
+LEARNED = torch.ones(4, requires_grad=True)
+
+
+@pytest.mark.parametrize("given", ["slopes", "scale", "softcap"])
+@pytest.mark.parametrize("learns", [(), (0,), (1,), (0, 1, 2)])
+def test_a_learned_constant_of_attention_is_refused(given, learns):
+    """Whatever else learns: with a q that does the call goes through an autograd function, and one that took the
+    constant would give it no gradient."""
+    how = {given: LEARNED if given == "slopes" else LEARNED[0]}
+    args = [x.clone().requires_grad_(i in learns) for i, x in enumerate((Q, K, K))]
+    with pytest.raises(ValueError, match=given):
+        ops.attention(*args, **how)
+    with pytest.raises(ValueError, match=given):
+        ops.attention_fwd(*args, **how)
+    with pytest.raises(ValueError, match=given):
+        ops.attention_bwd(Q, *args, Q, torch.zeros(2, 4, 5), **how)
+    with pytest.raises(ValueError, match=given):
+        how = dict(dict(softcap=0.0, slopes=None, scale=None), **how)
+        ops.LEGOAttention.apply(*args, False, None, None, how["softcap"], how["slopes"], how["scale"])
+
+
+@pytest.mark.parametrize("learns", [(), (0,), (1,), (0, 1)])
+def test_learned_frequencies_are_refused(learns):
+    f = torch.ones(8, dtype=torch.float64, requires_grad=True)
+    q, k = (x.clone().requires_grad_(i in learns) for i, x in enumerate((Q, t(2, 5, 2, 64))))
+    with pytest.raises(ValueError, match="freqs"):
+        ops.rotary(q, k, ints(5), f)
+    with pytest.raises(ValueError, match="freqs"):
+        ops.LEGORotary.apply(q, None, ints(5), f, "half", 1.0)
+    with pytest.raises(ValueError, match="scale"):
+        ops.rotary(q, k, ints(5), f.detach(), scale=LEARNED[0])
+
+
+def test_learned_constants_of_tree_attention_are_refused():
+    for given in ("slopes", "scale", "softcap"):
+        with pytest.raises(ValueError, match=given):
+            ops.tree_attention(t(2, 3, 4, 64), t(9, 16, 2, 64), t(9, 16, 2, 64), ints(2, 4), ints(2),
+                               **{given: LEARNED if given == "slopes" else LEARNED[0]})
