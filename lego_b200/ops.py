@@ -25,6 +25,7 @@ import math
 from typing import List, Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _abi
 from .layout import Col, GroupBy, OrderBy, Row
@@ -861,6 +862,14 @@ def _check_slopes(t: torch.Tensor, heads: int) -> None:
         raise ValueError(f"slopes must be float32 [{heads}], got {t.dtype} {list(t.shape)}")
 
 
+def _check_tangents(*tensors) -> None:
+    """Refuses dual tensors: there is no forward-mode derivative, and a result without a tangent would be one of zero."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("no forward-mode derivative is computed: take the tensors' primals")
+
+
 def _check_constants(**given) -> None:
     """Refuses what takes no gradient and asks for one.  Called before an autograd function is entered:
     inside its forward pass the grad mode is off."""
@@ -913,6 +922,7 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[str] =
 
 def _rotary(xs, positions, freqs, pairs, scale, inverse):
     """Turned copies of ``xs`` (one or two tensors ``[B, S, H_i, D]``), one launch."""
+    _check_tangents(*xs, freqs)
     kind = {"half": _abi.PAIRS_HALF, "interleaved": _abi.PAIRS_INTERLEAVED}.get(pairs)
     if kind is None:
         raise ValueError(f"pairs must be 'half' or 'interleaved', got {pairs!r}")
@@ -968,6 +978,7 @@ class LEGORotary(torch.autograd.Function):
 
     @classmethod
     def apply(cls, q, k, positions, freqs, pairs, scale):
+        _check_tangents(q, k, freqs)
         _check_constants(freqs=freqs, scale=scale)
         return super().apply(q, k, positions, freqs, pairs, scale)
 
@@ -1006,6 +1017,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
 
 def _attention_desc(q, k, v, causal, prefix, documents, softcap, slopes, scale):
     """Checks of an attention call; ``(device, descriptor, tensors it refers to)`` with q, k, v first."""
+    _check_tangents(q, k, v, slopes)
     code = _ATTN_TYPES.get(q.dtype)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("attention takes q [B, Sq, Hq, D] and k, v [B, Sk, Hk, D]")
@@ -1083,6 +1095,7 @@ def attention_bwd(do, q, k, v, o, lse, causal=False, prefix=None, documents=None
     """Attention backward from what ``attention_fwd`` took and gave: ``(dq, dk, dv)``, contiguous,
     the same bits on every run.  ``o_low``: what the rounding of o left, as ``LEGOAttention`` keeps it;
     without it the gradients of rows with one large weight carry that rounding too."""
+    _check_tangents(do, o, lse, o_low)
     _check_constants(slopes=slopes, softcap=softcap, scale=scale)
     dev, d, keep = _attention_desc(q, k, v, causal, prefix, documents, softcap, slopes, scale)
     _same_device(do, o, lse, o_low, keep[0])
@@ -1114,6 +1127,7 @@ class LEGOAttention(torch.autograd.Function):
 
     @classmethod
     def apply(cls, q, k, v, causal, prefix, documents, softcap, slopes, scale):
+        _check_tangents(q, k, v, slopes)
         _check_constants(slopes=slopes, softcap=softcap, scale=scale)
         return super().apply(q, k, v, causal, prefix, documents, softcap, slopes, scale)
 
@@ -1174,6 +1188,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     parent is neither -1 nor an earlier token, or descends from such a one, is unused and gets zeros,
     as do all tokens of a sequence of negative length.  What the cache holds past a sequence's last
     place is not used.  No gradient."""
+    _check_tangents(q, k_cache, v_cache, slopes)
     if q.dim() != 4 or k_cache.dim() != 4 or v_cache.dim() != 4:
         raise ValueError("tree_attention takes q [B, T, Hq, D] and caches [pages, page_size, Hk, D]")
     code = _ATTN_TYPES.get(q.dtype)

@@ -195,3 +195,35 @@ def test_learned_constants_of_tree_attention_are_refused():
         with pytest.raises(ValueError, match=given):
             ops.tree_attention(t(2, 3, 4, 64), t(9, 16, 2, 64), t(9, 16, 2, 64), ints(2, 4), ints(2),
                                **{given: LEARNED if given == "slopes" else LEARNED[0]})
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_forward_mode_derivatives_are_refused(which):
+    """A dual tensor asks for a derivative without requiring a gradient: a result without a tangent would be a
+    derivative of zero."""
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        def dual(i, x):
+            return forward_ad.make_dual(x, torch.ones_like(x)) if i == which else x
+
+        refused = pytest.raises(ValueError, match="forward-mode")
+        for learns in (False, True):
+            q = Q.clone().requires_grad_(learns)
+            args = [dual(i, x) for i, x in enumerate((q, K, K, torch.zeros(4)))]
+            with refused:
+                ops.attention(*args[:3], slopes=args[3])
+            with refused:
+                ops.attention_fwd(*args[:3], slopes=args[3])
+            with refused:
+                ops.LEGOAttention.apply(*args[:3], False, None, None, 0.0, args[3], None)
+            if which < 3:
+                pair = [dual(i, x) for i, x in enumerate((q, t(2, 5, 2, 64), torch.ones(8, dtype=torch.float64)))]
+                with refused:
+                    ops.rotary(*pair[:2], ints(5), pair[2])
+                with refused:
+                    ops.LEGORotary.apply(*pair[:2], ints(5), pair[2], "half", 1.0)
+        with refused:
+            ops.attention_bwd(dual(0, Q), Q, K, K, dual(1, Q), dual(2, torch.zeros(2, 4, 5)), o_low=dual(3, Q))
+        with refused:
+            ops.tree_attention(dual(0, t(2, 3, 4, 64)), dual(1, t(9, 16, 2, 64)), dual(2, t(9, 16, 2, 64)), ints(2, 4),
+                               ints(2), slopes=dual(3, torch.zeros(4)))
