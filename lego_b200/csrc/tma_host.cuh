@@ -16,28 +16,39 @@ using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, voi
                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 inline EncodeFn encode_fn(int32_t* err) {
+  using CurrentFn = CUresult (*)(CUcontext*);
   static EncodeFn fn = nullptr;
+  static CurrentFn current = nullptr;
   static std::once_flag once;
   static int32_t status = LEGO_OK;
   std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
-    if (e != cudaSuccess) { (void)cudaGetLastError(); status = cuda_status(e); return; }
-    if (q != cudaDriverEntryPointSuccess || !p) { status = LEGO_ERR_UNSUPPORTED; return; }
-    fn = (EncodeFn)p;
+    auto find = [](const char* name) {
+      void* p = nullptr;
+      cudaDriverEntryPointQueryResult q;
+      const cudaError_t e = cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &q);
+      if (e != cudaSuccess) { (void)cudaGetLastError(); status = cuda_status(e); return (void*)nullptr; }
+      if (q != cudaDriverEntryPointSuccess || !p) { status = LEGO_ERR_UNSUPPORTED; return (void*)nullptr; }
+      return p;
+    };
+    current = (CurrentFn)find("cuCtxGetCurrent");
+    if (current) fn = (EncodeFn)find("cuTensorMapEncodeTiled");
   });
-  // The driver call wants a current context, which a thread that has made no runtime call of its own
-  // (autograd's, say) does not have: make the device's primary context current.
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess) e = cudaSetDevice(device);
-  if (e != cudaSuccess) {
-    (void)cudaGetLastError();
-    if (err) *err = cuda_status(e);
-    return nullptr;
-  }
   if (err) *err = status;
+  if (!fn) return nullptr;
+  // The driver call wants a current context, which a thread that has made no runtime call of its own
+  // (autograd's, say) does not have: it gets the device's primary one.  A context that is current, the
+  // primary one or the caller's own, stays.
+  CUcontext now = nullptr;
+  if (current(&now) != CUDA_SUCCESS || !now) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaSetDevice(device);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      if (err) *err = cuda_status(e);
+      return nullptr;
+    }
+  }
   return fn;
 }
 
