@@ -670,12 +670,11 @@ struct QueryShared {
 template <int DP, bool BF16, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const __grid_constant__ BwdArgs a) {
   constexpr int TILE = tile_bytes<DP>(), NK = query_k_stages<DP>(), NV = query_v_stages<DP>();
-  // Under a cap the scores are meant to be large: few keys carry a row, and the rounding of dS to 16 bits
-  // would take dQ's error from 1.07 times that of its own rounding to 1.46 times (1.10 against 1.53 measured,
-  // documents of 45 to 2162 tokens, scores of deviation 4).  There what the rounding left makes a
-  // product of its own: 8192 causal tokens x 16 heads of 64 backward 1120 -> 1160 us.  Without a cap it is
-  // 1.43 to 1.48 (scores of deviation 1.5, all masks), and the product costs more: 2 x 4096 causal
-  // tokens x 32/8 heads of 128 970 -> 1100 us.
+  // dS in 16 bits makes dQ's error 1.41 to 1.66 times that of its own rounding, little as scores differ (deviations
+  // of 0.3 to 8, capped or not); with what the rounding left as a product of its own it is 1.02 to 1.24 times.
+  // Under a cap the warps' arithmetic bounds this kernel and the tensor pipe waits: there the product costs 3 %
+  // (8192 causal tokens x 16 heads of 64 backward 1120 -> 1160 us) and is taken; without a cap the pipe is in
+  // its way and it costs 13 % (2 x 4096 causal tokens x 32/8 heads of 128 970 -> 1100 us).
   constexpr bool REST = CAP;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = ptx::smem_u32(smem_raw);
