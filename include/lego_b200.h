@@ -437,7 +437,7 @@ int32_t lego_rotary(const lego_rotary_t* desc, const void* x0, const void* x1, v
  * o: contiguous like q; lse: dev float[batch, q_heads, q_len], the natural logarithm of the
  * sum of exp(s).  o_low (nullable, like o): what the rounding of o to its type left over, in
  * that type; given to the backward pass it keeps the gradients of rows with one large weight
- * as exact as the others.  Strides in elements (batch, token, head), multiples of 8, pointers 16-byte
+ * as exact as the others; o is the same with and without it.  Strides in elements (batch, token, head), multiples of 8, pointers 16-byte
  * aligned; head_dim a multiple of 8 up to 128.  No counterpart in the reference.
  *
  * The backward pass takes o, o_low (or NULL), lse as the forward pass left them and d_o (contiguous like q)

@@ -306,13 +306,23 @@ __device__ __forceinline__ void score(float (&s)[N], const Scores& sc, int first
   }
 }
 
+// Both 16-bit values of a pair, added to 32-bit sums.
+template <bool BF16>
+__device__ __forceinline__ void add_packed(uint32_t pair, float* lo, float* hi) {
+  if constexpr (BF16)
+    asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; add.f32.bf16 %0, l, %0; add.f32.bf16 %1, h, %1;}" : "+f"(*lo), "+f"(*hi) : "r"(pair));
+  else
+    asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; add.f32.f16 %0, l, %0; add.f32.f16 %1, h, %1;}" : "+f"(*lo), "+f"(*hi) : "r"(pair));
+}
+
 // One thread per row: the row's 128 scores s (hidden ones -inf) become weights
 // 2^(s by - m) (SCALED: s is in log2 units already), packed to 16 bits over columns 0 .. 63 of
 // s_tmem; ready[i] gets the warp's arrival when 64 of them are in place.  `sum` takes the weights as
-// they are, for the row's logarithm; with BOTH `packed_sum` takes them as they were rounded:
-// divided by it, the result's weights add up to one, so an error all of them share, above all
-// that of a row's one large weight, falls out.  by > 0.
-template <bool BF16, bool SCALED, bool BOTH>
+// they are, for the row's logarithm, `packed_sum` as they were rounded: divided by it, the result's
+// weights add up to one, so an error all of them share, above all that of a row's one large weight,
+// falls out.  (Two sums cost 3 %: 16384 causal tokens x 8 heads of 128 406 -> 418 us; pairs unpacked to 32
+// bits before the second one 442.)  by > 0.
+template <bool BF16, bool SCALED>
 __device__ __forceinline__ void weigh(const float (&s)[kTile], float by, float m, float* sum, float* packed_sum,
                                       uint32_t s_tmem, uint64_t* ready, int lane) {
   const float mu = m == -INFINITY ? 0.f : m;
@@ -331,7 +341,7 @@ __device__ __forceinline__ void weigh(const float (&s)[kTile], float by, float m
         const int k = (i >> 1) & 1;
         add[k] = ptx::add2(add[k], x);
         w[i >> 1] = pack2<BF16>(x.x, x.y);
-        if (BOTH) packed_add[k] = ptx::add2(packed_add[k], unpack2<BF16>(w[i >> 1]));
+        add_packed<BF16>(w[i >> 1], &packed_add[k].x, &packed_add[k].y);
       }
       ptx::tmem_st_32x16(s_tmem + c / 2, w);
     }
@@ -341,17 +351,15 @@ __device__ __forceinline__ void weigh(const float (&s)[kTile], float by, float m
     if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ready[half]));
   }
   *sum += (add[0].x + add[0].y) + (add[1].x + add[1].y);
-  if (BOTH) *packed_sum += (packed_add[0].x + packed_add[0].y) + (packed_add[1].x + packed_add[1].y);
+  *packed_sum += (packed_add[0].x + packed_add[0].y) + (packed_add[1].x + packed_add[1].y);
 }
 template <int DP, bool BF16, bool SCALED>
 __device__ __forceinline__ void weigh_tile(const float (&s)[kTile], float by, bool first, float* m, float* sum,
-                                           float* packed_sum, bool both, uint32_t s_tmem, uint32_t o_tmem,
-                                           uint64_t* ready, int lane) {
+                                           float* packed_sum, uint32_t s_tmem, uint32_t o_tmem, uint64_t* ready, int lane) {
   float mt = max_of(s);
   if (!SCALED) mt *= by;
   follow_maximum<DP>(mt, first, m, sum, packed_sum, o_tmem);
-  if (both) weigh<BF16, SCALED, true>(s, by, *m, sum, packed_sum, s_tmem, ready, lane);
-  else weigh<BF16, SCALED, false>(s, by, *m, sum, packed_sum, s_tmem, ready, lane);
+  weigh<BF16, SCALED>(s, by, *m, sum, packed_sum, s_tmem, ready, lane);
 }
 
 __device__ __forceinline__ void attn_fail(uint32_t* status, volatile uint32_t* abort_flag, uint32_t code) {

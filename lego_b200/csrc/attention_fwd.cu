@@ -328,12 +328,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
 #pragma unroll
         for (int c = 0; c < kTile; ++c) s[c] = (see[c >> 5] >> (c & 31)) & 1u ? s[c] : -INFINITY;
       }
-      weigh_tile<DP, BF16, CAP || BIAS>(s, sc.by, j == l, &m, &sum, &packed_sum, a.low, s_tmem, o_tmem, sh->p_full[t], lane);
+      weigh_tile<DP, BF16, CAP || BIAS>(s, sc.by, j == l, &m, &sum, &packed_sum, s_tmem, o_tmem, sh->p_full[t], lane);
     }
     // result
     const bool has = sum > 0.f || sum != sum;
-    if (!a.low) packed_sum = sum;
-    const float inv = packed_sum > 0.f || sum != sum ? 1.f / packed_sum : 0.f;
+    const float inv = has ? 1.f / packed_sum : 0.f;
     if (ok && l < e) {
       if (!ptx::mbar_wait_bounded(ptx::smem_u32(&sh->o_full[t]), 0, abort_flag, kAttnWait)) ok = false;
       if (!__all_sync(~0u, ok)) {

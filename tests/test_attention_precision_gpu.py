@@ -124,3 +124,14 @@ def test_tree_errors_are_those_of_the_roundings(spread, dtype):
         k, v = (c[table.long()].flatten(1, 2)[:, :L] for c in (kc, vc))
         exact, with_r = model(q, k, v, causal=True, softcap=softcap)
         assert times(got, exact["o"], with_r["o"]) <= WHOLE
+
+
+@pytest.mark.parametrize("shape", [(2, 700, 700, 4, 2, 64), (1, 2, 5000, 4, 2, 128), (1, 300, 300, 160, 160, 64)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("how", [dict(), dict(softcap=20.0)])
+def test_the_result_is_the_same_whether_a_gradient_is_wanted(how, dtype, shape):
+    q, k, v, _ = make(3, *shape, dtype, 4.0)
+    with torch.no_grad():
+        o, lse = ops.attention(q, k, v, causal=True, return_lse=True, **how)
+    o2, lse2 = ops.attention(q.requires_grad_(), k, v, causal=True, return_lse=True, **how)
+    assert o2.requires_grad and torch.equal(o, o2) and torch.equal(lse, lse2)
