@@ -216,18 +216,27 @@ __device__ __forceinline__ void copy_tile_clean(uint8_t* tile, const uint16_t* b
 
 // ---- a tile of scores to weights ---------------------------------------------------------------
 
-// log2 of the growth a row's reference value may lag behind its maximum: weights stay below
-// 2^8, their sum is kept in 32 bits, and O in TMEM is rarely rescaled.
-constexpr float kRescale = 8.f;
+// A row's weights are 2^(s - m) for a reference value m that moves only when the row's maximum outgrows it by
+// kLag, so O in TMEM is rarely rescaled.  bf16: m is the maximum of its time, weights stay below 2^8.
+// fp16 has no range to spare: a weight loses bits below 2^-14 and is zero below 2^-25, and many keys far below
+// the largest can make up much of a row.  There m is the maximum less kLift and lags by less, so
+// the weights stand times 2^11 and more and stay below 2^15: 17 nats under the largest still have all bits, what becomes
+// zero is under 2^-36 of it, and 2^20 such keys together under a thirtieth of the result's rounding.
+// (Lags of 2^2, 2^4 and 2^8: 2 x 4096 causal tokens x 32/8 heads of 128 255, 246 and 247 us; documents of 45 to
+// 2162 tokens with a cap no difference.)
+template <bool BF16> constexpr float kLag = BF16 ? 8.f : 4.f;
+template <bool BF16> constexpr float kLift = BF16 ? 0.f : 11.f;
+static_assert(kLag<false> + kLift<false> <= 15.f, "weights have to stay in fp16's range");
 
 // A row's reference value m for a tile whose maximum is mt (log2 units).  Not the first tile:
 // where some row of the warp outgrew its reference value, its sums, in two registers and over DP
 // columns of o_tmem, follow it.
-template <int DP>
+template <int DP, bool BF16>
 __device__ __forceinline__ void follow_maximum(float mt, bool first, float* m, float* sum, float* sum2, uint32_t o_tmem) {
+  mt -= kLift<BF16>;
   if (first) {
     *m = mt;
-  } else if (__any_sync(~0u, mt > *m + kRescale)) {
+  } else if (__any_sync(~0u, mt > *m + kLag<BF16>)) {
     const float mn = fmaxf(*m, mt);
     const float f = mn == -INFINITY ? 1.f : ex2(*m - mn);
     *m = mn;
@@ -243,6 +252,12 @@ __device__ __forceinline__ void follow_maximum(float mt, bool first, float* m, f
       ptx::tmem_st_32x16(o_tmem + c, o);
     }
   }
+}
+// The natural logarithm of a row's sum of exp(s).
+template <bool BF16>
+__device__ __forceinline__ float log_of_sum(float m, float sum) {
+  constexpr float by = BF16 ? 1.f : 1.f / (1 << (int)kLift<false>);
+  return (m + kLift<BF16> + log2f(sum * by)) * kLn2;
 }
 
 // Raw scores to log2 units: z = cap tanh(scale s / cap) - slope distance, times log2(e).  first:
@@ -358,7 +373,7 @@ __device__ __forceinline__ void weigh_tile(const float (&s)[kTile], float by, bo
                                            float* packed_sum, uint32_t s_tmem, uint32_t o_tmem, uint64_t* ready, int lane) {
   float mt = max_of(s);
   if (!SCALED) mt *= by;
-  follow_maximum<DP>(mt, first, m, sum, packed_sum, o_tmem);
+  follow_maximum<DP, BF16>(mt, first, m, sum, packed_sum, o_tmem);
   weigh<BF16, SCALED>(s, by, *m, sum, packed_sum, s_tmem, ready, lane);
 }
 

@@ -13,9 +13,9 @@
 // sums in 32 bits and (m, sums) of its rows in the workspace, a second kernel joins them in the
 // order of the keys.
 //
-// Running maximum: the reference value m of a row moves only when a tile's maximum exceeds it
-// by more than 2^8 -- weights stay below 2^8, the row sum is kept in 32 bits -- so O in
-// TMEM is rarely rescaled.  The rounding of the weights to 16 bits, half a step of the type
+// Running maximum: the reference value m of a row moves only when a tile's maximum outgrows it by more
+// than 2^8 (fp16 2^4, its weights stand times 2^11: see attention.cuh), so O in TMEM is rarely rescaled;
+// the row sums are kept in 32 bits.  The rounding of the weights to 16 bits, half a step of the type
 // each, and the one of the result are the only ones below 32 bits.  What the last one takes
 // away goes to a second output where the caller wants it: the backward pass subtracts dO O
 // from terms of nearly the same size wherever a row has one large weight.
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_kernel(const __grid_c
       ok = false;      // the second kernel writes the results
     }
     if (row < p.q_len && ok)
-      a.lse[((long long)b * p.q_heads + h) * p.q_len + row] = has ? (m + log2f(sum)) * kLn2 : -INFINITY;
+      a.lse[((long long)b * p.q_heads + h) * p.q_len + row] = has ? log_of_sum<BF16>(m, sum) : -INFINITY;
     for (int low = 0; ok && low <= (a.low ? 1 : 0) && q0 + quarter * 32 < p.q_len; ++low) {   // the tile's own queries are no longer needed: stage there
 #pragma unroll
       for (int c = 0; c < DP; c += 32) {
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
       }
     }
   }
-  if (lane == 0) a.lse[row] = has ? (top + log2f(sum)) * kLn2 : -INFINITY;
+  if (lane == 0) a.lse[row] = has ? log_of_sum<BF16>(top, sum) : -INFINITY;
 }
 
 // Pieces of a call's loop over the keys, and the workspace they take.

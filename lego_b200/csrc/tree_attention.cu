@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attn_kernel(const __grid
           if (chunks > 1 && back) ptx::tmem_st_wait();
           if (!CAP && !BIAS) mt *= by;     // by > 0 in this instance
           float unused = 0.f;
-          follow_maximum<DP>(mt, i == t, &m, &sum, &unused, o_tmem);
+          follow_maximum<DP, BF16>(mt, i == t, &m, &sum, &unused, o_tmem);
           const float mu = m == -INFINITY ? 0.f : m;
           const float2 by2 = make_float2(by, by), mu2 = make_float2(-mu, -mu);
           for (int x = 0; x < 4; ++x) {

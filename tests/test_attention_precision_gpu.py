@@ -135,3 +135,76 @@ def test_the_result_is_the_same_whether_a_gradient_is_wanted(how, dtype, shape):
         o, lse = ops.attention(q, k, v, causal=True, return_lse=True, **how)
     o2, lse2 = ops.attention(q.requires_grad_(), k, v, causal=True, return_lse=True, **how)
     assert o2.requires_grad and torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+# ---- the range of fp16 -----------------------------------------------------------------------------
+
+N = 1 << 16
+
+
+def tail(nats, at):
+    """N keys `nats` below one key of value zero at place `at`: (q, k, v [S, D], weights, result in 64 bits) with
+    scale 1.  The values are of one sign, so nothing cancels."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k = torch.zeros(N + 1, 64, device="cuda", dtype=torch.float16)
+    k[at, 0] = nats / 4
+    q = torch.zeros(64, device="cuda", dtype=torch.float16)
+    q[0] = 4
+    v = (1 + 0.1 * torch.randn(N + 1, 64, generator=g, device="cuda")).half()
+    v[at] = 0
+    p = torch.softmax(k.double() @ q.double(), 0)
+    return q, k, v, p, p @ v.double()
+
+
+def tail_room(p, v, o):
+    """Half a step of every weight, or where a weight is below the type's normal range half of its smallest step,
+    2^-25, of weights that stand times 2^11; half a step of the result; 2^-18 for 32 bits."""
+    u = 2.0 ** -11
+    return ((u + 2.0 ** -18) * p + 2.0 ** -36) @ v.double().abs() + u * o.abs()
+
+
+@pytest.mark.parametrize("nats", [9.0, 14.0, 17.4])
+@pytest.mark.parametrize("at", [0, 3000, N])
+@pytest.mark.parametrize("H", [1, 160])
+def test_a_long_tail_in_fp16(H, at, nats):
+    """Many keys far below one of value zero make the whole result.  One head: the loop is cut into
+    pieces; 160 of them: it is not."""
+    q, k, v, p, o = tail(nats, at)
+    full = q.expand(1, 1, H, 64)
+    kk, vv = k[None, :, None], v[None, :, None]
+    got, lse, low = ops._attention_fwd(full, kk, vv, False, None, None, 0.0, None, 1.0, True)
+    room = tail_room(p, v, o)
+    assert ((got[0, 0].double() - o).abs() <= room).all()
+    exact = torch.logsumexp(k.double() @ q.double(), 0)
+    assert ((lse.double() - exact).abs() <= 2.0 ** -18 * exact).all()
+    # dO of ones: delta is the sum of o, the one key's score gradient -p delta, and dq that times the key
+    do = torch.ones_like(full)
+    dq, dk, dv = ops.attention_bwd(do, full, kk, vv, got, lse, scale=1.0, o_low=low)
+    delta = o.sum()
+    want = -p[at] * delta * k[at, 0].double()
+    # of delta: that of the weights; then the rounding of the score gradient and of the result
+    assert ((dq[0, 0, :, 0].double() - want).abs() <= want.abs() * (room.sum() / delta + 2 * 2.0 ** -11)).all()
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("nats", [9.0, 14.0, 17.4])
+@pytest.mark.parametrize("at", [0, 3000, N])
+@pytest.mark.parametrize("T,H", [(1, 1), (9, 4), (30, 4)])
+def test_a_long_tail_in_fp16_over_pages(T, H, at, nats):
+    """All forms of the rows: four copies, two, one.  Drafted tokens see only the cached ones and themselves, whose
+    keys are like the others."""
+    q, k, v, p, o = tail(nats, at)
+    pages = (N + 1 + T + 63) // 64
+    kc, vc = (torch.zeros(pages * 64, 1, 64, device="cuda", dtype=torch.float16) for _ in range(2))
+    kc[:N + 1, 0], vc[:N + 1, 0] = k, v
+    vc[N + 1:] = 1
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    got = ops.tree_attention(q.expand(1, T, H, 64).contiguous(), kc.view(-1, 64, 1, 64), vc.view(-1, 64, 1, 64), table,
+                             torch.tensor([N + 1], dtype=torch.int32, device="cuda"),
+                             torch.full((1, T), -1, dtype=torch.int32, device="cuda"), scale=1.0)
+    one = torch.exp(-torch.tensor(float(k[at, 0]) * 4, dtype=torch.float64, device="cuda"))     # one more key of the tail
+    total = 1 / p[at]
+    o = (o * total + one) / (total + one)
+    room = tail_room(torch.cat([p * total, one[None]]) / (total + one), torch.cat([v, torch.ones_like(v[:1])]), o)
+    assert ((got[0].double() - o).abs() <= room).all()
+    assert ops.device_status() == 0
