@@ -23,9 +23,13 @@
 // columns of TMEM are in use (64-wide heads: 384).  Query kernel: S in two buffers, so the
 // weights of a tile are ready when its dP is.
 //
-// fp16: P is kept times 2^14 (weights of long rows fall below the type's normal range) and dS
-// times a power of two per key head that a bound on it, 2 D max|dO| max|V|, leaves in range;
-// both are taken out of the 32-bit sums at the end.
+// fp16: P is kept times 2^14 (weights of long rows fall below the type's normal range) and dS times a
+// power of two that a bound on it leaves in range, |dS| <= |dP - delta| <= max|dO_i| sum|V_j| + |delta_i|.  The
+// query kernel has one per row, from the keys it walks.  In the key kernel the rows of a sum are queries: one
+// per step (128 queries of one head), and where the next step's is another, dK in TMEM follows, which
+// a power of two does exactly.  So a token's gradients do not depend on how large dO is elsewhere, but for
+// dK from queries of one tile: what is 2^-29 of the tile's bound still has all bits.  All powers are taken out of
+// the 32-bit sums at the end.
 //
 // What bounds it: the tensor pipe (67 % and 60 % busy) and the warps that feed it take turns; memory is idle.
 // Counting 10 flop per visible pair and value: 16384 tokens x 8/1 heads of 128, bf16 2.95 ms (0.93 PFLOP/s), causal
@@ -45,7 +49,7 @@ constexpr int kBwdThreads = 384;
 constexpr int kBwdRegs = 168, kMathRegs = 216, kBwdOtherRegs = 72;
 static_assert(2 * kMathRegs + kBwdOtherRegs <= 3 * kBwdRegs, "more registers than the launch has would wait forever");
 constexpr int kWeightShift = 14;     // fp16: log2 of the factor on P
-constexpr float kScoreLimit = 30000.f;   // fp16: what the bound on dS is scaled to stay under
+constexpr int kStats = 264;          // floats of a step's rows: -lse, -delta, and in fp16 4 x (peak of dO, of |delta|)
 
 struct BwdArgs {
   CUtensorMap q, k, v, d_o;          // boxes of 128 tokens
@@ -54,7 +58,10 @@ struct BwdArgs {
   const uint16_t *q_raw, *k_raw, *o_raw, *low_raw, *do_raw, *v_raw;    // low_raw: what o's rounding left, or null
   const float* lse;
   float *neg_lse, *neg_delta;        // [batch][q_heads][q_len up to whole tiles], log2 units
-  uint32_t* peak;                    // fp16: [batch][k_heads][2] bits of max|dO|, max|V|
+  // fp16: max|dO| of every row; of 32 rows, and the largest |delta|; the largest sum|V| of 32 keys
+  float *row_peak;                   // like neg_lse
+  float2 *query_peaks;               // [batch][q_heads][query tiles][4]
+  float *key_peaks;                  // [batch][k_heads][key tiles][4]
   uint32_t* status;
   int key_pieces, query_pieces;
   float *key_part, *query_part;      // [piece][tile CTA](dV, dK)[128][DP]; [piece][tile CTA][128][DP]
@@ -65,26 +72,22 @@ __device__ __forceinline__ long long row_slot(const AttnProblem& p, int b, int h
   return ((long long)b * p.q_heads + h) * tiles_of(p.q_len) * kTile;
 }
 
-// fp16: the power of two dS is kept times, from the peaks of one key head.
-__device__ __forceinline__ float score_factor(const BwdArgs& a, int b, int hk) {
-  const uint32_t* pk = a.peak + ((long long)b * a.p.k_heads + hk) * 2;
-  const float bound = 2.f * a.p.dim * __uint_as_float(pk[0]) * __uint_as_float(pk[1]);
-  if (!(bound > 1e-30f) || !(bound < 1e30f)) return 1.f;
-  return ldexpf(1.f, ilogbf(kScoreLimit / bound));
+// fp16: log2 of the factor that brings a bound on dS to 2^14 .. 2^15, half of the type's range; false
+// where there is none (nothing but zeros; an infinity or a NaN, which no factor mends).
+__device__ __forceinline__ bool factor_log2(float bound, int* e) {
+  if (!(bound > 1e-30f) || !(bound < 1e30f)) return false;
+  *e = 14 - ((int)(__float_as_uint(bound) >> 23) - 127);
+  return true;
 }
-
-// A maximum over many rows: most rows find a larger one there already and leave it.
-__device__ __forceinline__ void raise_peak(uint32_t* at, uint32_t bits) {
-  if (bits > __ldcg(at)) atomicMax(at, bits);
-}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ float max_of4(float4 v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
 
 // ---- preparation -----------------------------------------------------------------------------
 
-// Per row delta and the negated log-sum, and in fp16 the peaks of dO and V.  Rows past q_len (whole
+// Per row delta and the negated log-sum, and in fp16 the peaks of dO, delta and V.  Rows past q_len (whole
 // tiles) and padding get weight zero: -inf.  A warp takes 32 tokens of one head, a block the same
 // tokens of eight heads, which lie together in memory; four rows are under way at a time, and lane i
-// keeps token i's results so they leave as one line.  Memory bound.  The peaks are maxima, so the
-// order of the atomics, one per warp that raises a peak, does not matter.
+// keeps token i's results so they leave as one line.  Memory bound.
 struct PrepGrid {
   int q_chunks, q_blocks, k_blocks;     // of 32 tokens; of 8 heads x 32 tokens
 };
@@ -92,7 +95,7 @@ __host__ __device__ inline PrepGrid prep_grid(const AttnProblem& p, bool peaks) 
   PrepGrid g;
   g.q_chunks = tiles_of(p.q_len) * 4;
   g.q_blocks = p.batch * g.q_chunks * ((p.q_heads + 7) / 8);
-  g.k_blocks = peaks ? p.batch * ((p.k_len + 31) / 32) * ((p.k_heads + 7) / 8) : 0;
+  g.k_blocks = peaks ? p.batch * tiles_of(p.k_len) * 4 * ((p.k_heads + 7) / 8) : 0;
   return g;
 }
 template <bool BF16>
@@ -110,7 +113,7 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __grid_constan
     const int i0 = chunk * 32, own = i0 + lane;
     const bool real = own < p.q_len && (!p.documents || p.documents[(long long)b * p.k_len + p.offset + own] >= 0);
     const uint32_t rows = __ballot_sync(~0u, real);
-    float kept = 0.f, peak = 0.f;
+    float kept = 0.f, own_peak = 0.f;
     const long long stride = (long long)p.q_heads * p.dim;
     const long long at0 = ((long long)b * p.q_len + i0) * stride + (long long)h * p.dim + lane * 4;
     for (int r = 0; r < 32; r += 4) {
@@ -130,10 +133,15 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __grid_constan
         const float2 x1 = ptx::add2(unpack2<BF16>(x[k].y), unpack2<BF16>(y[k].y));
         const float2 d0 = unpack2<BF16>(d[k].x), d1 = unpack2<BF16>(d[k].y);
         float delta = fmaf(x0.x, d0.x, fmaf(x0.y, d0.y, fmaf(x1.x, d1.x, x1.y * d1.y)));
-        if (!BF16) peak = fmaxf(peak, fmaxf(fmaxf(fabsf(d0.x), fabsf(d0.y)), fmaxf(fabsf(d1.x), fabsf(d1.y))));
+        uint32_t peak = 0;
+        if (!BF16)
+          peak = __reduce_max_sync(~0u, __float_as_uint(fmaxf(fmaxf(fabsf(d0.x), fabsf(d0.y)), fmaxf(fabsf(d1.x), fabsf(d1.y)))));
 #pragma unroll
         for (int o = 16; o; o >>= 1) delta += __shfl_xor_sync(~0u, delta, o);
-        if (lane == r + k) kept = delta;
+        if (lane == r + k) {
+          kept = delta;
+          own_peak = __uint_as_float(peak);
+        }
       }
     }
     float nl = -INFINITY;
@@ -145,27 +153,31 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __grid_constan
     a.neg_lse[at] = nl;
     a.neg_delta[at] = -kept;
     if (!BF16) {
-      const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(peak));
-      if (lane == 0) raise_peak(a.peak + ((long long)b * p.k_heads + h / p.group) * 2, top);
+      a.row_peak[at] = own_peak;
+      const float top = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(own_peak)));
+      const float most = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(fabsf(kept))));
+      if (lane == 0) a.query_peaks[at / 32] = make_float2(top, most);
     }
     return;
   }
   if (BF16) return;
-  const int id = (int)blockIdx.x - g.q_blocks, groups = (p.k_heads + 7) / 8, chunks = (p.k_len + 31) / 32;
+  const int id = (int)blockIdx.x - g.q_blocks, groups = (p.k_heads + 7) / 8, chunks = tiles_of(p.k_len) * 4;
   const int h = id % groups * 8 + warp, i0 = id / groups % chunks * 32, b = id / groups / chunks;
   if (h >= p.k_heads) return;
   float peak = 0.f;
 #pragma unroll 4
   for (int r = 0; r < 32; ++r) {
     const int j = i0 + r;
-    const bool real = j < p.k_len && (!p.documents || p.documents[(long long)b * p.k_len + j] >= 0);
-    if (!real || !mine) continue;
-    const uint2 x = __ldg(reinterpret_cast<const uint2*>(a.v_raw + b * p.v_stride[0] + j * p.v_stride[1] + h * p.v_stride[2] + lane * 4));
+    if (j >= p.k_len || (p.documents && p.documents[(long long)b * p.k_len + j] < 0)) continue;     // the same for the warp
+    uint2 x = make_uint2(0, 0);
+    if (mine) x = __ldg(reinterpret_cast<const uint2*>(a.v_raw + b * p.v_stride[0] + j * p.v_stride[1] + h * p.v_stride[2] + lane * 4));
     const float2 x0 = unpack2<BF16>(x.x), x1 = unpack2<BF16>(x.y);
-    peak = fmaxf(peak, fmaxf(fmaxf(fabsf(x0.x), fabsf(x0.y)), fmaxf(fabsf(x1.x), fabsf(x1.y))));
+    float sum = (fabsf(x0.x) + fabsf(x0.y)) + (fabsf(x1.x) + fabsf(x1.y));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    peak = fmaxf(peak, sum);
   }
-  const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(peak));
-  if (lane == 0) raise_peak(a.peak + ((long long)b * p.k_heads + h) * 2 + 1, top);
+  if (lane == 0) a.key_peaks[((long long)b * p.k_heads + h) * chunks + i0 / 32] = peak;
 }
 
 // ---- shared by the two product kernels ---------------------------------------------------------
@@ -285,7 +297,7 @@ __device__ __forceinline__ uint32_t packed_at(int step) { return (step < 4 ? 0 :
 
 template <int DP> constexpr int key_stages() { return DP == 128 ? 2 : 4; }
 template <int DP> constexpr int key_smem() {
-  return (2 + 2 * key_stages<DP>()) * tile_bytes<DP>() + key_stages<DP>() * 1024 + 1024 + 512;
+  return (2 + 2 * key_stages<DP>()) * tile_bytes<DP>() + key_stages<DP>() * kStats * 4 + 1024 + 512;
 }
 
 struct KeyShared {
@@ -301,9 +313,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = ptx::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
-  // K, V, ring of Q, ring of dO, ring of the rows' (-lse, -delta)
+  // K, V, ring of Q, ring of dO, ring of the rows' (-lse, -delta, peaks)
   float* stats = reinterpret_cast<float*>(smem + (2 + 2 * NS) * TILE);
-  KeyShared* sh = reinterpret_cast<KeyShared*>(smem + (2 + 2 * NS) * TILE + NS * 1024);
+  KeyShared* sh = reinterpret_cast<KeyShared*>(smem + (2 + 2 * NS) * TILE + NS * kStats * 4);
   volatile uint32_t* abort_flag = &sh->abort_flag;
   const uint32_t k_smem = ptx::smem_u32(smem), v_smem = k_smem + TILE, q_smem = v_smem + TILE, do_smem = q_smem + NS * TILE;
   const AttnProblem& p = a.p;
@@ -413,7 +425,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
                                 i * kTile, p.q_len, p.documents + (long long)b * p.k_len + p.offset, lane);
           }
           if (lane == 0) {
-            const uint32_t bytes = (dirty ? 0 : TILE) + (g ? 0 : 1024);
+            const uint32_t bytes = (dirty ? 0 : TILE) + (g ? 0 : BF16 ? 1024 : 1024 + 32);
             if (bytes) ptx::mbar_arrive_expect_tx(full, bytes);
             else ptx::mbar_arrive(full);
             if (!dirty)
@@ -423,8 +435,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
               }
             if (!g) {
               const long long at = row_slot(p, b, h) + i * kTile;
-              ptx::bulk_load(ptx::smem_u32(stats + slot * 256), a.neg_lse + at, 512, full);
-              ptx::bulk_load(ptx::smem_u32(stats + slot * 256 + 128), a.neg_delta + at, 512, full);
+              ptx::bulk_load(ptx::smem_u32(stats + slot * kStats), a.neg_lse + at, 512, full);
+              ptx::bulk_load(ptx::smem_u32(stats + slot * kStats + 128), a.neg_delta + at, 512, full);
+              if (!BF16) ptx::bulk_load(ptx::smem_u32(stats + slot * kStats + 256), a.query_peaks + at / 32, 32, full);
             }
           }
         }
@@ -500,8 +513,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_tmem = s_at + lanes + half * 64, dp_tmem = dp_at + lanes + half * 64;
     const int key = j0 + quarter * 32 + lane;
-    const float ds_factor = BF16 ? 1.f : score_factor(a, b, hk);
-    const float w_by = BF16 ? 1.f : ldexpf(ds_factor, -kWeightShift);
+    // fp16: log2 of the factor on dS, and the smallest so far
+    int factor = 0, least = 1000;
+    const float key_peak = BF16 ? 0.f : max_of4(reinterpret_cast<const float4*>(a.key_peaks)[((long long)b * p.k_heads + hk) * tiles_of(p.k_len) + kt]);
     int own_doc = -1;
     int4 tile_docs = make_int4(0, 0, 0, 0);
     const int* docs = nullptr;      // of query 0 on
@@ -530,7 +544,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
       // seen whole: the first query sees the last key (queries past the end have weight zero)
       bool masked = p.causal && last_key(p, prefix, i0 + p.offset) < j0 + kTile - 1;
       if (qd) masked = masked || !docs_same(qd[i], tile_docs);
-      const float4* nl4 = reinterpret_cast<const float4*>(stats + slot * 256 + half * 64);
+      const float4* nl4 = reinterpret_cast<const float4*>(stats + slot * kStats + half * 64);
       const float4* nd4 = nl4 + 32;
       // the row sums arrive with Q, before the scores made from it
       if (!wait(&sh->q_full[slot], (n / NS) & 1, 0x540000u) || !wait(&sh->s_full, n & 1, 0x540001u)) break;
@@ -593,7 +607,33 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sh->p_full));
 
+      const int before = factor;
+      if (!BF16) {
+        const float4* peaks = reinterpret_cast<const float4*>(stats + slot * kStats + 256);
+        const float4 x = peaks[0], y = peaks[1];
+        int best;
+        if (factor_log2(fmaxf(fmaxf(x.x, x.z), fmaxf(y.x, y.z)) * key_peak + fmaxf(fmaxf(x.y, x.w), fmaxf(y.y, y.w)), &best)) {
+          // Steps whose bounds differ little share a factor: one that leaves the bound at 2^11 or more and below
+          // 2^15 stays.  None is more than 2^48 times the smallest, so the sums, 2^51 at that one, stay in range.
+          if (least == 1000 || factor > best || factor < best - 3) factor = best - 1;
+          factor = factor < least + 48 ? factor : least + 48;
+          least = factor < least ? factor : least;
+        }
+      }
+      const float w_by = BF16 ? 1.f : power_of_two(factor - kWeightShift);
       if (!wait(&sh->dp_full, n & 1, 0x540002u)) break;
+      if (!BF16 && n > 0 && factor != before) {      // dP came after dK's last product, and the next one waits for this dS
+        const float by = power_of_two(factor - before);
+#pragma unroll 1
+        for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 16) {
+          uint32_t o[16];
+          ptx::tmem_ld_32x16(dk_at + lanes + c, o);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
+          ptx::tmem_st_32x16(dk_at + lanes + c, o);
+        }
+      }
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         float d[32];
@@ -630,7 +670,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_keys_kernel(const __g
     }
     if (ok && steps > 0) wait(&sh->acc_full, 0, 0x550000u);
     const int row0 = j0 + quarter * 32;
-    const float dv_by = BF16 ? 1.f : ldexpf(1.f, -kWeightShift), dk_by = p.scale / ds_factor;
+    const float dv_by = BF16 ? 1.f : ldexpf(1.f, -kWeightShift), dk_by = p.scale * power_of_two(-factor);
     if (ok && a.key_pieces > 1) {
       const long long slot = ((long long)piece * (gridDim.x / a.key_pieces) + cta) * 2 + half;
       keep_rows<DP>(a.key_part + (slot * kTile + quarter * 32) * DP, (half ? dk_at : dv_at) + lanes, steps > 0,
@@ -876,10 +916,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
     const int row = q0 + quarter * 32 + lane, pos = row + p.offset;
     const int last = last_key(p, prefix, pos), last_first = last_key(p, prefix, q0 + p.offset);
     const Scores sc = scores_of<CAP>(p.scale, p.softcap, p.slopes, h);
-    const float ds_factor = BF16 ? 1.f : score_factor(a, b, hk);
-    const float w_by = BF16 ? 1.f : ldexpf(ds_factor, -kWeightShift);
     const long long slot = row_slot(p, b, h) + row;
     const float nl = a.neg_lse[slot], nd = a.neg_delta[slot];
+    int factor = 0;        // fp16: log2 of the factor on the row's dS
+    if (!BF16) {
+      const float4* peaks = reinterpret_cast<const float4*>(a.key_peaks) + ((long long)b * p.k_heads + hk) * tiles_of(p.k_len) + lo;
+      float peak = 0.f;
+#pragma unroll 4
+      for (int j = lane; j < steps; j += 32) peak = fmaxf(peak, max_of4(peaks[j]));
+      peak = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(peak)));
+      factor_log2(fmaf(a.row_peak[slot], peak, fabsf(nd)), &factor);
+    }
+    const float w_by = BF16 ? 1.f : power_of_two(factor - kWeightShift), dq_by = p.scale * power_of_two(-factor);
     const float2 nl2 = make_float2(nl, nl), nd2 = make_float2(nd, nd);
     int own_doc = -1;
     int4 tile_docs = make_int4(0, 0, 0, 0);
@@ -974,9 +1022,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_queries_kernel(const 
     const int row0 = q0 + quarter * 32;
     if (ok && half == 0 && a.query_pieces > 1) {
       const long long slot = (long long)piece * (gridDim.x / a.query_pieces) + cta;
-      keep_rows<DP>(a.query_part + (slot * kTile + quarter * 32) * DP, dq_at + lanes, steps > 0, p.scale / ds_factor, lane);
+      keep_rows<DP>(a.query_part + (slot * kTile + quarter * 32) * DP, dq_at + lanes, steps > 0, dq_by, lane);
     } else if (ok && half == 0 && row0 < p.q_len)      // staged where Q was
-      store_rows<DP, BF16>(&a.dq, dq_at + lanes, steps > 0, p.scale / ds_factor, smem + quarter * 4096, row0, h, b, lane);
+      store_rows<DP, BF16>(&a.dq, dq_at + lanes, steps > 0, dq_by, smem + quarter * 4096, row0, h, b, lane);
   }
 
   ptx::tc_fence_before();
@@ -1027,16 +1075,18 @@ int32_t launch_bwd_scores(const BwdArgs& a, int device, cudaStream_t s) {
 // Workspace of the backward pass: document summaries, row sums, peaks, the pieces' sums (those of dQ
 // are written after those of dK, dV have been added up, and use their place).
 struct BwdLayout {
-  int64_t rows, neg_lse, neg_delta, peak, part, bytes;
+  int64_t neg_lse, neg_delta, row_peak, query_peaks, key_peaks, part, bytes;
   int key_pieces, query_pieces;
 };
-BwdLayout bwd_layout(const AttnProblem& p) {
+BwdLayout bwd_layout(const AttnProblem& p, bool fp16) {
   BwdLayout l;
-  l.rows = (int64_t)p.batch * p.q_heads * tiles_of(p.q_len) * kTile;
+  const int64_t rows = (int64_t)p.batch * p.q_heads * tiles_of(p.q_len) * kTile;
   l.neg_lse = attention_docs_bytes(p);
-  l.neg_delta = l.neg_lse + l.rows * 4;
-  l.peak = l.neg_delta + l.rows * 4;
-  l.part = l.peak + ((int64_t)p.batch * p.k_heads * 8 + 15) / 16 * 16;
+  l.neg_delta = l.neg_lse + rows * 4;
+  l.row_peak = l.neg_delta + rows * 4;
+  l.query_peaks = l.row_peak + (fp16 ? rows * 4 : 0);
+  l.key_peaks = l.query_peaks + (fp16 ? rows / 32 * 8 : 0);
+  l.part = l.key_peaks + (fp16 ? (int64_t)p.batch * p.k_heads * tiles_of(p.k_len) * 16 : 0);
   const int64_t key_ctas = (int64_t)tiles_of(p.k_len) * p.batch * p.k_heads, query_ctas = (int64_t)tiles_of(p.q_len) * p.batch * p.q_heads;
   l.key_pieces = pieces_of(p, key_ctas, (int64_t)tiles_of(p.q_len) * p.group);
   l.query_pieces = pieces_of(p, query_ctas, tiles_of(p.k_len));
@@ -1058,7 +1108,7 @@ int64_t lego_attention_workspace_bytes(const lego_attention_t* d, int32_t backwa
   AttnProblem p;
   const int32_t st = attention_problem(d, &p);
   if (st != LEGO_OK) return st;
-  return backward ? bwd_layout(p).bytes : attention_fwd_bytes(p);
+  return backward ? bwd_layout(p, d->dtype == LEGO_F16).bytes : attention_fwd_bytes(p);
 }
 
 int32_t lego_attention_bwd(const lego_attention_t* d, const void* q, const void* k, const void* v, const void* o,
@@ -1072,7 +1122,7 @@ int32_t lego_attention_bwd(const lego_attention_t* d, const void* q, const void*
        (uintptr_t)dv | (uintptr_t)workspace) & 15)
     return LEGO_ERR_ALIGN;
   const AttnProblem& p = a.p;
-  const BwdLayout l = bwd_layout(p);
+  const BwdLayout l = bwd_layout(p, d->dtype == LEGO_F16);
   if (workspace_bytes < l.bytes) return LEGO_ERR_SIZE;
   DeviceCtx* ctx = device_ctx(&st);
   if (!ctx) return st;
@@ -1100,7 +1150,9 @@ int32_t lego_attention_bwd(const lego_attention_t* d, const void* q, const void*
   a.lse = lse;
   a.neg_lse = reinterpret_cast<float*>(ws + l.neg_lse);
   a.neg_delta = reinterpret_cast<float*>(ws + l.neg_delta);
-  a.peak = reinterpret_cast<uint32_t*>(ws + l.peak);
+  a.row_peak = reinterpret_cast<float*>(ws + l.row_peak);
+  a.query_peaks = reinterpret_cast<float2*>(ws + l.query_peaks);
+  a.key_peaks = reinterpret_cast<float*>(ws + l.key_peaks);
   a.key_pieces = l.key_pieces;
   a.query_pieces = l.query_pieces;
   a.key_part = a.query_part = reinterpret_cast<float*>(ws + l.part);
@@ -1108,18 +1160,14 @@ int32_t lego_attention_bwd(const lego_attention_t* d, const void* q, const void*
   a.dk_raw = (uint16_t*)dk;
   a.dv_raw = (uint16_t*)dv;
   a.status = ctx->status_word;
-  if ((int64_t)p.batch * (tiles_of(p.q_len) * 4LL * ((p.q_heads + 7) / 8) + (p.k_len / 32 + 1LL) * ((p.k_heads + 7) / 8)) > 0x7fffffffLL)
+  if ((int64_t)p.batch * (tiles_of(p.q_len) * 4LL * ((p.q_heads + 7) / 8) + tiles_of(p.k_len) * 4LL * ((p.k_heads + 7) / 8)) > 0x7fffffffLL)
     return LEGO_ERR_SIZE;
   const PrepGrid grid = prep_grid(p, !bf16);
   const int blocks = grid.q_blocks + grid.k_blocks;
   st = attention_docs(&a.p, workspace, s);
   if (st != LEGO_OK) return st;
-  if (bf16) {
-    LEGO_CUDA_TRY(launch_overlapped(attn_bwd_prep_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, s, a));
-  } else {
-    LEGO_CUDA_TRY(cudaMemsetAsync(a.peak, 0, (size_t)(l.part - l.peak), s));
-    LEGO_CUDA_TRY(launch_overlapped(attn_bwd_prep_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, s, a));
-  }
+  LEGO_CUDA_TRY(launch_overlapped(bf16 ? attn_bwd_prep_kernel<true> : attn_bwd_prep_kernel<false>, dim3((unsigned)blocks),
+                                  dim3(256), 0, s, a));
   if (p.dim <= 64)
     return bf16 ? launch_bwd_scores<64, true>(a, ctx->device, s) : launch_bwd_scores<64, false>(a, ctx->device, s);
   return bf16 ? launch_bwd_scores<128, true>(a, ctx->device, s) : launch_bwd_scores<128, false>(a, ctx->device, s);

@@ -4,8 +4,8 @@ A kernel rounds to the type: the weights before their product with V, the score 
 the results.  ``rounded`` does the same to values of 64 bits without the type's limits of range, and ``model`` gives
 the results with those roundings and without.  Both errors are sums of the same independent roundings, so over
 n independent values their norms differ by a part of sqrt(1 / (2 n)) in the deviation: 0.022 for 1000
-rows.  WHOLE allows seven deviations.  What 32 bits lose is under 2^-18 of a value, against 2^-12 and
-more."""
+rows, 0.063 for 128.  WHOLE allows seven deviations, TILE five.  What 32 bits lose is under 2^-18 of a
+value, against 2^-12 and more; what fp16's range took would be many times the model's error."""
 import pytest
 import torch
 
@@ -13,7 +13,7 @@ from lego_b200 import ops
 
 pytestmark = pytest.mark.gpu
 
-WHOLE = 1.15
+WHOLE, TILE = 1.15, 1.32
 BITS = {torch.float16: 11, torch.bfloat16: 8}
 
 
@@ -208,3 +208,94 @@ def test_a_long_tail_in_fp16_over_pages(T, H, at, nats):
     room = tail_room(torch.cat([p * total, one[None]]) / (total + one), torch.cat([v, torch.ones_like(v[:1])]), o)
     assert ((got[0].double() - o).abs() <= room).all()
     assert ops.device_status() == 0
+
+
+def sized(kind, S):
+    """Sizes of dO's tokens, five powers of ten apart."""
+    size = torch.full((S,), 1e-2, device="cuda")
+    if kind == "one":
+        size[100] = 1e3
+    elif kind == "alternating":
+        size[::2] = 1e3
+    elif kind == "tiles":
+        size[torch.arange(S, device="cuda") // 128 % 2 == 0] = 1e3
+    elif kind == "falling":
+        size[:S // 2] = 1e3
+    return size
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kind", ["one", "alternating", "tiles", "falling"])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_fp16_gradients_of_tokens_of_any_size(softcap, kind, D):
+    """dq of a token does not depend on how large another's dO is; nor dk of keys on that of tiles of 128 queries
+    that do not see them."""
+    S = 1024
+    q, k, v, do = make(6, 1, S, S, 4, 2, D, torch.float16, 1.5)
+    size = sized(kind, S)
+    do = (do.float() * 20 * size[None, :, None, None]).half()
+    got = run(q, k, v, do, True, softcap=softcap)
+    exact, with_r = model(q, k, v, do, True, softcap=softcap, rest=softcap > 0)
+    for one in size.unique():
+        at = torch.nonzero(size == one)[:, 0]
+        if len(at) >= 128:
+            assert times(got["dq"], exact["dq"], with_r["dq"], at) <= TILE, float(one)
+    for t in range(0, S, 128):
+        at = slice(t, t + 128)
+        assert times(got["dv"], exact["dv"], with_r["dv"], at) <= TILE, t
+        if kind != "alternating":       # its keys have large and small contributions of one tile
+            assert times(got["dk"], exact["dk"], with_r["dk"], at) <= TILE, t
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_gradients_of_heads_of_any_size(D):
+    """Query heads that share a key head, five powers of ten apart; a document with large values beside one with small."""
+    S = 512
+    q, k, v, do = make(7, 1, S, S, 4, 2, D, torch.float16, 1.5)
+    by = torch.tensor([100.0, 1e-3, 1e-3, 100.0], device="cuda")
+    do = (do.float() * 20 * by[None, None, :, None]).half()
+    docs = (torch.arange(S, device="cuda")[None] // 256).int()
+    v[:, :256] *= 30
+    got = run(q, k, v, do, True, docs)
+    exact, with_r = model(q, k, v, do, True, docs)
+    for h in range(4):
+        for at in (slice(0, 256), slice(256, 512)):
+            assert times(got["dq"][:, :, h], exact["dq"][:, :, h], with_r["dq"][:, :, h], at) <= TILE
+    for at in (slice(0, 256), slice(256, 512)):
+        for n in ("dk", "dv"):
+            assert times(got[n], exact[n], with_r[n], at) <= TILE, n
+
+
+def test_fp16_gradients_at_the_ends_of_the_range():
+    """dO of zeros in some tiles, of the type's smallest and largest values in others: finite, and each right."""
+    S = 640
+    q, k, v, do = make(8, 1, S, S, 2, 1, 64, torch.float16, 1.5)
+    v = (v.float() * 0.01).half()
+    size = torch.tensor([0.0, 2e-7, 1.0, 0.0, 1e6], device="cuda").repeat_interleave(128)
+    do = (do.float() * 20 * size[None, :, None, None]).clamp(-3e4, 3e4).half()
+    got = run(q, k, v, do, True)
+    exact, with_r = model(q, k, v, do, True)
+    for n in ("dq", "dk", "dv"):
+        assert torch.isfinite(got[n]).all()
+    for t in range(0, S, 128):
+        at = slice(t, t + 128)
+        if (with_r["dq"] - exact["dq"])[:, at].norm() == 0:
+            assert (got["dq"][:, at].double() == exact["dq"][:, at]).all()
+        else:
+            assert times(got["dq"], exact["dq"], with_r["dq"], at) <= TILE, t
+        assert times(got["dk"], exact["dk"], with_r["dk"], at) <= TILE, t
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_gradients_of_documents_within_a_tile(D):
+    """Two documents of one tile of queries, four powers of ten apart: dk of both.  The small one's score gradients, near
+    2^-18 of the tile's bound times the weight, have all bits for weights down to 2^-10 and some below."""
+    q, k, v, do = make(9, 4, 128, 128, 4, 2, D, torch.float16, 1.0)
+    do[:, :64] = (do[:, :64].float() * 2e4).half()
+    do[:, 64:] = (do[:, 64:].float() * 2).half()
+    docs = (torch.arange(128, device="cuda")[None].expand(4, -1) // 64).int()
+    got = run(q, k, v, do, True, docs)
+    exact, with_r = model(q, k, v, do, True, docs)
+    for at in (slice(0, 64), slice(64, 128)):
+        for n in ("dq", "dk", "dv"):
+            assert times(got[n], exact[n], with_r[n], at) <= TILE, n
