@@ -335,8 +335,8 @@ __device__ __forceinline__ void add_packed(uint32_t pair, float* lo, float* hi) 
 // s_tmem; ready[i] gets the warp's arrival when 64 of them are in place.  `sum` takes the weights as
 // they are, for the row's logarithm, `packed_sum` as they were rounded: divided by it, the result's
 // weights add up to one, so an error all of them share, above all that of a row's one large weight,
-// falls out.  (Two sums cost 3 %: 16384 causal tokens x 8 heads of 128 406 -> 418 us; pairs unpacked to 32
-// bits before the second one 442.)  by > 0.
+// falls out.  (Two sums cost 2 %: 16384 causal tokens x 8 heads of 128 415 -> 422 us; 426 where a pair is added
+// before its group is stored, 440 with pairs unpacked to 32 bits first.)  by > 0.
 template <bool BF16, bool SCALED>
 __device__ __forceinline__ void weigh(const float (&s)[kTile], float by, float m, float* sum, float* packed_sum,
                                       uint32_t s_tmem, uint64_t* ready, int lane) {
@@ -353,12 +353,12 @@ __device__ __forceinline__ void weigh(const float (&s)[kTile], float by, float m
         float2 z = make_float2(s[c + i], s[c + i + 1]);
         z = SCALED ? ptx::add2(z, mu2) : ptx::fma2(z, by2, mu2);
         const float2 x = make_float2(ex2(z.x), ex2(z.y));
-        const int k = (i >> 1) & 1;
-        add[k] = ptx::add2(add[k], x);
+        add[(i >> 1) & 1] = ptx::add2(add[(i >> 1) & 1], x);
         w[i >> 1] = pack2<BF16>(x.x, x.y);
-        add_packed<BF16>(w[i >> 1], &packed_add[k].x, &packed_add[k].y);
       }
       ptx::tmem_st_32x16(s_tmem + c / 2, w);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) add_packed<BF16>(w[i], &packed_add[i & 1].x, &packed_add[i & 1].y);
     }
     ptx::tmem_st_wait();
     ptx::tc_fence_before();
