@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __grid_constan
     if (real) {
       const float ls = a.lse[((long long)b * p.q_heads + h) * p.q_len + own];
       if (ls > -INFINITY) nl = -ls * kLog2e + (BF16 ? 0.f : (float)kWeightShift);
+      else own_peak = 0.f;      // sees nothing: no gradient passes it
     }
     const long long at = row_slot(p, b, h) + own;
     a.neg_lse[at] = nl;

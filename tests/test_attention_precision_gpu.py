@@ -299,3 +299,15 @@ def test_fp16_gradients_of_documents_within_a_tile(D):
     for at in (slice(0, 64), slice(64, 128)):
         for n in ("dq", "dk", "dv"):
             assert times(got[n], exact[n], with_r[n], at) <= TILE, n
+
+
+def test_fp16_gradients_beside_queries_that_see_nothing():
+    """More queries than keys: the first see none, and how large their dO is matters to no gradient."""
+    q, k, v, do = make(10, 8, 200, 100, 2, 2, 64, torch.float16, 1.5)
+    do = (do.float() * 0.1).half()
+    do[:, :100] = 6e4
+    got = run(q, k, v, do, True)
+    exact, with_r = model(q, k, v, do, True)
+    assert not got["dq"][:, :100].any()
+    for n, at in (("dq", slice(100, 200)), ("dk", slice(0, 28)), ("dk", slice(0, 100)), ("dv", slice(0, 100))):
+        assert times(got[n], exact[n], with_r[n], at) <= TILE, (n, at)
