@@ -39,7 +39,8 @@ inline __host__ __device__ int tiles_of(int n) { return (n + kTile - 1) / kTile;
 // steps (a piece costs its start and its sums' way through memory).  148 SMs whatever the device,
 // so that the workspace follows from the call alone.  Measured: backward, 16384 causal tokens on one
 // key head (128 CTAs), 2392 -> 1580 us; equal loops of that number cut the same way were slower
-// (2944 -> 3322 us), and so was a forward pass of 192 CTAs (81 -> 116 us).
+// (2944 -> 3322 us), and so was a forward pass of 192 CTAs (81 -> 116 us), although calls of 149 to some 300
+// unequal CTAs take two waves whose longest CTAs set the time.
 inline int pieces_of(const AttnProblem& p, long long ctas, long long steps) {
   if (ctas >= 148) return 1;
   const long long want = p.causal || p.documents ? (2 * 148 + ctas - 1) / ctas : 148 / ctas, most = steps / 4;

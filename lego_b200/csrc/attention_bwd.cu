@@ -31,10 +31,12 @@
 // dK from queries of one tile: what is 2^-29 of the tile's bound still has all bits.  All powers are taken out of
 // the 32-bit sums at the end.
 //
-// What bounds it: the tensor pipe (67 % and 60 % busy) and the warps that feed it take turns; memory is idle.
-// Counting 10 flop per visible pair and value: 16384 tokens x 8/1 heads of 128, bf16 2.95 ms (0.93 PFLOP/s), causal
-// 1.57 ms (0.88); 2 x 4096 causal x 32/8 heads 0.96 ms (0.72); 8192 causal x 16 heads of 64, fp16 0.87 ms (0.40),
-// with a cap 1.16 ms.  Slower: products of 64 columns in the key kernel (858 -> 1143 us).
+// What bounds it: the tensor pipe (67 % and 60 % busy at heads of 128, 28 % at 64) and the warps that feed it (issue
+// slots 47 % and 39 %, under a cap 53 %) take turns; memory is idle.  Counting 10 flop per visible pair and value, from
+// a cold L2: 16384 causal tokens x 8/1 heads of 128, bf16 1.60 ms (0.86 PFLOP/s), all keys, fp16 3.30 ms (0.83);
+// 2 x 4096 causal x 32/8 heads, bf16 0.90 ms (0.76), fp16 0.96; 8192 causal x 16 heads of 64, fp16 0.84 ms (0.41), bf16
+// 0.77, with a cap, fp16 1.20 ms.  The key kernels of 64-wide heads spill 4 or 5 registers, as do the query kernels
+// under a cap.  Slower: products of 64 columns in the key kernel (858 -> 1143 us).
 #include <cuda.h>
 
 #include <type_traits>
@@ -87,7 +89,8 @@ __device__ __forceinline__ float max_of4(float4 v) { return fmaxf(fmaxf(v.x, v.y
 // Per row delta and the negated log-sum, and in fp16 the peaks of dO, delta and V.  Rows past q_len (whole
 // tiles) and padding get weight zero: -inf.  A warp takes 32 tokens of one head, a block the same
 // tokens of eight heads, which lie together in memory; four rows are under way at a time, and lane i
-// keeps token i's results so they leave as one line.  Memory bound.
+// keeps token i's results so they leave as one line.  Memory bound at heads of 128 (4.6 TB/s); at 64 half the lanes
+// have nothing to load, and in fp16 it is 1.7 TB/s (2 x 4096 tokens x 16 heads 40 us).
 struct PrepGrid {
   int q_chunks, q_blocks, k_blocks;     // of 32 tokens; of 8 heads x 32 tokens
 };

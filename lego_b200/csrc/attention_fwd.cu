@@ -24,11 +24,14 @@
 // the mask is evaluated only on tiles that are not seen whole, as 128 bits per row.
 //
 // What bounds it: the way of a row tile from scores to weights to the product.  The tensor pipe and the
-// exponentials' unit are each 63 % busy (4 x 4096 tokens, 16/4 heads of 128), and two row tiles are what TMEM and
-// the registers hold.  16384 causal tokens x 8 heads of 128, bf16: 434 us (1.27 PFLOP/s); 2 x 4096 causal x 32/8
-// heads 295 us (0.93); 8192 causal x 16 heads of 64, fp16 242 us (0.57), with a cap 438 us (its polynomial, 9
-// instructions on a pair of scores).  Slower, 16384 x 16384 x 8 heads, PFLOP/s where this form had 1.21: steps of
-// 64 keys 0.72, two issuing threads 0.83, four softmax warpgroups 1.11, K and V released together 1.18.
+// exponentials' unit are each 63 % busy (4 x 4096 tokens, 16/4 heads of 128, no mask), and two row tiles are what TMEM
+// and the registers hold.  Heads of 64 have half the products for the same exponentials: 28 % and 57 % (2 x 4096
+// causal tokens, 16 heads); under a cap 15 % and 30 %, issue slots 46 %, so there it is the length of a warp's way, a
+// polynomial of 9 instructions on a pair of scores in it, with two such warps per scheduler.  From a cold L2: 16384
+// causal tokens x 8 heads of 128, bf16 465 us (1.18 PFLOP/s; 417 us, 1.32, where K and V are in L2); 2 x 4096
+// causal x 32/8 heads 272 us (1.01); 8192 causal x 16 heads of 64, fp16 219 us (0.63), with a cap 426 us.  (The capped
+// instances without a bias spill 2 to 6 registers.)  Slower, 16384 x 16384 x 8 heads, PFLOP/s where this form had 1.21:
+// steps of 64 keys 0.72, two issuing threads 0.83, four softmax warpgroups 1.11, K and V released together 1.18.
 #include <cuda.h>
 
 #include "attention.cuh"

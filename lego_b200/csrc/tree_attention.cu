@@ -34,10 +34,13 @@
 // zeros in shared memory: a box past the cache reads as zeros, other rows are cleared by the
 // loading warp before it hands the tile on.
 //
-// Measured: 64 sequences of 1024 .. 8192 tokens x 32/8 heads of 128, bf16, one token 257 us (5.1 TB/s); 8 of 8192 ..
-// 65536 tokens 260 us (5.8, what a plain sum reads here: the difference is the change of sequence);
-// 2 x 131072 tokens x 64 rows with a bias 156 us (4.7); 8 x 16384 x 37 tokens of 2 heads with a cap 99 us, bound by
-// the cap's arithmetic.  Slower: scores and weights of one copy in registers (drafts 95 -> 104 us).
+// Measured, calls in turn: 64 sequences of 1024 .. 8192 tokens x 32/8 heads of 128, bf16, one token 257 us (5.1 TB/s);
+// 8 of 8192 .. 65536 tokens 260 us (5.8, what a plain sum reads here: the difference is the change of sequence and
+// the join, a launch of 8 us that starts when the last run has ended); 2 x 131072 tokens x 64 rows with a
+// bias 157 us (4.7).  8 x 16384 x 37 tokens of 2 heads with a cap 100 us: no unit is half busy (issue slots 39 %, FMA 18 %,
+// exponentials 16 %, memory 25 %); above 64 rows a warp takes 128 columns in four chunks, each read from TMEM, written
+// back and read again, and two warps per scheduler do not hide that.  Slower: scores and weights of one copy in
+// registers (drafts 95 -> 104 us).
 #include <cuda.h>
 
 #include "attention.cuh"
