@@ -311,3 +311,25 @@ def test_fp16_gradients_beside_queries_that_see_nothing():
     assert not got["dq"][:, :100].any()
     for n, at in (("dq", slice(100, 200)), ("dk", slice(0, 28)), ("dk", slice(0, 100)), ("dv", slice(0, 100))):
         assert times(got[n], exact[n], with_r[n], at) <= TILE, (n, at)
+
+
+def test_fp16_gradients_eighty_powers_of_two_apart():
+    """Two heads of one key head, whose first queries and keys have the type's smallest values and whose last its
+    largest: the factor on dK's sums falls by 2^80 within a head and cannot come back as far for the next one.  The
+    weights of a row are all alike, so the errors of dk's tokens are too: 64 independent values in each, a deviation
+    of 0.125 between two norms, and a limit of 2."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    n = lambda *s: torch.randn(*s, generator=g, device="cuda")   # noqa: E731
+    q, k = (n(1, 256, 2, 64) * 1e-6).half(), (n(1, 256, 1, 64) * 1e-6).half()
+    v, do = n(1, 256, 1, 64).sign(), n(1, 256, 2, 64).sign()
+    for x in (v, do):
+        x[:, :128] *= 6e-8
+        x[:, 128:] *= 6e4
+    v, do = v.half(), do.half()
+    got = run(q, k, v, do, True)
+    exact, with_r = model(q, k, v, do, True)
+    for name in ("dq", "dk", "dv"):
+        assert torch.isfinite(got[name]).all()
+    assert not got["dq"][:, :128].any()          # far below the type's range
+    for name, at in (("dq", slice(128, 256)), ("dk", slice(0, 128)), ("dk", slice(128, 256)), ("dv", slice(0, 256))):
+        assert times(got[name], exact[name], with_r[name], at) <= 2, (name, at)
